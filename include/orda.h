@@ -447,6 +447,56 @@ ORDA_API int orda_vocab_backward_device(OrdaContext* ctx, const OrdaDeviceMat* s
                                         const OrdaDeviceOutputs* out, void* stream, OrdaChunkPlan* plan_out,
                                         char* err, size_t err_len);
 
+/* Linear softmax cross entropy without a teacher: with z = hidden @ weight^T,
+ * lse = log sum_v e^{z_v} and label smoothing a,
+ *   nll  = (1 - a) (lse - z_label) + a (lse - mean_v z_v)     per live token
+ *   loss = sum nll (SUM), or divided by the count of live tokens, at least 1 (MEAN)
+ * and the gradients of the loss with respect to hidden and weight. A token
+ * whose label is ignore_index is not live: its nll, lse and grad_hidden row
+ * are 0 and what its hidden row holds is not used. The student term of
+ * `distillation_loss` (src/reference/cross_entropy.rs:20-74) on its own; the
+ * reference has no entry without a teacher.
+ *
+ * The logits are never kept in fp32. A call with gradients holds 16-bit logits
+ * (then logit gradients, in place) of a piece of the vocabulary, at most
+ * piece_bytes for all rows; columns beyond the first piece are computed a
+ * second time. A call without gradients keeps none.
+ *
+ * hidden [BT, H] and weight [V, H] as in orda_distillation_loss_device. The
+ * products take bf16 operands: gradients carry the rounding of the logit
+ * gradients to bf16 (relative L2 about 2e-3) whatever their type; losses come
+ * from fp32 sums of the fp32 products. Enqueued on `stream` without host
+ * synchronisation; labels out of range are reported by orda_context_check.
+ * Under stream capture the context must hold the workspace already (make the
+ * same call once before); the graph may be replayed until the context is
+ * destroyed. */
+typedef struct OrdaLinearCeOptions {
+  int64_t ignore_index;
+  float label_smoothing;     /* in [0, 1] */
+  OrdaReduction reduction;
+  int64_t global_non_ignore; /* > 0: use this token count as the mean denominator */
+  size_t piece_bytes;        /* bytes of 16-bit logits kept at once; 0 = 4 GiB. Pieces are multiples of 512
+                                columns, so one holds at least 1 KiB for each row. Smaller pieces are
+                                taken when the device memory is short. */
+} OrdaLinearCeOptions;
+typedef struct OrdaLinearCeOutputs {
+  float* loss;        /* required device float[1] */
+  float* nll;         /* optional [BT] */
+  float* lse;         /* optional [BT] */
+  void* grad_hidden;  /* optional [BT, H] */
+  size_t ld_grad_hidden;
+  void* grad_weight;  /* optional [V, H] */
+  size_t ld_grad_weight;
+  OrdaDType grad_hidden_dtype; /* bf16 or f32 */
+  OrdaDType grad_weight_dtype;
+} OrdaLinearCeOutputs;
+/* ignore_index -100, no smoothing, mean reduction. */
+ORDA_API void orda_linear_ce_options_default(OrdaLinearCeOptions* out);
+ORDA_API int orda_linear_cross_entropy_device(OrdaContext* ctx, const OrdaDeviceMat* hidden,
+                                              const OrdaDeviceMat* weight, const int64_t* labels, size_t bt,
+                                              const OrdaLinearCeOptions* opts, const OrdaLinearCeOutputs* out,
+                                              void* stream, char* err, size_t err_len);
+
 /* Fused grad_W reduce-scatter for row-sharded runs on the GPUs of one node
  * (up to 8 ranks, one process per GPU). There is no counterpart in the
  * reference, which runs on one device; for data-parallel callers that

@@ -114,6 +114,24 @@ const OrdaFieldLayout kLayout[] = {
     ORDA_FIELD(OrdaVocabShard, scatter_grad_hidden),
     ORDA_FIELD(OrdaVocabShard, pad),
 
+    ORDA_STRUCT(OrdaLinearCeOptions),
+    ORDA_FIELD(OrdaLinearCeOptions, ignore_index),
+    ORDA_FIELD(OrdaLinearCeOptions, label_smoothing),
+    ORDA_FIELD(OrdaLinearCeOptions, reduction),
+    ORDA_FIELD(OrdaLinearCeOptions, global_non_ignore),
+    ORDA_FIELD(OrdaLinearCeOptions, piece_bytes),
+
+    ORDA_STRUCT(OrdaLinearCeOutputs),
+    ORDA_FIELD(OrdaLinearCeOutputs, loss),
+    ORDA_FIELD(OrdaLinearCeOutputs, nll),
+    ORDA_FIELD(OrdaLinearCeOutputs, lse),
+    ORDA_FIELD(OrdaLinearCeOutputs, grad_hidden),
+    ORDA_FIELD(OrdaLinearCeOutputs, ld_grad_hidden),
+    ORDA_FIELD(OrdaLinearCeOutputs, grad_weight),
+    ORDA_FIELD(OrdaLinearCeOutputs, ld_grad_weight),
+    ORDA_FIELD(OrdaLinearCeOutputs, grad_hidden_dtype),
+    ORDA_FIELD(OrdaLinearCeOutputs, grad_weight_dtype),
+
     ORDA_STRUCT(OrdaIpcHandle),
     ORDA_FIELD(OrdaIpcHandle, bytes),
 

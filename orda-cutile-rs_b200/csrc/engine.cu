@@ -47,10 +47,16 @@
 struct OrdaContext {
   int device = 0;
   int num_sms = 148;
-  int* d_words = nullptr;  // [0] status, [1] n_non_ignore
+  // [0] status, [1] n_non_ignore, [2] finished blocks of the cross entropy's
+  // combining kernel, [3] token ids out of range (kept until it is reported)
+  int* d_words = nullptr;
   float* d_mean_scale = nullptr;
   void* ws = nullptr;
   size_t ws_bytes = 0;
+  // A graph captured with this workspace replays with its address: once that
+  // has happened a workspace that is outgrown lives on until the context ends.
+  bool ws_in_graph = false;
+  std::vector<void*> ws_retired;
   void* stage = nullptr;
   size_t stage_bytes = 0;
   int inject_fail = 0;
@@ -184,9 +190,11 @@ cudaError_t ensure_ws(OrdaContext* ctx, size_t bytes) {
   }
   if (ctx->ws_bytes >= bytes) return cudaSuccess;
   if (ctx->ws) {
-    cudaFree(ctx->ws);
+    if (ctx->ws_in_graph) ctx->ws_retired.push_back(ctx->ws);
+    else cudaFree(ctx->ws);
     ctx->ws = nullptr;
     ctx->ws_bytes = 0;
+    ctx->ws_in_graph = false;
   }
   void* p = nullptr;
   cudaError_t e = cudaMalloc(&p, bytes);
@@ -907,6 +915,295 @@ int run_device(OrdaContext* ctx, const DevInputs& in, const OrdaLossOptions& o, 
   return ORDA_OK;
 }
 
+// ------------------------------------------------- linear cross entropy
+// Makes the context's device current and the caller's device current again.
+struct DeviceScope {
+  int prev = -1, dev;
+  explicit DeviceScope(int d) : dev(d) {
+    if (cudaGetDevice(&prev) != cudaSuccess) prev = -1;
+    if (prev != dev) cudaSetDevice(dev);
+  }
+  ~DeviceScope() {
+    if (prev >= 0 && prev != dev) cudaSetDevice(prev);
+  }
+};
+
+// The workspace for a call on `st`. Under stream capture nothing may be
+// allocated, and the graph keeps the workspace's address.
+int call_ws(OrdaContext* ctx, size_t bytes, cudaStream_t st, bool* capturing, char* err, size_t len) {
+  cudaStreamCaptureStatus cap = cudaStreamCaptureStatusNone;
+  cudaError_t e = cudaStreamIsCapturing(st, &cap);
+  if (e != cudaSuccess) return cuda_fail(e, "cudaStreamIsCapturing", err, len);
+  *capturing = cap != cudaStreamCaptureStatusNone;
+  if (*capturing) {
+    if (ctx->ws_bytes < bytes) {
+      set_error(err, len, "a captured call cannot allocate its %zu bytes of workspace: make the same call once "
+                          "before the capture", bytes);
+      return ORDA_ERR_OOM;
+    }
+    ctx->ws_in_graph = true;
+    return ORDA_OK;
+  }
+  if (ensure_ws(ctx, bytes) != cudaSuccess) {
+    set_error(err, len, "device workspace allocation of %zu bytes failed", bytes);
+    return ORDA_ERR_OOM;
+  }
+  return ORDA_OK;
+}
+
+// Bytes of 16-bit logits that a call with gradients keeps by default: the
+// whole batch of the largest benchmark shape (8192 rows x 131072) is half of it.
+constexpr size_t kCePieceBytes = size_t{4} << 30;
+constexpr size_t kCePieceCols = 512;  // pieces are whole 512-column tiles
+
+struct CeLayout {
+  size_t h_clean = 0, ref = 0, rec = 0, sx = 0, row_const = 0, nll = 0, piece = 0, dgrad = 0, total = 0;
+  size_t cols = 0;      // vocabulary columns of one piece
+  size_t n_parts = 0, rec_ld = 0, ld_clean = 0, ld_piece = 0, ld_dgrad = 0, slab_rows = 0;
+  int slabs = 1;
+  bool dgrad_direct = false;  // the dgrad product writes the fp32 output itself
+};
+
+// K slabs of the dgrad product: with fewer 256 x 256 tiles than CTA pairs its
+// long K (the vocabulary) is cut so that every pair has a tile, each at least
+// eight K blocks deep (the depth of the ring and a little more); the slabs'
+// partial sums are added in order afterwards. One token at H = 4096, V =
+// 131072: 16 tiles would leave 58 of 74 pairs idle while all of W is read.
+int ce_slabs(size_t rows, size_t h, size_t cols, int num_sms) {
+  const size_t pairs = static_cast<size_t>(std::max(1, num_sms / 2));
+  const size_t tiles = ceil_div(rows, 256) * ceil_div(h, 256);
+  const size_t k_blocks = ceil_div(cols, 64);
+  if (tiles >= pairs) return 1;
+  return static_cast<int>(std::max<size_t>(1, std::min(pairs / tiles, k_blocks / 8)));
+}
+
+CeLayout ce_layout(size_t bt, size_t h, size_t v, size_t cols, bool smooth, const OrdaLinearCeOutputs& o,
+                   int num_sms) {
+  CeLayout L;
+  const bool grads = o.grad_hidden || o.grad_weight;
+  L.cols = cols;
+  L.n_parts = ceil_div(v, kCePartCols);
+  L.rec_ld = round_up(bt, 32);
+  L.ld_clean = round_up(h, 8);
+  L.ld_piece = round_up(cols, 8);
+  size_t off = 0;
+  auto take = [&](size_t bytes) {
+    const size_t at = off;
+    off = round_up(off + bytes, 256);
+    return at;
+  };
+  L.h_clean = take(bt * L.ld_clean * 2);
+  L.ref = take(bt * sizeof(float2));
+  L.rec = take(L.n_parts * L.rec_ld * sizeof(float2));
+  L.sx = take(smooth ? L.n_parts * L.rec_ld * sizeof(float) : 0);
+  L.row_const = take(bt * sizeof(float4));
+  L.nll = take(o.nll ? 0 : bt * sizeof(float));
+  L.piece = take(grads ? bt * L.ld_piece * 2 : 0);
+  if (o.grad_hidden) {
+    L.slabs = ce_slabs(bt, h, cols, num_sms);
+    L.slab_rows = round_up(bt, 32);
+    L.ld_dgrad = round_up(h, 4);
+    L.dgrad_direct = L.slabs == 1 && o.grad_hidden_dtype == ORDA_DTYPE_F32;
+    L.dgrad = take(L.dgrad_direct ? 0 : static_cast<size_t>(L.slabs) * L.slab_rows * L.ld_dgrad * 4);
+  }
+  L.total = off;
+  return L;
+}
+
+// One call: label pass, logits product (the statistics of every piece but
+// one, then that piece with its 16-bit logits kept), losses, and for each
+// piece its logit gradients (from the kept logits, or by the logits product
+// again) and the two gradient products. No [BT, V] buffer exists unless it fits
+// piece_bytes; each further piece costs its share of one more product.
+int run_linear_ce(OrdaContext* ctx, const OrdaDeviceMat& hm, const OrdaDeviceMat& wm, const int64_t* labels, size_t bt,
+                  const OrdaLinearCeOptions& o, const OrdaLinearCeOutputs& out, cudaStream_t st, char* err,
+                  size_t len) {
+  const size_t h = hm.cols, v = wm.rows;
+  const bool grads = out.grad_hidden || out.grad_weight;
+  const bool smooth = o.label_smoothing > 0.0f;
+  ctx->vocab_ready = false;  // the workspace no longer holds a vocabulary forward phase
+
+  // the piece: all of the vocabulary if that fits, else even pieces of whole tiles
+  const size_t limit = o.piece_bytes ? o.piece_bytes : kCePieceBytes;
+  size_t pieces = 1, cols = v;
+  if (grads) {
+    const size_t fit = std::max(kCePieceCols, limit / (2 * bt) / kCePieceCols * kCePieceCols);
+    if (fit < v) {
+      pieces = ceil_div(v, fit);
+      cols = round_up(ceil_div(v, pieces), kCePieceCols);
+    }
+  }
+  CeLayout L;
+  bool capturing = false;
+  while (true) {
+    pieces = ceil_div(v, cols);
+    L = ce_layout(bt, h, v, cols, smooth, out, ctx->num_sms);
+    const int rc = call_ws(ctx, L.total, st, &capturing, err, len);
+    if (rc == ORDA_OK) break;
+    // smaller pieces where the memory is short, as the chunk ladder does
+    if (rc != ORDA_ERR_OOM || capturing || !grads || cols <= kCePieceCols) return rc;
+    cols = round_up(ceil_div(cols, 2), kCePieceCols);
+  }
+
+  uint8_t* ws = static_cast<uint8_t*>(ctx->ws);
+  CeArgs a;
+  a.h = hm.data;
+  a.ldh = static_cast<long long>(hm.ld);
+  a.w = wm.data;
+  a.ldw = static_cast<long long>(wm.ld);
+  a.bt = static_cast<long long>(bt);
+  a.hd = static_cast<long long>(h);
+  a.v = static_cast<long long>(v);
+  a.labels = labels;
+  a.ignore_index = o.ignore_index;
+  a.alpha = o.label_smoothing;
+  a.reduction_sum = o.reduction == ORDA_REDUCTION_SUM;
+  a.denom_override = o.global_non_ignore;
+  a.h_clean = reinterpret_cast<uint16_t*>(ws + L.h_clean);
+  a.ld_clean = static_cast<long long>(L.ld_clean);
+  a.ref = reinterpret_cast<float2*>(ws + L.ref);
+  a.rec = reinterpret_cast<float2*>(ws + L.rec);
+  a.sx = smooth ? reinterpret_cast<float*>(ws + L.sx) : nullptr;
+  a.rec_ld = static_cast<long long>(L.rec_ld);
+  a.n_parts = static_cast<int>(L.n_parts);
+  a.row_const = reinterpret_cast<float4*>(ws + L.row_const);
+  a.nll = out.nll ? out.nll : reinterpret_cast<float*>(ws + L.nll);
+  a.lse = out.lse;
+  a.loss = out.loss;
+  a.status = ctx->d_words;
+  a.count = ctx->d_words + 1;
+  a.done = ctx->d_words + 2;
+  uint16_t* piece = grads ? reinterpret_cast<uint16_t*>(ws + L.piece) : nullptr;
+
+  cudaError_t e;
+  const char* why = nullptr;
+  {
+    Phase ph(ctx, 5, st);
+    ph.launched();
+    if ((e = cudaMemsetAsync(ctx->d_words, 0, 3 * sizeof(int), st)) != cudaSuccess)
+      return cuda_fail(e, "memset", err, len);
+    launch_ce_prep(a, st);
+    if ((e = cudaGetLastError()) != cudaSuccess) return cuda_fail(e, "label pass", err, len);
+  }
+  const MatRef hmat{a.h_clean, a.bt, a.hd, a.ld_clean};
+  // logits of vocabulary columns [v0, v0 + n): statistics (and kept 16-bit logits), or the gradients
+  auto logits = [&](size_t v0, size_t n, Epi epi, uint16_t* keep) -> int {
+    Phase ph(ctx, 0, st);
+    int nl = 0;
+    GemmDesc gd;
+    gd.a[0] = hmat;
+    gd.b[0] = MatRef{static_cast<const uint16_t*>(wm.data) + v0 * wm.ld, static_cast<long long>(n), a.hd, a.ldw};
+    gd.k_seg[0] = a.hd;
+    gd.M = a.bt;
+    gd.N = static_cast<long long>(n);
+    gd.epi = epi;
+    gd.status = ctx->d_words;
+    gd.args.out16 = keep;
+    gd.args.ld16 = static_cast<long long>(L.ld_piece);
+    gd.args.ce_v0 = static_cast<long long>(v0);
+    gd.args.ce_ref = a.ref;
+    gd.args.ce_rec = a.rec + v0 / kCePartCols * L.rec_ld;
+    gd.args.ce_sx = smooth ? a.sx + v0 / kCePartCols * L.rec_ld : nullptr;
+    gd.args.ce_rec_ld = a.rec_ld;
+    gd.args.ce_const = a.row_const;
+    gd.demote_kept = ctx->l2_set;
+    gd.launches = &nl;
+    if ((e = gemm_launch(gd, ctx->num_sms, st, &why)) != cudaSuccess)
+      return cuda_fail(e, why ? why : "logits GEMM", err, len);
+    ph.launched(nl);
+    return ORDA_OK;
+  };
+  if (pieces > 1) {
+    if (int rc = logits(cols, v - cols, Epi::CeStats, nullptr)) return rc;
+  }
+  if (int rc = logits(0, std::min(cols, v), Epi::CeStats, piece)) return rc;
+  {
+    Phase ph(ctx, 1, st);
+    ph.launched();
+    launch_ce_combine(a, st);
+    if ((e = cudaGetLastError()) != cudaSuccess) return cuda_fail(e, "row kernels", err, len);
+  }
+  for (size_t v0 = 0; grads && v0 < v; v0 += cols) {
+    const size_t n = std::min(cols, v - v0);
+    if (v0 == 0) {
+      Phase ph(ctx, 1, st);
+      ph.launched();
+      launch_ce_rewrite(a, piece, static_cast<long long>(L.ld_piece), 0, static_cast<long long>(n), st);
+      if ((e = cudaGetLastError()) != cudaSuccess) return cuda_fail(e, "row kernels", err, len);
+    } else if (int rc = logits(v0, n, Epi::CeGrad, piece)) {
+      return rc;
+    }
+    const MatRef dl{piece, a.bt, static_cast<long long>(n), static_cast<long long>(L.ld_piece)};
+    if (out.grad_hidden) {
+      Phase ph(ctx, 2, st);
+      int nl = 0;
+      GemmDesc gd;
+      gd.a[0] = dl;
+      gd.b_mn_major = true;
+      gd.b[0] = MatRef{static_cast<const uint16_t*>(wm.data) + v0 * wm.ld, static_cast<long long>(n), a.hd, a.ldw};
+      gd.k_seg[0] = static_cast<long long>(n);
+      gd.M = a.bt;
+      gd.N = a.hd;
+      gd.raster_n_fastest = true;
+      gd.status = ctx->d_words;
+      gd.args.beta = v0 > 0 ? 1.0f : 0.0f;
+      if (L.dgrad_direct) {
+        gd.args.out0 = static_cast<float*>(out.grad_hidden);
+        gd.args.ld0 = static_cast<long long>(out.ld_grad_hidden);
+      } else {
+        gd.args.out0 = reinterpret_cast<float*>(ws + L.dgrad);
+        gd.args.ld0 = static_cast<long long>(L.ld_dgrad);
+        // the last piece may be narrower than its slabs are many: every slab
+        // that earlier pieces wrote stays in the sum
+        gd.args.slabs = std::min<int>(L.slabs, static_cast<int>(ceil_div(n, 64)));
+        gd.args.slab_rows = static_cast<long long>(L.slab_rows);
+      }
+      gd.demote_kept = ctx->l2_set;
+      gd.launches = &nl;
+      if ((e = gemm_launch(gd, ctx->num_sms, st, &why)) != cudaSuccess)
+        return cuda_fail(e, why ? why : "dgrad GEMM", err, len);
+      ph.launched(nl);
+    }
+    if (out.grad_weight) {
+      Phase ph(ctx, 3, st);
+      int nl = 0;
+      GemmDesc gd;
+      gd.a_mn_major = true;
+      gd.b_mn_major = true;
+      gd.a[0] = dl;
+      gd.b[0] = hmat;
+      gd.k_seg[0] = a.bt;
+      gd.M = static_cast<long long>(n);
+      gd.N = a.hd;
+      gd.raster_n_fastest = true;
+      gd.status = ctx->d_words;
+      if (out.grad_weight_dtype == ORDA_DTYPE_BF16) {
+        gd.epi = Epi::StoreBf16;
+        gd.args.out16 = static_cast<uint16_t*>(out.grad_weight) + v0 * out.ld_grad_weight;
+        gd.args.ld16 = static_cast<long long>(out.ld_grad_weight);
+      } else {
+        gd.args.out0 = static_cast<float*>(out.grad_weight) + v0 * out.ld_grad_weight;
+        gd.args.ld0 = static_cast<long long>(out.ld_grad_weight);
+      }
+      gd.demote_kept = ctx->l2_set;
+      gd.launches = &nl;
+      if ((e = gemm_launch(gd, ctx->num_sms, st, &why)) != cudaSuccess)
+        return cuda_fail(e, why ? why : "wgrad GEMM", err, len);
+      ph.launched(nl);
+    }
+  }
+  if (out.grad_hidden && !L.dgrad_direct) {
+    Phase ph(ctx, 2, st);
+    ph.launched();
+    launch_slab_sum(reinterpret_cast<const float*>(ws + L.dgrad), L.slabs, static_cast<long long>(L.slab_rows),
+                    static_cast<long long>(L.ld_dgrad), a.bt, a.hd, out.grad_hidden,
+                    static_cast<long long>(out.ld_grad_hidden), out.grad_hidden_dtype == ORDA_DTYPE_BF16, st);
+    if ((e = cudaGetLastError()) != cudaSuccess) return cuda_fail(e, "dgrad sum", err, len);
+  }
+  ctx->last_stream = st;
+  return ORDA_OK;
+}
+
 // --------------------------------------------------------------- helpers
 bool device_is_sm100(int dev) {
   cudaDeviceProp p;
@@ -1253,6 +1550,7 @@ void orda_context_destroy(OrdaContext* ctx) {
   if (ctx->l2_set) cudaDeviceSetLimit(cudaLimitPersistingL2CacheSize, ctx->l2_prev);
   release_slots(ctx);
   cudaFree(ctx->ws);
+  for (void* p : ctx->ws_retired) cudaFree(p);
   cudaFree(ctx->stage);
   cudaFree(ctx->wire_local);
   cudaFree(ctx->d_words);
@@ -1408,6 +1706,75 @@ int orda_vocab_backward_device(OrdaContext* ctx, const OrdaDeviceMat* student_hi
   vc.scatter_hidden = vs->scatter_grad_hidden;
   vc.partials_in = all_partials;
   return run_device(ctx, in, *opts, *out, nullptr, static_cast<cudaStream_t>(stream), plan_out, err, err_len, &vc);
+}
+
+void orda_linear_ce_options_default(OrdaLinearCeOptions* out) {
+  if (!out) return;
+  std::memset(out, 0, sizeof *out);
+  out->ignore_index = -100;
+  out->reduction = ORDA_REDUCTION_MEAN;
+}
+
+// A gradient output of the linear cross entropy: any alignment of its element
+// type (an output that TMA cannot address is stored from registers).
+static bool grad_out_ok(const void* p, size_t ld, OrdaDType dt, size_t cols) {
+  if (!p) return true;
+  if (dt != ORDA_DTYPE_BF16 && dt != ORDA_DTYPE_F32) return false;
+  return ld >= cols && reinterpret_cast<uintptr_t>(p) % (dt == ORDA_DTYPE_BF16 ? 2 : 4) == 0;
+}
+
+int orda_linear_cross_entropy_device(OrdaContext* ctx, const OrdaDeviceMat* hidden, const OrdaDeviceMat* weight,
+                                     const int64_t* labels, size_t bt, const OrdaLinearCeOptions* opts,
+                                     const OrdaLinearCeOutputs* out, void* stream, char* err, size_t err_len) {
+  if (!ctx || !hidden || !weight || !labels || !opts || !out) {
+    set_error(err, err_len, "null argument");
+    return ORDA_ERR_INVALID;
+  }
+  if (hidden->rows == 0) {
+    set_error(err, err_len, "BT must be > 0");
+    return ORDA_ERR_INVALID;
+  }
+  if (weight->rows == 0 || hidden->cols == 0 || weight->cols != hidden->cols) {
+    set_error(err, err_len, "weight must be (V, %zu), got (%zu, %zu)", hidden->cols, weight->rows, weight->cols);
+    return ORDA_ERR_INVALID;
+  }
+  if (bt != hidden->rows) {
+    set_error(err, err_len, "labels must have BT=%zu entries, got %zu", hidden->rows, bt);
+    return ORDA_ERR_INVALID;
+  }
+  constexpr size_t kMax = size_t{1} << 30;  // tile coordinates are 32-bit
+  if (bt > kMax || weight->rows > kMax || hidden->cols > kMax) {
+    set_error(err, err_len, "BT, V and H must be at most 2^30, got %zu, %zu and %zu", bt, weight->rows, hidden->cols);
+    return ORDA_ERR_INVALID;
+  }
+  if (!(opts->label_smoothing >= 0.0f && opts->label_smoothing <= 1.0f)) {
+    set_error(err, err_len, "label_smoothing must be in [0,1], got %s", fmt_f32(opts->label_smoothing).c_str());
+    return ORDA_ERR_INVALID;
+  }
+  if (opts->reduction != ORDA_REDUCTION_MEAN && opts->reduction != ORDA_REDUCTION_SUM) {
+    set_error(err, err_len, "unknown reduction %d", static_cast<int>(opts->reduction));
+    return ORDA_ERR_INVALID;
+  }
+  if (opts->global_non_ignore < 0) {
+    set_error(err, err_len, "global_non_ignore must be >= 0, got %lld", static_cast<long long>(opts->global_non_ignore));
+    return ORDA_ERR_INVALID;
+  }
+  if (!dev_mat_ok(*hidden, true) || !dev_mat_ok(*weight, true)) {
+    set_error(err, err_len, "hidden and weight must be bf16, 16-byte aligned, with ld*2 a multiple of 16");
+    return ORDA_ERR_INVALID;
+  }
+  if (!out->loss) {
+    set_error(err, err_len, "loss output is required");
+    return ORDA_ERR_INVALID;
+  }
+  if (!grad_out_ok(out->grad_hidden, out->ld_grad_hidden, out->grad_hidden_dtype, hidden->cols) ||
+      !grad_out_ok(out->grad_weight, out->ld_grad_weight, out->grad_weight_dtype, hidden->cols)) {
+    set_error(err, err_len, "gradient outputs must be bf16 or f32 with ld >= H=%zu", hidden->cols);
+    return ORDA_ERR_INVALID;
+  }
+  std::lock_guard<std::mutex> lock(ctx->mu);
+  DeviceScope dev(ctx->device);
+  return run_linear_ce(ctx, *hidden, *weight, labels, bt, *opts, *out, static_cast<cudaStream_t>(stream), err, err_len);
 }
 
 int orda_quantize_grad_w_device(OrdaContext* ctx, float* grad_w, size_t v, size_t h, size_t ld, const int64_t* labels,

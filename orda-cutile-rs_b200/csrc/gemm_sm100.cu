@@ -23,7 +23,8 @@
 //   logits = h @ W^T      (A K-major, B K-major)
 //   grad_h = dlogits @ W  (A K-major, B MN-major)
 //   grad_W = dlogits^T @ h (A MN-major, B MN-major)
-// Epilogues: plain scaled store (or TMA reduce-add), or the logits epilogue
+// Epilogues: plain scaled store (or TMA reduce-add), bf16 store, stores of K
+// slabs, the two epilogues of the linear cross entropy, or the logits epilogue
 // that writes fp32 logits and per-(row, 128-column part) online-softmax
 // statistics (max, sum exp(x-m), sum exp((x-m)/T), sum x) from the fp32
 // accumulators, so the loss needs no separate reduction pass over the logits.
@@ -108,6 +109,8 @@ struct KParams {
   // halves whose partial sums are reduce-added into a zeroed output. An
   // unsplit tile sums K in one order whatever the tile shape; a split tile
   // sums each half in that order and adds the two.
+  // With K slabs every tile is split into nsplit = slabs K parts, each stored
+  // in an output of its own.
   int full_tiles, rem_tiles, nsplit, num_items;
   int allow_split;  // host side: the output may take split tiles (plain TMA store, one K segment)
   EpiArgs e;
@@ -334,6 +337,172 @@ __device__ __forceinline__ void stage_and_scatter(uint8_t* buf, int lane, const 
   }
 }
 
+// Epilogue codes of the kernel template (0 is the plain store, 16..19 the
+// logits epilogue).
+constexpr int kEpiStoreBf16 = 32;
+constexpr int kEpiStoreSlab = 33;
+constexpr int kEpiCeStats = 64;  // + 1: keep the 16-bit logits, + 2: sums of the logits
+constexpr int kEpiCeGrad = 68;
+
+// Two fp32 values as a bf16 pair (round to nearest even), the first in the low half.
+__device__ __forceinline__ uint32_t pack_bf16x2(float a, float b) {
+  const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+
+// Stages this row's 32 16-bit values (16 packed words) as half `side` of a
+// 64-column row (128 bytes, 128-byte swizzle); after side 1 the 32 x 64 block
+// goes out in one TMA store, clipped at the tensor bounds. All lanes call it
+// for side 0 and then side 1.
+__device__ __forceinline__ void stage16(uint8_t* buf, int lane, int side, const uint32_t (&w)[16],
+                                        const CUtensorMap* map, int x, int y, bool store, uint64_t policy) {
+  if (side == 0) {
+    if (lane == 0) bulk_wait_read_all();
+    __syncwarp();
+  }
+#pragma unroll
+  for (int k = 0; k < 4; ++k)
+    *reinterpret_cast<uint4*>(buf + lane * 128 + (((side * 4 + k) ^ (lane & 7)) << 4)) =
+        make_uint4(w[4 * k], w[4 * k + 1], w[4 * k + 2], w[4 * k + 3]);
+  if (side == 1) {
+    fence_proxy_async_smem();
+    __syncwarp();
+    if (lane == 0 && store) {
+      tma_store_2d_hint(map, buf, x, y, policy);
+      bulk_commit();
+    }
+  }
+}
+
+// One 32-column chunk of one row of the linear cross entropy's first pass:
+// t = log2(e^(x - reference)) as one FMA, the sum of 2^t over the columns
+// other than the label's (MASK: the chunk has a label or ends the vocabulary),
+// the sum of x, and t as 16-bit fixed point. The fixed point comes from the
+// mantissa of t * 512 + (2^23 + 2^15): one FMA and half a byte permute per
+// element, where a conversion instruction would share the SFU's pipe with ex2.
+template <bool MASK, bool STORE, bool SX>
+__device__ __forceinline__ void ce_stats_chunk(const uint32_t (&r)[32], float ref2, int lab, int nvalid, float& d,
+                                               float& sx, uint32_t (&q)[16]) {
+  float a[4] = {0.f, 0.f, 0.f, 0.f}, ax[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+  for (int j = 0; j < 32; ++j) {
+    const float x = __uint_as_float(r[j]);
+    const float t = fmaf(x, LOG2E, -ref2);
+    float e = fast_exp2(t);
+    if (MASK) e = (j < nvalid && j != lab) ? e : 0.0f;
+    a[j & 3] += e;
+    if (SX) ax[j & 3] += (!MASK || j < nvalid) ? x : 0.0f;
+    if (STORE) {
+      const uint32_t u = __float_as_uint(fmaf(fmaxf(t, kCeQLow), kCeQScale, 8388608.0f + kCeQBias));
+      if (j & 1) q[j >> 1] = __byte_perm(q[j >> 1], u, 0x5410);
+      else q[j >> 1] = u;
+    }
+  }
+  d += (a[0] + a[1]) + (a[2] + a[3]);
+  if (SX) sx += (ax[0] + ax[1]) + (ax[2] + ax[3]);
+}
+
+// Linear cross entropy, one warp's 32 rows x 128 columns of a tile.
+// CeStats: one record (sum of 2^t, reference) per row and part, and (+ 1) the
+// 16-bit t of the part. The sum is taken against the row's reference logit;
+// only when it leaves the range that the fixed point resolves (every logit 27
+// nats below the reference, or one 43 nats above it) the part is done again
+// against its own maximum, from TMEM.
+// CeGrad: the logit gradients 2^(x log2 e + c.x) - c.z, c.w at the label.
+template <int EPI, typename Release>
+__device__ __forceinline__ void ce_epilogue(const KParams& p, const CUtensorMap* map, uint8_t* buf, int lane,
+                                            uint32_t t_row, int colh, int row0, long long grow, bool row_ok, int part,
+                                            const float4& row_c, uint64_t pol_c, const Release& release_tmem) {
+  constexpr bool GRAD = EPI == kEpiCeGrad;
+  constexpr bool STORE = GRAD || (EPI & 1) != 0;
+  constexpr bool SX = !GRAD && (EPI & 2) != 0;
+  if (colh >= p.N) {  // the second half of the last tile may hold no column
+    release_tmem();
+    return;
+  }
+  const long long lab_rel = static_cast<long long>(__float_as_int(row_c.y)) - p.e.ce_v0 - colh;
+  const int lab = lab_rel >= 0 && lab_rel < kCePartCols ? static_cast<int>(lab_rel) : -1;
+  float d = 0.f, sx = 0.f;
+  float ref2 = row_c.x;
+  auto chunk = [&](int c, const uint32_t(&r)[32]) {
+    const int nvalid = p.N - (colh + c * 32);
+    const int lc = lab - c * 32;
+    const bool has_label = __any_sync(0xffffffffu, lc >= 0 && lc < 32);
+    uint32_t q[16];
+    if constexpr (GRAD) {
+#pragma unroll
+      for (int j = 0; j < 16; ++j) {
+        float v0 = fast_exp2(fmaf(__uint_as_float(r[2 * j]), LOG2E, row_c.x)) - row_c.z;
+        float v1 = fast_exp2(fmaf(__uint_as_float(r[2 * j + 1]), LOG2E, row_c.x)) - row_c.z;
+        if (has_label) {
+          if (lc == 2 * j) v0 = row_c.w;
+          if (lc == 2 * j + 1) v1 = row_c.w;
+        }
+        q[j] = pack_bf16x2(v0, v1);
+      }
+    } else if (has_label || nvalid < 32) {
+      ce_stats_chunk<true, STORE, SX>(r, ref2, lc, nvalid, d, sx, q);
+    } else {
+      ce_stats_chunk<false, STORE, SX>(r, ref2, lc, 32, d, sx, q);
+    }
+    if constexpr (STORE) {
+      const int x = colh + (c & ~1) * 32;
+      stage16(buf, lane, c & 1, q, map, x, row0, row0 < p.M && x < p.N, pol_c);
+    }
+  };
+  uint32_t ra[32], rb[32];
+  tmem_ld_32x32b_x32(t_row, ra);
+  tmem_ld_wait();
+  tmem_ld_32x32b_x32(t_row + 32, rb);
+  chunk(0, ra);
+  tmem_ld_wait();
+  tmem_ld_32x32b_x32(t_row + 64, ra);
+  chunk(1, rb);
+  tmem_ld_wait();
+  tmem_ld_32x32b_x32(t_row + 96, rb);
+  chunk(2, ra);
+  tmem_ld_wait();
+  if constexpr (GRAD) {
+    release_tmem();
+    chunk(3, rb);
+  } else {
+    chunk(3, rb);
+    const bool out_of_range = !(d >= kCeSumLow && d < kCeSumHigh);  // NaN too
+    if (__any_sync(0xffffffffu, out_of_range)) {
+      float m = -INFINITY;
+#pragma unroll 1
+      for (int c = 0; c < 4; ++c) {
+        tmem_ld_32x32b_x32(t_row + c * 32, ra);
+        tmem_ld_wait();
+        const int nvalid = p.N - (colh + c * 32);
+#pragma unroll
+        for (int j = 0; j < 32; ++j)
+          if (j < nvalid && j != lab - c * 32) m = fmaxf(m, __uint_as_float(ra[j]));
+      }
+      __syncwarp();
+      // a part of nothing, or of logits near the type's lowest value, keeps the row's reference
+      if (out_of_range && m * LOG2E > -INFINITY) ref2 = m * LOG2E;
+      d = 0.f;
+      sx = 0.f;
+      // the first stores of this part are complete before it is written again
+      if (STORE && lane == 0) bulk_wait_all();
+      __syncwarp();
+#pragma unroll 1
+      for (int c = 0; c < 4; ++c) {
+        tmem_ld_32x32b_x32(t_row + c * 32, ra);
+        tmem_ld_wait();
+        chunk(c, ra);
+      }
+    }
+    release_tmem();
+    if (row_ok && colh < p.N) {
+      const long long ri = static_cast<long long>(part) * p.e.ce_rec_ld + grow;
+      p.e.ce_rec[ri] = make_float2(d, ref2);
+      if (SX) p.e.ce_sx[ri] = sx;
+    }
+  }
+}
+
 // ------------------------------------------------------------------ kernel
 
 template <int CG, bool A_MN, bool B_MN, int EPI, bool WIDE>
@@ -342,7 +511,8 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
                 const __grid_constant__ CUtensorMap mapB0, const __grid_constant__ CUtensorMap mapB1,
                 const __grid_constant__ CUtensorMap mapC, const __grid_constant__ KParams p) {
   using T = TileCfg<CG, WIDE>;
-  static_assert(!WIDE || EPI == static_cast<int>(Epi::Store), "wide tiles take the store epilogue");
+  static_assert(!WIDE || EPI == static_cast<int>(Epi::Store) || EPI == kEpiStoreBf16,
+                "wide tiles take the store epilogues");
   constexpr bool PAIR = CG == 2;
   extern __shared__ uint8_t smem_raw[];
   // Same static layout in both CTAs of a pair: the MMA reads the peer's
@@ -537,10 +707,19 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
       // a K half of a split tile adds its partial sum into the zeroed output
       const bool split = w >= p.full_tiles && p.nsplit > 1;
       tile_coords(p, tile, mb, nb);
-      if (!mbar_wait<PAIR>(&tfull[acc], acc_phase, p.status, DEV_TIMEOUT_EPILOGUE)) break;
-      tc_fence_after();
       const long long grow = static_cast<long long>(mb) * T::TILE_M + row_in_tile;
       const bool row_ok = grow < p.M;
+      // this row's constants, in flight while the tile's products finish
+      float4 row_c = make_float4(0.f, 0.f, 0.f, 0.f);
+      if constexpr (EPI == kEpiCeGrad) {
+        if (row_ok) row_c = p.e.ce_const[grow];
+      } else if constexpr (EPI >= kEpiCeStats) {
+        const float2 rr = row_ok ? p.e.ce_ref[grow] : make_float2(0.f, __int_as_float(-1));
+        row_c.x = rr.x;
+        row_c.y = rr.y;
+      }
+      if (!mbar_wait<PAIR>(&tfull[acc], acc_phase, p.status, DEV_TIMEOUT_EPILOGUE)) break;
+      tc_fence_after();
       // this warp's half of the tile's columns: TMEM column j holds tile column j
       const uint32_t t_row = tmem_base + (static_cast<uint32_t>(quad * 32) << 16) +
                              static_cast<uint32_t>(acc * BN + half * (T::TILE_N / 2));
@@ -557,7 +736,59 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
           else mbar_arrive(&tempty[acc]);
         }
       };
-      if constexpr (EPI == static_cast<int>(Epi::Store)) {
+      if constexpr (EPI >= kEpiCeStats) {
+        ce_epilogue<EPI>(p, &mapC, buf, lane, t_row, colh, row0, grow, row_ok, nb * 2 + half, row_c, pol_c,
+                         release_tmem);
+      } else if constexpr (EPI == kEpiStoreBf16) {
+        auto store = [&](int c, const uint32_t(&r)[32]) {
+          const int col0 = colh + c * 32;
+          if (p.tma_store) {
+            uint32_t q[16];
+#pragma unroll
+            for (int j = 0; j < 16; ++j) q[j] = pack_bf16x2(__uint_as_float(r[2 * j]), __uint_as_float(r[2 * j + 1]));
+            const int x = colh + (c & ~1) * 32;
+            stage16(buf, lane, c & 1, q, &mapC, x, row0, row0 < p.M && x < p.N, pol_c);
+          } else if (row_ok) {
+            __nv_bfloat16* dst = static_cast<__nv_bfloat16*>(p.e.out16) + grow * p.e.ld16 + col0;
+#pragma unroll
+            for (int j = 0; j < 32; ++j)
+              if (col0 + j < p.N) dst[j] = __float2bfloat16_rn(__uint_as_float(r[j]));
+          }
+        };
+        constexpr int NCH = T::TILE_N / 2 / 32;
+        uint32_t ra[32], rb[32];
+        tmem_ld_32x32b_x32(t_row, ra);
+        tmem_ld_wait();
+#pragma unroll
+        for (int c = 0; c < NCH; c += 2) {
+          tmem_ld_32x32b_x32(t_row + (c + 1) * 32, rb);
+          store(c, ra);
+          tmem_ld_wait();
+          if (c + 2 < NCH) tmem_ld_32x32b_x32(t_row + (c + 2) * 32, ra);
+          else release_tmem();
+          store(c + 1, rb);
+          if (c + 2 < NCH) tmem_ld_wait();
+        }
+      } else if constexpr (EPI == kEpiStoreSlab) {
+        const int y = row0 + (w / p.rem_tiles) * static_cast<int>(p.e.slab_rows);
+        auto store = [&](int c, const uint32_t(&r)[32]) {
+          const int col0 = colh + c * 32;
+          if (col0 < p.N && row0 < p.M) stage_and_store(buf, lane, r, 1.0f, &mapC, col0, y, p.tma_reduce != 0, pol_c);
+        };
+        uint32_t ra[32], rb[32];
+        tmem_ld_32x32b_x32(t_row, ra);
+        tmem_ld_wait();
+#pragma unroll
+        for (int c = 0; c < 4; c += 2) {
+          tmem_ld_32x32b_x32(t_row + (c + 1) * 32, rb);
+          store(c, ra);
+          tmem_ld_wait();
+          if (c + 2 < 4) tmem_ld_32x32b_x32(t_row + (c + 2) * 32, ra);
+          else release_tmem();
+          store(c + 1, rb);
+          if (c + 2 < 4) tmem_ld_wait();
+        }
+      } else if constexpr (EPI == static_cast<int>(Epi::Store)) {
         const float alpha = p.e.alpha_ptr ? *p.e.alpha_ptr : p.e.alpha;
         auto store = [&](int c, const uint32_t(&r)[32]) {
           const int col0 = colh + c * 32;
@@ -759,6 +990,18 @@ bool encode_out_map_f16(CUtensorMap* map, void* ptr, long long rows, long long c
   return r == CUDA_SUCCESS;
 }
 
+// bf16 (or other 16-bit) output map: the box and swizzle of stage16's 32 x 64 blocks.
+bool encode_out_map_16(CUtensorMap* map, void* ptr, long long rows, long long cols, long long ld) {
+  cuuint64_t dims[2] = {static_cast<cuuint64_t>(cols), static_cast<cuuint64_t>(rows)};
+  cuuint64_t strides[1] = {static_cast<cuuint64_t>(ld) * 2};
+  cuuint32_t box[2] = {64, 32};
+  cuuint32_t estr[2] = {1, 1};
+  CUresult r = g_encode(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, ptr, dims, strides, box, estr,
+                        CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_NONE,
+                        CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  return r == CUDA_SUCCESS;
+}
+
 // Per-device, per-instantiation launch state: the shared-memory opt-in
 // (a function attribute that must be set once per device) and, for CTA
 // pairs, how many 2-CTA clusters can be resident at once.
@@ -849,6 +1092,12 @@ cudaError_t launch_t(const CUtensorMap* maps, const KParams& kp_in, int num_sms,
       }
     }
   }
+  if (kp.e.slabs > 1) {
+    kp.full_tiles = 0;
+    kp.rem_tiles = kp.num_tiles;
+    kp.nsplit = kp.e.slabs;
+    kp.num_items = kp.num_tiles * kp.e.slabs;
+  }
   if (kp.num_items < units) units = kp.num_items;
   if (CG == 1) {
     kern<<<units, NUM_THREADS, T::SMEM, stream>>>(maps[0], maps[1], maps[2], maps[3], maps[4], kp);
@@ -893,6 +1142,40 @@ cudaError_t dispatch(const GemmDesc& d, const CUtensorMap* maps, const KParams& 
     if (d.args.own_dT) return launch_t<CG, false, false, 17>(maps, kp, num_sms, stream);
     return launch_t<CG, false, false, 16>(maps, kp, num_sms, stream);
   }
+  if (d.epi == Epi::CeStats || d.epi == Epi::CeGrad) {
+    if (d.a_mn_major || d.b_mn_major) {
+      if (why) *why = "cross entropy epilogues require K-major operands";
+      return cudaErrorInvalidValue;
+    }
+    if (d.epi == Epi::CeGrad) return launch_t<CG, false, false, kEpiCeGrad>(maps, kp, num_sms, stream);
+    if (d.args.out16) {
+      if (d.args.ce_sx) return launch_t<CG, false, false, kEpiCeStats + 3>(maps, kp, num_sms, stream);
+      return launch_t<CG, false, false, kEpiCeStats + 1>(maps, kp, num_sms, stream);
+    }
+    if (d.args.ce_sx) return launch_t<CG, false, false, kEpiCeStats + 2>(maps, kp, num_sms, stream);
+    return launch_t<CG, false, false, kEpiCeStats>(maps, kp, num_sms, stream);
+  }
+  if (d.epi == Epi::StoreBf16) {
+    if (!d.a_mn_major || !d.b_mn_major) {
+      if (why) *why = "the bf16 store epilogue takes MN-major operands";
+      return cudaErrorInvalidValue;
+    }
+    if constexpr (CG == 2) {
+      if (wide) return launch_t<CG, true, true, kEpiStoreBf16, true>(maps, kp, num_sms, stream);
+    }
+    return launch_t<CG, true, true, kEpiStoreBf16, false>(maps, kp, num_sms, stream);
+  }
+  if (d.args.slabs > 1) {
+    if (d.nseg != 1 || d.args.slabs > kp.seg_kblocks[0]) {
+      if (why) *why = "K slabs take one K segment with a K block for each slab";
+      return cudaErrorInvalidValue;
+    }
+    if (d.a_mn_major || !d.b_mn_major || !kp.tma_store) {
+      if (why) *why = "K slabs take a K-major A, an MN-major B and a TMA-aligned output";
+      return cudaErrorInvalidValue;
+    }
+    return launch_t<CG, false, true, kEpiStoreSlab>(maps, kp, num_sms, stream);
+  }
   if (!d.a_mn_major && !d.b_mn_major) return store_launch<CG, false, false>(wide, maps, kp, num_sms, stream);
   if (!d.a_mn_major && d.b_mn_major) return store_launch<CG, false, true>(wide, maps, kp, num_sms, stream);
   if (d.a_mn_major && !d.b_mn_major) return store_launch<CG, true, false>(wide, maps, kp, num_sms, stream);
@@ -919,7 +1202,7 @@ bool use_cta_pair() {
 bool use_wide(const GemmDesc& d, long long k_blocks, long long m_blocks, int num_sms) {
   const char* v = std::getenv("ORDA_GEMM_WIDE");
   const int mode = v ? (v[0] - '0') : 1;
-  if (mode == 0 || d.epi != Epi::Store || d.N <= BN) return false;
+  if (mode == 0 || (d.epi != Epi::Store && d.epi != Epi::StoreBf16) || d.N <= BN || d.args.slabs > 1) return false;
   if (mode == 2) return true;
   const long long tiles = m_blocks * ((d.N + 2 * BN - 1) / (2 * BN));
   return tiles >= num_sms && k_blocks >= (d.args.scatter ? 1024 : 128);
@@ -977,7 +1260,9 @@ cudaError_t gemm_launch(const GemmDesc& d, int num_sms, cudaStream_t stream, con
   // other one is re-read by every tile of its rows/columns: keep it
   // (evict-last). Outputs larger than 32 MB are written once: evict-first.
   constexpr long long kKeepBytes = 64ll << 20;
-  const long long a_bytes = d.M * k_total * 2, b_bytes = d.N * k_total * 2, c_bytes = d.M * d.N * 4;
+  const long long a_bytes = d.M * k_total * 2, b_bytes = d.N * k_total * 2;
+  const long long c_bytes = d.epi == Epi::CeStats && !d.args.out16 ? 0
+                            : d.M * d.N * (d.epi == Epi::Store || d.epi == Epi::Logits ? 4 : 2) * d.args.slabs;
   kp.pol_a = (a_bytes <= kKeepBytes && a_bytes <= b_bytes) ? 2 : 0;
   kp.pol_b = (b_bytes <= kKeepBytes && b_bytes < a_bytes) ? 2 : 0;
   kp.pol_c = c_bytes > (32ll << 20) ? 1 : 0;
@@ -1013,6 +1298,23 @@ cudaError_t gemm_launch(const GemmDesc& d, int num_sms, cudaStream_t stream, con
                encode_out_map(&maps[4], static_cast<float*>(d.args.logits), d.M, d.N, d.args.ldl)) {
       kp.tma_store = 1;
     }
+  } else if (d.epi == Epi::StoreBf16 || d.epi == Epi::CeStats || d.epi == Epi::CeGrad) {
+    if (d.args.out16 && out_map_ok(d.args.out16, d.args.ld16, 2) &&
+        encode_out_map_16(&maps[4], d.args.out16, d.M, d.N, d.args.ld16)) {
+      kp.tma_store = 1;
+    } else if (d.epi == Epi::CeGrad || (d.epi == Epi::CeStats && d.args.out16)) {
+      if (why) *why = "16-bit pieces need a 16-byte aligned buffer with ld a multiple of 8";
+      return cudaErrorInvalidValue;
+    }
+  } else if (d.args.slabs > 1) {
+    // partial rows of slab i are stored below slab i + 1: slab_rows covers whole 32-row blocks
+    if (d.args.slab_rows % 32 != 0 || d.args.slab_rows < d.M || !out_map_ok(d.args.out0, d.args.ld0) ||
+        !encode_out_map(&maps[4], d.args.out0, d.args.slabs * d.args.slab_rows, d.N, d.args.ld0)) {
+      if (why) *why = "K slabs need slab_rows a multiple of 32, >= M, and a TMA-aligned output";
+      return cudaErrorInvalidValue;
+    }
+    kp.tma_store = 1;
+    kp.tma_reduce = d.args.beta == 1.0f ? 1 : 0;
   } else if (d.args.split_row >= d.M && (d.args.beta == 0.0f || d.args.beta == 1.0f) &&
              out_map_ok(d.args.out0, d.args.ld0) && encode_out_map(&maps[4], d.args.out0, d.M, d.N, d.args.ld0)) {
     kp.tma_store = 1;
@@ -1021,7 +1323,7 @@ cudaError_t gemm_launch(const GemmDesc& d, int num_sms, cudaStream_t stream, con
   // Split tail tiles only for wide tiles: a split tile sums its K range as
   // two halves plus one add, so its rows are associated differently from
   // those of an unsplit tile of another call.
-  kp.allow_split = wide && kp.tma_store && !kp.tma_reduce && d.nseg == 1 && !d.args.scatter;
+  kp.allow_split = wide && d.epi == Epi::Store && kp.tma_store && !kp.tma_reduce && d.nseg == 1 && !d.args.scatter;
   if (kp.num_tiles == 0) return cudaSuccess;
   cudaError_t e = cg == 2 ? dispatch<2>(d, maps, kp, num_sms, stream, why, wide)
                           : dispatch<1>(d, maps, kp, num_sms, stream, why, false);

@@ -17,12 +17,15 @@ struct MatRef {
   long long ld = 0;
 };
 
-enum class Epi : int { Store = 0, Logits = 1 };
+enum class Epi : int { Store = 0, Logits = 1, StoreBf16 = 2, CeStats = 3, CeGrad = 4 };
 
 // Epilogue arguments. Store: out = alpha * acc (+ beta * out); rows below
 // split_row go to out0, the rest to out1 (row - split_row).
 // Logits: fp32 logits written to `logits` (ldl) plus per-(row, 128-column
 // part) online-softmax records (see rows.cu for the record layout).
+// StoreBf16: out16 = acc rounded to bf16.
+// CeStats / CeGrad: the two passes of the linear cross entropy over a piece
+// of the vocabulary (see linear_ce.cu).
 constexpr int kMaxSlotRanks = 8;  // ranks of one node that a scattered grad_W store can address
 
 struct EpiArgs {
@@ -52,6 +55,22 @@ struct EpiArgs {
   long long slot_slice = 0;
   long long slot_ld = 0;
   float* slot[kMaxSlotRanks] = {};
+  // Store, in K slabs: the K range is cut into `slabs` parts and part i is
+  // written (or added, beta == 1) to rows [i * slab_rows, i * slab_rows + M) of
+  // out0, whose leading dimension must allow TMA stores. slab_rows is a
+  // multiple of 32 and >= M.
+  int slabs = 1;
+  long long slab_rows = 0;
+  // StoreBf16, and the 16-bit piece that CeStats (optionally) and CeGrad write
+  void* out16 = nullptr;
+  long long ld16 = 0;
+  // CeStats, CeGrad: column c is vocabulary index ce_v0 + c
+  long long ce_v0 = 0;
+  const float2* ce_ref = nullptr;    // CeStats: per row (reference logit * log2 e, label as int bits)
+  float2* ce_rec = nullptr;          // CeStats: [parts][ce_rec_ld] records, from column 0 of this launch
+  float* ce_sx = nullptr;            // CeStats, optional: [parts][ce_rec_ld] sums of the logits
+  long long ce_rec_ld = 0;
+  const float4* ce_const = nullptr;  // CeGrad: per row constants (CeRowConst)
 };
 
 struct GemmDesc {
@@ -79,6 +98,54 @@ struct GemmDesc {
 // Encodes the tensor maps and launches the persistent tcgen05 GEMM.
 // Returns cudaSuccess or the first error.
 cudaError_t gemm_launch(const GemmDesc& d, int num_sms, cudaStream_t stream, const char** why);
+
+// ------------------------------------------- linear cross entropy (linear_ce.cu)
+// Fixed point of the 16-bit logits that CeStats keeps: (t + 64) * 512 for
+// t = log2(e^logit / reference); 0 stands for every t <= -64, a gradient of
+// zero (see linear_ce.cu).
+constexpr float kCeQScale = 512.0f;
+constexpr float kCeQBias = 32768.0f;
+constexpr float kCeQLow = -64.0f;
+// A part whose sum of 2^t lies outside [2^-40, 2^62) is stored relative to its own maximum.
+constexpr float kCeSumLow = 9.094947017729282e-13f;
+constexpr float kCeSumHigh = 4611686018427387904.0f;
+constexpr int kCePartCols = 128;
+
+struct CeArgs {
+  const void* h = nullptr;  // bf16 [bt, hd]
+  long long ldh = 0;
+  const void* w = nullptr;  // bf16 [v, hd]
+  long long ldw = 0;
+  long long bt = 0, hd = 0, v = 0;
+  const int64_t* labels = nullptr;
+  int64_t ignore_index = 0;
+  float alpha = 0.0f;  // label smoothing
+  int reduction_sum = 0;
+  long long denom_override = 0;
+  uint16_t* h_clean = nullptr;  // bf16 [bt, ld_clean]
+  long long ld_clean = 0;
+  float2* ref = nullptr;       // [bt]
+  float2* rec = nullptr;       // [n_parts][rec_ld]
+  float* sx = nullptr;         // [n_parts][rec_ld], with label smoothing
+  long long rec_ld = 0;
+  int n_parts = 0;
+  float4* row_const = nullptr;  // [bt]
+  float* nll = nullptr;         // [bt]
+  float* lse = nullptr;         // [bt], optional
+  float* loss = nullptr;        // [1]
+  int* status = nullptr;
+  int* count = nullptr;  // live tokens; zero before the call
+  int* done = nullptr;   // finished blocks of the combining kernel; zero before the call
+};
+// Labels, reference logits and the copy of the hidden states with ignored rows cleared.
+void launch_ce_prep(const CeArgs& a, cudaStream_t stream);
+// Records -> nll, lse, the gradient's row constants and the loss.
+void launch_ce_combine(const CeArgs& a, cudaStream_t stream);
+// The kept 16-bit logits of vocabulary columns [v0, v0 + n) -> bf16 logit gradients, in place.
+void launch_ce_rewrite(const CeArgs& a, uint16_t* piece, long long ld, long long v0, long long n, cudaStream_t stream);
+// out = the sum over slabs of buf (fp32 [slabs][slab_rows][ldb]) for rows x cols, as bf16 or fp32.
+void launch_slab_sum(const float* buf, int slabs, long long slab_rows, long long ldb, long long rows, long long cols,
+                     void* out, long long ldo, int out_bf16, cudaStream_t stream);
 
 // ------------------------------------------------------------ row kernels
 // Element type of a logits buffer the row kernels read.

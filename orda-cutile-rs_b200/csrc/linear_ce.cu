@@ -1,0 +1,338 @@
+// linear_ce.cu -- row kernels of the linear softmax cross entropy
+// (orda_linear_cross_entropy_device); its products run in gemm_sm100.cu.
+//
+// With z = h W^T, y the label, a the label smoothing and g the loss scale:
+//   lse = log sum_v e^{z_v}
+//   nll = (1 - a) (lse - z_y) + a (lse - mean_v z_v)
+//   dz_v = g (e^{z_v - lse} - (1 - a) [v = y] - a / V),  dh = dz W,  dW = dz^T h
+// The label's logit is the reference of its row: the logits product sums
+// Z_o = sum_{v != y} e^{z_v - z_y} per 128-column part, so that
+//   lse - z_y = log(1 + Z_o),  1 - p_y = Z_o / (1 + Z_o)
+// lose nothing to cancellation when the label's probability nears 1.
+//
+// Between the logits product and the two gradient products the logits of a
+// piece are kept as 16-bit fixed point, t = log2 e^{z - z_y} in steps of
+// 2^-9 over (-64, 64), and 0 below (a part whose own sum is under 2^-40 is
+// kept against its own maximum, so 0 stands for less than 2^-16 of a part's
+// largest probability): an error of at most 2^-10 ln 2 = 6.8e-4 (3.9e-4 rms) of
+// each probability, where the bf16 rounding of the gradient operand that
+// follows is at most 2^-8 = 3.9e-3 (1.6e-3 rms). It takes half the bytes of
+// fp32 logits; the statistics are fp32 and come from the accumulators.
+#include <cuda_bf16.h>
+#include <cuda_runtime.h>
+
+#include <algorithm>
+#include <cstdint>
+
+#include "kernels.h"
+#include "ptx.cuh"
+
+namespace orda {
+namespace {
+
+constexpr float kLog2E = 1.4426950408889634f;
+constexpr double kLn2 = 0.6931471805599453;
+
+__device__ __forceinline__ float bf16_lo(uint32_t w) { return __uint_as_float(w << 16); }
+__device__ __forceinline__ float bf16_hi(uint32_t w) { return __uint_as_float(w & 0xffff0000u); }
+
+__device__ __forceinline__ float warp_sum(float v) {
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+  return v;
+}
+
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+// One block per token: the label's logit (fp32 products and sums of the bf16
+// operands) and a copy of the hidden state in which an ignored token is zero,
+// so that whatever an ignored row holds (NaN and infinities of padding
+// included) reaches no product. Bound by bandwidth: 3 rows of H bf16 each.
+constexpr int kPrepThreads = 128;
+
+__global__ void __launch_bounds__(kPrepThreads) ce_prep_kernel(const CeArgs a) {
+  const long long row = blockIdx.x;
+  const int64_t y = a.labels[row];
+  bool live = y != a.ignore_index;
+  if (live && (y < 0 || y >= a.v)) {
+    if (threadIdx.x == 0) atomicCAS(a.status, DEV_OK, DEV_LABEL_RANGE);
+    live = false;
+  }
+  const uint16_t* h = static_cast<const uint16_t*>(a.h) + row * a.ldh;
+  const uint16_t* w = static_cast<const uint16_t*>(a.w) + (live ? y : 0) * a.ldw;
+  uint16_t* out = a.h_clean + row * a.ld_clean;
+  const int nvec = static_cast<int>(a.hd / 8);
+  float s = 0.f;
+  if (live) {
+#pragma unroll 4
+    for (int i = threadIdx.x; i < nvec; i += kPrepThreads) {
+      const uint4 p = __ldcs(reinterpret_cast<const uint4*>(h) + i);
+      const uint4 q = *(reinterpret_cast<const uint4*>(w) + i);
+      reinterpret_cast<uint4*>(out)[i] = p;
+      const uint32_t pw[4] = {p.x, p.y, p.z, p.w}, qw[4] = {q.x, q.y, q.z, q.w};
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        s = fmaf(bf16_lo(pw[k]), bf16_lo(qw[k]), s);
+        s = fmaf(bf16_hi(pw[k]), bf16_hi(qw[k]), s);
+      }
+    }
+    for (long long i = 8ll * nvec + threadIdx.x; i < a.hd; i += kPrepThreads) {
+      out[i] = h[i];
+      s = fmaf(bf16_lo(h[i]), bf16_lo(w[i]), s);
+    }
+  } else {
+    for (int i = threadIdx.x; i < nvec; i += kPrepThreads) reinterpret_cast<uint4*>(out)[i] = make_uint4(0, 0, 0, 0);
+    for (long long i = 8ll * nvec + threadIdx.x; i < a.hd; i += kPrepThreads) out[i] = 0;
+  }
+  s = warp_sum(s);
+  __shared__ float part[kPrepThreads / 32];
+  if ((threadIdx.x & 31) == 0) part[threadIdx.x >> 5] = s;
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    float x = 0.f;
+#pragma unroll
+    for (int k = 0; k < kPrepThreads / 32; ++k) x += part[k];
+    a.ref[row] = make_float2(live ? x * kLog2E : 0.f, __int_as_float(live ? static_cast<int>(y) : -1));
+    if (live) atomicAdd(a.count, 1);
+  }
+}
+
+// Sum of 2^(r_i) * d_i with a running maximum of the references r_i.
+struct Acc {
+  double d;
+  float r;
+};
+__device__ __forceinline__ void acc_add(Acc& a, double d, float r) {
+  // equal references, the usual case, add without a factor
+  if (r == a.r) {
+    a.d += d;
+  } else if (d != 0.0) {
+    if (!(r <= a.r)) {
+      a.d = (a.d == 0.0 ? 0.0 : a.d * exp2(static_cast<double>(a.r) - static_cast<double>(r))) + d;
+      a.r = r;
+    } else {
+      a.d += d * exp2(static_cast<double>(r) - static_cast<double>(a.r));
+    }
+  }
+}
+
+// R rows per block, 256 / R threads per row over the parts (their records lie
+// [part][row], so R rows are read together); then the row's loss and constants
+// in 64 bits. The block that finishes last sums the losses in row order.
+constexpr int kCombineThreads = 256;
+
+template <int R>
+__global__ void __launch_bounds__(kCombineThreads) ce_combine_kernel(const CeArgs a) {
+  constexpr int T = kCombineThreads / R;
+  __shared__ Acc acc_s[kCombineThreads];
+  __shared__ double sx_s[kCombineThreads];
+  __shared__ bool last;
+  const int r = threadIdx.x % R, t = threadIdx.x / R;
+  const long long row = static_cast<long long>(blockIdx.x) * R + r;
+  const float2 ref = row < a.bt ? a.ref[row] : make_float2(0.f, __int_as_float(-1));
+  const bool live = __float_as_int(ref.y) >= 0;
+  Acc acc{0.0, ref.x};
+  double sx = 0.0;
+  if (live) {
+#pragma unroll 8
+    for (int p = t; p < a.n_parts; p += T) {
+      const float2 c = a.rec[p * a.rec_ld + row];
+      acc_add(acc, static_cast<double>(c.x), c.y);
+    }
+    if (a.alpha > 0.f)
+#pragma unroll 8
+      for (int p = t; p < a.n_parts; p += T) sx += static_cast<double>(a.sx[p * a.rec_ld + row]);
+  }
+  acc_s[threadIdx.x] = acc;
+  sx_s[threadIdx.x] = sx;
+  __syncthreads();
+#pragma unroll
+  for (int o = T / 2; o > 0; o >>= 1) {
+    if (t < o) {
+      Acc m = acc_s[threadIdx.x];
+      const Acc other = acc_s[threadIdx.x + o * R];
+      acc_add(m, other.d, other.r);
+      acc_s[threadIdx.x] = m;
+      sx_s[threadIdx.x] += sx_s[threadIdx.x + o * R];
+    }
+    __syncthreads();
+  }
+  if (t == 0 && row < a.bt) {
+    float nll = 0.f, lse = 0.f;
+    float4 c = make_float4(-INFINITY, __int_as_float(-1), 0.f, 0.f);
+    if (live) {
+      const long long n = a.denom_override > 0 ? a.denom_override : max(*static_cast<volatile int*>(a.count), 1);
+      const double g = a.reduction_sum ? 1.0 : 1.0 / static_cast<double>(n);
+      const Acc m = acc_s[threadIdx.x];
+      // Z_o = m.d 2^(m.r - ref): everything but the label
+      const double up = static_cast<double>(m.r) - static_cast<double>(ref.x);
+      double gap, miss, l;  // lse - z_y, 1 - p_y and lse
+      if (m.r == ref.x) {
+        gap = log1p(m.d);
+        miss = m.d / (1.0 + m.d);
+        l = static_cast<double>(ref.x) * kLn2 + gap;
+      } else {
+        const double own = exp2(-up);  // the label's term next to m.d
+        gap = up * kLn2 + log(m.d + own);
+        miss = m.d / (m.d + own);
+        l = static_cast<double>(m.r) * kLn2 + log(m.d + own);
+      }
+      const double al = static_cast<double>(a.alpha), uni = al / static_cast<double>(a.v);
+      nll = static_cast<float>(al > 0.0 ? (1.0 - al) * gap + al * l - uni * sx_s[threadIdx.x] : gap);
+      lse = static_cast<float>(l);
+      c.x = static_cast<float>(log2(g) - l / kLn2);
+      c.y = ref.y;
+      c.z = static_cast<float>(g * uni);
+      c.w = static_cast<float>(g * (al - uni - miss));
+    }
+    a.row_const[row] = c;
+    a.nll[row] = nll;
+    if (a.lse) a.lse[row] = lse;
+    __threadfence();
+  }
+  __syncthreads();
+  if (threadIdx.x == 0) last = atomicAdd(a.done, 1) == static_cast<int>(gridDim.x) - 1;
+  __syncthreads();
+  if (last) {
+    __threadfence();
+    double s = 0.0;
+#pragma unroll 4
+    for (long long i = threadIdx.x; i < a.bt; i += kCombineThreads) s += static_cast<double>(__ldcg(a.nll + i));
+    sx_s[threadIdx.x] = s;
+    __syncthreads();
+    for (int o = kCombineThreads / 2; o > 0; o >>= 1) {
+      if (static_cast<int>(threadIdx.x) < o) sx_s[threadIdx.x] += sx_s[threadIdx.x + o];
+      __syncthreads();
+    }
+    if (threadIdx.x == 0) {
+      const long long n = a.denom_override > 0 ? a.denom_override : max(*static_cast<volatile int*>(a.count), 1);
+      *a.loss = static_cast<float>(a.reduction_sum ? sx_s[0] : sx_s[0] / static_cast<double>(n));
+    }
+  }
+}
+
+// Kept 16-bit logits -> bf16 logit gradients, in place: 2^(t + c) - a / V g,
+// with c = (the part's reference - lse) log2 e + log2 g. Bound by bandwidth
+// (4 bytes per element); each thread holds 8 neighbouring columns.
+constexpr int kRewriteThreads = 256;
+constexpr int kRewriteSteps = 4;
+constexpr int kRewriteCols = kRewriteThreads * 8 * kRewriteSteps;
+
+__global__ void __launch_bounds__(kRewriteThreads)
+    ce_rewrite_kernel(const float4* __restrict__ row_const, const float2* __restrict__ rec, long long rec_ld,
+                      uint16_t* piece, long long ld, long long v0, long long n, int segs) {
+  const long long row = blockIdx.x / segs;
+  const int seg = static_cast<int>(blockIdx.x - row * segs);
+  const float4 c = row_const[row];
+  const long long label = static_cast<long long>(__float_as_int(c.y)) - v0;
+  uint16_t* base = piece + row * ld;
+  uint4 v[kRewriteSteps];
+  float off[kRewriteSteps];
+#pragma unroll
+  for (int i = 0; i < kRewriteSteps; ++i) {
+    const long long col = static_cast<long long>(seg) * kRewriteCols + i * (kRewriteThreads * 8) + threadIdx.x * 8;
+    if (col < n) {
+      v[i] = __ldcs(reinterpret_cast<const uint4*>(base + col));
+      off[i] = rec[((v0 + col) / kCePartCols) * rec_ld + row].y + c.x;
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < kRewriteSteps; ++i) {
+    const long long col = static_cast<long long>(seg) * kRewriteCols + i * (kRewriteThreads * 8) + threadIdx.x * 8;
+    if (col >= n) continue;
+    uint32_t w[4] = {v[i].x, v[i].y, v[i].z, v[i].w};
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      // 2^23 + u as a float, from u's 16 bits
+      const float q0 = __uint_as_float(__byte_perm(w[k], 0x4B000000u, 0x7610)) - (8388608.0f + kCeQBias);
+      const float q1 = __uint_as_float(__byte_perm(w[k], 0x4B000000u, 0x7632)) - (8388608.0f + kCeQBias);
+      const float e0 = ex2(fmaf(q0, 1.0f / kCeQScale, off[i]));
+      const float e1 = ex2(fmaf(q1, 1.0f / kCeQScale, off[i]));
+      float d0 = (q0 == -kCeQBias ? 0.f : e0) - c.z;
+      float d1 = (q1 == -kCeQBias ? 0.f : e1) - c.z;
+      const long long l = label - col - 2 * k;
+      if (l == 0) d0 = c.w;
+      if (l == 1) d1 = c.w;
+      const __nv_bfloat162 b = __floats2bfloat162_rn(d0, d1);
+      w[k] = *reinterpret_cast<const uint32_t*>(&b);
+    }
+    *reinterpret_cast<uint4*>(base + col) = make_uint4(w[0], w[1], w[2], w[3]);
+  }
+}
+
+// Sum over K slabs, in slab order, and the output's type.
+template <bool BF16>
+__global__ void __launch_bounds__(256)
+    slab_sum_kernel(const float* __restrict__ buf, int slabs, long long slab_rows, long long ldb, long long rows,
+                    long long cols, void* out, long long ldo, int vec_ok) {
+  const long long groups = (cols + 3) / 4;
+  for (long long i = blockIdx.x * 256ll + threadIdx.x; i < rows * groups; i += gridDim.x * 256ll) {
+    const long long r = i / groups, c = (i - r * groups) * 4;
+    float4 s = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 4
+    for (int k = 0; k < slabs; ++k) {
+      const float4 x = *reinterpret_cast<const float4*>(buf + (k * slab_rows + r) * ldb + c);
+      s.x += x.x;
+      s.y += x.y;
+      s.z += x.z;
+      s.w += x.w;
+    }
+    const float f[4] = {s.x, s.y, s.z, s.w};
+    if (BF16) {
+      __nv_bfloat16* o = static_cast<__nv_bfloat16*>(out) + r * ldo + c;
+      if (vec_ok && c + 4 <= cols) {
+        const __nv_bfloat162 lo = __floats2bfloat162_rn(f[0], f[1]), hi = __floats2bfloat162_rn(f[2], f[3]);
+        *reinterpret_cast<uint2*>(o) =
+            make_uint2(*reinterpret_cast<const uint32_t*>(&lo), *reinterpret_cast<const uint32_t*>(&hi));
+      } else {
+        for (int k = 0; k < 4 && c + k < cols; ++k) o[k] = __float2bfloat16_rn(f[k]);
+      }
+    } else {
+      float* o = static_cast<float*>(out) + r * ldo + c;
+      if (vec_ok && c + 4 <= cols) *reinterpret_cast<float4*>(o) = s;
+      else
+        for (int k = 0; k < 4 && c + k < cols; ++k) o[k] = f[k];
+    }
+  }
+}
+
+}  // namespace
+
+void launch_ce_prep(const CeArgs& a, cudaStream_t stream) {
+  ce_prep_kernel<<<static_cast<unsigned>(a.bt), kPrepThreads, 0, stream>>>(a);
+}
+
+// Eight rows per block read whole 64-byte sectors of the records; fewer rows
+// per block where that would leave SMs without a block.
+void launch_ce_combine(const CeArgs& a, cudaStream_t stream) {
+  if (a.bt >= 2048)
+    ce_combine_kernel<8><<<static_cast<unsigned>((a.bt + 7) / 8), kCombineThreads, 0, stream>>>(a);
+  else if (a.bt >= 512)
+    ce_combine_kernel<4><<<static_cast<unsigned>((a.bt + 3) / 4), kCombineThreads, 0, stream>>>(a);
+  else
+    ce_combine_kernel<1><<<static_cast<unsigned>(a.bt), kCombineThreads, 0, stream>>>(a);
+}
+
+void launch_ce_rewrite(const CeArgs& a, uint16_t* piece, long long ld, long long v0, long long n, cudaStream_t stream) {
+  const int segs = static_cast<int>((n + kRewriteCols - 1) / kRewriteCols);
+  ce_rewrite_kernel<<<static_cast<unsigned>(a.bt * segs), kRewriteThreads, 0, stream>>>(a.row_const, a.rec, a.rec_ld,
+                                                                                        piece, ld, v0, n, segs);
+}
+
+void launch_slab_sum(const float* buf, int slabs, long long slab_rows, long long ldb, long long rows, long long cols,
+                     void* out, long long ldo, int out_bf16, cudaStream_t stream) {
+  const long long n = rows * ((cols + 3) / 4);
+  const unsigned blocks = static_cast<unsigned>(std::min<long long>((n + 255) / 256, 148 * 16));
+  const int esz = out_bf16 ? 2 : 4;
+  const int vec_ok = reinterpret_cast<uintptr_t>(out) % (4 * esz) == 0 && ldo % 4 == 0;
+  if (out_bf16)
+    slab_sum_kernel<true><<<blocks, 256, 0, stream>>>(buf, slabs, slab_rows, ldb, rows, cols, out, ldo, vec_ok);
+  else
+    slab_sum_kernel<false><<<blocks, 256, 0, stream>>>(buf, slabs, slab_rows, ldb, rows, cols, out, ldo, vec_ok);
+}
+
+}  // namespace orda

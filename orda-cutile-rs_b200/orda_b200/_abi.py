@@ -142,6 +142,30 @@ class OrdaVocabShard(C.Structure):
                 ("scatter_grad_hidden", C.c_int32), ("pad", C.c_int32)]
 
 
+class OrdaLinearCeOptions(C.Structure):
+    _fields_ = [
+        ("ignore_index", C.c_int64),
+        ("label_smoothing", C.c_float),
+        ("reduction", C.c_int),
+        ("global_non_ignore", C.c_int64),
+        ("piece_bytes", C.c_size_t),
+    ]
+
+
+class OrdaLinearCeOutputs(C.Structure):
+    _fields_ = [
+        ("loss", C.c_void_p),
+        ("nll", C.c_void_p),
+        ("lse", C.c_void_p),
+        ("grad_hidden", C.c_void_p),
+        ("ld_grad_hidden", C.c_size_t),
+        ("grad_weight", C.c_void_p),
+        ("ld_grad_weight", C.c_size_t),
+        ("grad_hidden_dtype", C.c_int),
+        ("grad_weight_dtype", C.c_int),
+    ]
+
+
 class OrdaIpcHandle(C.Structure):
     _fields_ = [("bytes", C.c_ubyte * 64)]  # opaque; c_ubyte so no NUL truncation
 
@@ -227,6 +251,11 @@ SIGNATURES = {
         [C.c_void_p, C.POINTER(OrdaDeviceMat), C.POINTER(OrdaDeviceMat), C.c_void_p, C.c_size_t,
          C.POINTER(OrdaDeviceTeacher), C.POINTER(OrdaLossOptions), C.POINTER(OrdaVocabShard), C.c_void_p,
          C.POINTER(OrdaDeviceOutputs), C.c_void_p, C.POINTER(OrdaChunkPlan), C.c_char_p, C.c_size_t]),
+    "orda_linear_ce_options_default": (None, [C.POINTER(OrdaLinearCeOptions)]),
+    "orda_linear_cross_entropy_device": (
+        C.c_int,
+        [C.c_void_p, C.POINTER(OrdaDeviceMat), C.POINTER(OrdaDeviceMat), C.c_void_p, C.c_size_t,
+         C.POINTER(OrdaLinearCeOptions), C.POINTER(OrdaLinearCeOutputs), C.c_void_p, C.c_char_p, C.c_size_t]),
     "orda_context_slots_create": (
         C.c_int, [C.c_void_p, C.c_int, C.c_int, C.c_size_t, C.c_size_t, C.c_int, C.POINTER(OrdaIpcHandle),
                   C.c_char_p, C.c_size_t]),

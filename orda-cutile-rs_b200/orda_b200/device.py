@@ -9,7 +9,7 @@ from typing import Optional
 
 import torch
 
-from . import ChunkPlan, LossOptions, TeacherMode, _abi, _check
+from . import ChunkPlan, LossOptions, Reduction, TeacherMode, _abi, _check
 from ._abi import load_library
 
 
@@ -354,6 +354,116 @@ def vocab_backward_device(
         _stream(stream), C.byref(plan), buf, len(buf))
     _check(rc, buf)
     return DeviceLossResult(chunk_plan=ChunkPlan(int(plan.chunk_size), int(plan.num_chunks)), **tensors)
+
+
+def _on_context(ctx: DeviceContext, **tensors: Optional[torch.Tensor]) -> None:
+    """Every tensor lies on the context's GPU."""
+    for name, t in tensors.items():
+        if t is not None and (not t.is_cuda or t.device.index != ctx.device):
+            raise ValueError(f"{name} must be on cuda:{ctx.device}, the context's device, got {t.device}")
+
+
+def _context_stream(ctx: DeviceContext, stream) -> int:
+    """The given stream, else the current one of the context's device."""
+    return torch.cuda.current_stream(ctx.device).cuda_stream if stream is None else _stream(stream)
+
+
+def _grad_dtype(t: torch.Tensor, name: str) -> int:
+    if t.dtype == torch.bfloat16:
+        return _abi.DTYPE_BF16
+    if t.dtype == torch.float32:
+        return _abi.DTYPE_F32
+    raise ValueError(f"{name}: unsupported dtype {t.dtype}")
+
+
+def _row_major(rows: int, cols: int, dtype: torch.dtype, device) -> torch.Tensor:
+    """[rows, cols] whose rows start on 16 bytes (what TMA stores address)."""
+    step = 16 // torch.empty(0, dtype=dtype).element_size()
+    return torch.empty(rows, -(-cols // step) * step, device=device, dtype=dtype)[:, :cols]
+
+
+@dataclass
+class LinearCrossEntropyResult:
+    loss: torch.Tensor  # device float, 0-dim
+    nll: torch.Tensor  # float [bt], 0 for ignored tokens
+    lse: torch.Tensor  # float [bt], 0 for ignored tokens
+    grad_hidden: Optional[torch.Tensor]
+    grad_weight: Optional[torch.Tensor]
+
+
+def linear_cross_entropy_device(
+    ctx: DeviceContext,
+    hidden: torch.Tensor,
+    weight: torch.Tensor,
+    labels: torch.Tensor,
+    ignore_index: int = -100,
+    label_smoothing: float = 0.0,
+    reduction: Reduction = Reduction.Mean,
+    need_grad_hidden: bool = True,
+    need_grad_weight: bool = True,
+    grad_dtype: torch.dtype = torch.float32,
+    out: Optional[dict] = None,
+    global_non_ignore: int = 0,
+    piece_bytes: int = 0,
+    stream=None,
+) -> LinearCrossEntropyResult:
+    """`orda_linear_cross_entropy_device`: softmax cross entropy of
+    hidden [bt, H] @ weight [V, H]^T (bf16) against labels [bt] (int64), with
+    the gradients of hidden and weight and without a teacher.
+
+    need_grad_hidden / need_grad_weight select the gradients (neither: the
+    losses alone, for scoring). grad_dtype (bf16 or f32) is the type of the
+    gradients that are allocated here; `out` may hold loss (float [1]), nll,
+    lse, grad_hidden and grad_weight to write into (their own types decide).
+    piece_bytes bounds the 16-bit logits kept at once (0: 4 GiB); columns of
+    the vocabulary beyond it are computed twice. nll and lse are those of
+    each token, for log-probabilities (-nll) and for a z-loss of the caller's.
+    Labels out of range are reported by ctx.check()."""
+    if hidden.dim() != 2 or weight.dim() != 2 or labels.dim() != 1:
+        raise ValueError("hidden and weight must be 2-D and labels 1-D")
+    if labels.dtype != torch.int64 or not labels.is_contiguous():
+        raise ValueError("labels must be contiguous int64")
+    out = dict(out or {})
+    unknown = set(out) - {"loss", "nll", "lse", "grad_hidden", "grad_weight"}
+    if unknown:
+        raise ValueError(f"unknown outputs {sorted(unknown)}")
+    _on_context(ctx, hidden=hidden, weight=weight, labels=labels, **out)
+    (bt, h), v, dev = hidden.shape, weight.shape[0], hidden.device
+    loss = out.get("loss")
+    if loss is None:
+        loss = torch.empty(1, device=dev, dtype=torch.float32)
+    vectors = {}
+    for name in ("nll", "lse"):
+        t = out.get(name)
+        vectors[name] = torch.empty(bt, device=dev, dtype=torch.float32) if t is None else t
+    for name, t, n in (("loss", loss, 1), ("nll", vectors["nll"], bt), ("lse", vectors["lse"], bt)):
+        if t.dtype != torch.float32 or t.numel() != n or not t.is_contiguous():
+            raise ValueError(f"{name} must be contiguous float32 of {n} element(s)")
+    o = _abi.OrdaLinearCeOutputs()
+    o.loss, o.nll, o.lse = loss.data_ptr(), vectors["nll"].data_ptr(), vectors["lse"].data_ptr()
+    grads = {"grad_hidden": None, "grad_weight": None}
+    for name, rows, need in (("grad_hidden", bt, need_grad_hidden), ("grad_weight", v, need_grad_weight)):
+        if not need:
+            if name in out:
+                raise ValueError(f"out holds {name}, which need_{name}=False leaves out")
+            continue
+        t = out.get(name)
+        if t is None:
+            t = _row_major(rows, h, grad_dtype, dev)
+        if tuple(t.shape) != (rows, h) or t.stride(1) != 1:
+            raise ValueError(f"{name} must be ({rows}, {h}) with unit column stride")
+        grads[name] = t
+        setattr(o, name, t.data_ptr())
+        setattr(o, f"ld_{name}", max(t.stride(0), h))
+        setattr(o, f"{name}_dtype", _grad_dtype(t, name))
+    opts = _abi.OrdaLinearCeOptions(int(ignore_index), float(label_smoothing), int(reduction),
+                                    int(global_non_ignore), int(piece_bytes))
+    buf = _abi.err_buf()
+    rc = _lib().orda_linear_cross_entropy_device(
+        ctx.handle, C.byref(dev_mat(hidden)), C.byref(dev_mat(weight)), labels.data_ptr(), labels.numel(),
+        C.byref(opts), C.byref(o), _context_stream(ctx, stream), buf, len(buf))
+    _check(rc, buf)
+    return LinearCrossEntropyResult(loss=loss.view(-1)[0], nll=vectors["nll"], lse=vectors["lse"], **grads)
 
 
 def gemm_bf16(

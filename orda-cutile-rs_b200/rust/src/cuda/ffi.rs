@@ -203,6 +203,30 @@ pub struct OrdaVocabShard {
 }
 
 #[repr(C)]
+#[derive(Clone, Copy, Debug)]
+pub struct OrdaLinearCeOptions {
+    pub ignore_index: i64,
+    pub label_smoothing: f32,
+    pub reduction: c_int,
+    pub global_non_ignore: i64,
+    pub piece_bytes: usize,
+}
+
+#[repr(C)]
+#[derive(Clone, Copy, Debug)]
+pub struct OrdaLinearCeOutputs {
+    pub loss: *mut f32,
+    pub nll: *mut f32,
+    pub lse: *mut f32,
+    pub grad_hidden: *mut c_void,
+    pub ld_grad_hidden: usize,
+    pub grad_weight: *mut c_void,
+    pub ld_grad_weight: usize,
+    pub grad_hidden_dtype: c_int,
+    pub grad_weight_dtype: c_int,
+}
+
+#[repr(C)]
 #[derive(Clone, Copy)]
 pub struct OrdaIpcHandle {
     pub bytes: [c_char; 64],
@@ -276,6 +300,12 @@ extern "C" {
                                       vs: *const OrdaVocabShard, all_partials: *const f32,
                                       out: *const OrdaDeviceOutputs, stream: *mut c_void,
                                       plan_out: *mut OrdaChunkPlan, err: *mut c_char, err_len: usize) -> c_int;
+
+    pub fn orda_linear_ce_options_default(out: *mut OrdaLinearCeOptions);
+    pub fn orda_linear_cross_entropy_device(ctx: *mut OrdaContext, hidden: *const OrdaDeviceMat,
+                                            weight: *const OrdaDeviceMat, labels: *const i64, bt: usize,
+                                            opts: *const OrdaLinearCeOptions, out: *const OrdaLinearCeOutputs,
+                                            stream: *mut c_void, err: *mut c_char, err_len: usize) -> c_int;
 
     pub fn orda_context_slots_create(ctx: *mut OrdaContext, world: c_int, rank: c_int, total_rows: usize, h: usize,
                                      copies: c_int, handle_out: *mut OrdaIpcHandle, err: *mut c_char,

@@ -1,0 +1,359 @@
+"""Linear cross entropy (orda_linear_cross_entropy_device) against its formula in 64 bits.
+
+Tolerances, from the arithmetic (u = half a step, relative: bf16 2^-8, fp32 2^-24):
+  logits    fp32 sums of H exact products: |dz| <= 2 H 2^-24 sum_k |h_k w_k| (twice the bound of a
+            rounded sum, for an accumulator that cuts instead of rounding); nll and lse move by at most
+            the largest two such errors, plus 2^-20 for the exponentials and the rounding of the result
+  dlogits   2^-8 |dz| for the rounding to bf16, 2^-10 ln 2 p g for the fixed-point logits, and the
+            logits' own error and 2^-18 (exponentials of arguments up to 64) in p g
+  gradients the sum of the dlogits' errors times |W| (or |h|), K 2^-23 for the fp32 sums, and half a
+            step of the output's type
+"""
+from __future__ import annotations
+
+import math
+
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+LN2 = math.log(2.0)
+
+
+@pytest.fixture(scope="module")
+def ctx():
+    from orda_b200.device import DeviceContext
+
+    with DeviceContext(0) as c:
+        yield c
+
+
+def make(bt, h, v, seed=0, ignored=0.0, std=0.5, ld=None, pull=0.0):
+    gen = torch.Generator(device="cuda").manual_seed(seed)
+    ld = ld or -(-h // 8) * 8
+    w = torch.zeros(v, ld, device="cuda", dtype=torch.bfloat16)[:, :h]
+    w.copy_(torch.randn(v, h, generator=gen, device="cuda") * (std / math.sqrt(h)))
+    labels = torch.randint(0, v, (bt,), generator=gen, device="cuda")
+    x = torch.zeros(bt, ld, device="cuda", dtype=torch.bfloat16)[:, :h]
+    x.copy_(torch.randn(bt, h, generator=gen, device="cuda") * 2.0 + pull * w[labels].float() * h)
+    if ignored:
+        labels[torch.rand(bt, generator=gen, device="cuda") < ignored] = -100
+    return x, w, labels
+
+
+def formula(x, w, labels, a=0.0, mean=True, denom=None, ignore=-100):
+    """loss, nll, lse, dh, dW and the error bounds of the last four, in 64 bits."""
+    live = labels != ignore
+    xd = torch.where(live[:, None], x.double(), 0.0)
+    wd = w.double()
+    v, h = wd.shape
+    z = xd @ wd.T
+    lse = torch.logsumexp(z, 1)
+    y = torch.where(live, labels, 0)
+    zy = z.gather(1, y[:, None])[:, 0]
+    nll = torch.where(live, lse - (1 - a) * zy - a * z.mean(1), 0.0)
+    n = denom or max(int(live.sum()), 1)
+    g = torch.where(live, 1.0 / n if mean else 1.0, 0.0)
+    p = torch.exp(z - lse[:, None])
+    dz = p - a / v
+    # the label's entry through 1 - p = the sum of the others: p itself may round to 1 in 64 bits
+    miss = p.scatter(1, y[:, None], 0.0).sum(1)
+    dz[torch.arange(len(y), device="cuda"), y] = a - a / v - miss
+    dz = dz * g[:, None]
+    dh, dw = dz @ wd, dz.T @ xd
+    ez = 2 * h * 2.0**-24 * (xd.abs() @ wd.abs().T).amax(1)
+    row_tol = 2 * ez + 2.0**-20 * (1 + lse.abs() + zy.abs() + z.abs().amax(1))
+    pg = p * g[:, None]
+    err = 2.0**-8 * dz.abs() + pg * (2.0**-10 * LN2 + 2.0**-18 + 3 * ez[:, None])
+    # the label's entry is formed from 1 - p
+    mag = dz.abs() + pg
+    dh_tol = err @ wd.abs() + 2.0**-23 * v * (mag @ wd.abs()) / max(1.0, math.sqrt(v))
+    dw_tol = err.T @ xd.abs() + 2.0**-23 * len(y) * (mag.T @ xd.abs())
+    return {"loss": nll.sum() / n if mean else nll.sum(), "nll": nll, "lse": torch.where(live, lse, 0.0), "dh": dh,
+            "dw": dw, "row_tol": row_tol, "dh_tol": dh_tol, "dw_tol": dw_tol, "dz": dz, "n": n}
+
+
+def check(r, f, mean=True):
+    assert torch.all((r.nll.double() - f["nll"]).abs() <= f["row_tol"] + 2.0**-23 * f["nll"].abs()), "nll"
+    assert torch.all((r.lse.double() - f["lse"]).abs() <= f["row_tol"] + 2.0**-23 * f["lse"].abs()), "lse"
+    tol = f["row_tol"].sum() / (f["n"] if mean else 1) + 2.0**-22 * f["loss"].abs()
+    assert (r.loss.double() - f["loss"]).abs() <= tol, (float(r.loss), float(f["loss"]))
+    for got, want, tol in ((r.grad_hidden, f["dh"], f["dh_tol"]), (r.grad_weight, f["dw"], f["dw_tol"])):
+        if got is None:
+            continue
+        step = 2.0**-8 if got.dtype == torch.bfloat16 else 2.0**-24
+        off = (got.double() - want).abs() - (tol + step * (want.abs() + tol) + 1e-38)
+        assert off.max() <= 0, (float(off.max()), float(want.abs().max()))
+
+
+def call(ctx, x, w, labels, a=0.0, mean=True, **kw):
+    import orda_b200 as ob
+    from orda_b200.device import linear_cross_entropy_device
+
+    r = linear_cross_entropy_device(ctx, x, w, labels, label_smoothing=a,
+                                    reduction=ob.Reduction.Mean if mean else ob.Reduction.Sum, **kw)
+    torch.cuda.synchronize()
+    ctx.check()
+    return r
+
+
+SHAPES = [(1, 8, 1), (1, 8, 2), (3, 16, 5), (1, 64, 1000), (2, 72, 127), (31, 64, 128), (33, 136, 129), (127, 128, 255),
+          (128, 256, 257), (129, 8, 513), (257, 1000, 1031), (300, 520, 4099), (640, 264, 2500)]
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("bt,h,v", SHAPES)
+def test_shapes(ctx, bt, h, v, dtype):
+    x, w, labels = make(bt, h, v, seed=bt + v)
+    check(call(ctx, x, w, labels, grad_dtype=dtype), formula(x, w, labels))
+
+
+@pytest.mark.parametrize("bt,h,v", [(33, 136, 129), (300, 520, 4099)])
+@pytest.mark.parametrize("a,mean,ignored", [(0.1, True, 0.0), (1.0, True, 0.3), (0.1, False, 0.5), (0.0, False, 0.9)])
+def test_options(ctx, bt, h, v, a, mean, ignored):
+    x, w, labels = make(bt, h, v, seed=7, ignored=ignored)
+    r = call(ctx, x, w, labels, a, mean, grad_dtype=torch.bfloat16)
+    check(r, formula(x, w, labels, a, mean), mean)
+    dead = labels == -100
+    assert torch.all(r.nll[dead] == 0) and torch.all(r.lse[dead] == 0) and torch.all(r.grad_hidden[dead] == 0)
+
+
+@pytest.mark.parametrize("piece_bytes", [1, 300 * 1024 * 2, 300 * 1600 * 2])
+@pytest.mark.parametrize("a", [0.0, 0.2])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_pieces(ctx, piece_bytes, a, dtype):
+    """The vocabulary in 9, 5 and 3 pieces (the last one narrow)."""
+    x, w, labels = make(300, 264, 4099, seed=3, ignored=0.2)
+    check(call(ctx, x, w, labels, a, grad_dtype=dtype, piece_bytes=piece_bytes), formula(x, w, labels, a))
+
+
+def test_odd_h_and_row_strides(ctx):
+    x, w, labels = make(70, 61, 333, seed=5, ld=72)
+    assert x.stride(0) == 72
+    check(call(ctx, x, w, labels, grad_dtype=torch.bfloat16), formula(x, w, labels))
+    # outputs that no TMA store can address
+    for dtype in (torch.bfloat16, torch.float32):
+        out = {"grad_hidden": torch.full((70, 67), 7.0, device="cuda", dtype=dtype)[:, 3:64],
+               "grad_weight": torch.full((333, 67), 7.0, device="cuda", dtype=dtype)[:, 3:64]}
+        full = {k: t._base for k, t in out.items()}
+        r = call(ctx, x, w, labels, out=out)
+        check(r, formula(x, w, labels))
+        for t in full.values():
+            assert torch.all(t[:, :3] == 7.0) and torch.all(t[:, 64:] == 7.0)
+
+
+@pytest.mark.parametrize("need_h,need_w", [(False, False), (True, False), (False, True)])
+def test_gradients_asked_for(ctx, need_h, need_w):
+    x, w, labels = make(130, 128, 1500, seed=9, ignored=0.1)
+    f = formula(x, w, labels)
+    for pieces in (0, 1):
+        r = call(ctx, x, w, labels, need_grad_hidden=need_h, need_grad_weight=need_w, piece_bytes=pieces)
+        assert (r.grad_hidden is not None) == need_h and (r.grad_weight is not None) == need_w
+        check(r, f)
+
+
+@pytest.mark.parametrize("piece_bytes", [0, 1])
+def test_far_labels(ctx, piece_bytes):
+    """Labels whose logit lies far below or above every other one: parts outside the fixed point's range."""
+    bt, h, v = 96, 64, 1200
+    gen = torch.Generator(device="cuda").manual_seed(2)
+    w = torch.zeros(v, h, device="cuda")
+    w[:, 0] = torch.linspace(-1, 1, v, device="cuda")
+    w[:, 1:] = torch.randn(v, h - 1, generator=gen, device="cuda") * 0.1
+    w = w.bfloat16()
+    x = torch.randn(bt, h, generator=gen, device="cuda")
+    x[:, 0] = torch.linspace(-150, 150, bt, device="cuda")  # logits up to +-150 (e^300 apart)
+    x = x.bfloat16()
+    labels = torch.randint(0, v, (bt,), generator=gen, device="cuda")
+    labels[::3] = 0
+    labels[1::3] = v - 1
+    r = call(ctx, x, w, labels, grad_dtype=torch.bfloat16, piece_bytes=piece_bytes)
+    check(r, formula(x, w, labels))
+    # rows that are all but certain: the gradient's scale is 1 - p, far below a rounding of p
+    sure = torch.zeros(4, h, device="cuda", dtype=torch.bfloat16)
+    sure[:, 0] = 40.0
+    lab = torch.full((4,), v - 1, device="cuda")
+    w2 = w.clone()
+    w2[:-1, 0] = -1.0
+    f = formula(sure, w2, lab)
+    r = call(ctx, sure, w2, lab, piece_bytes=piece_bytes)
+    rel = ((r.grad_hidden.double() - f["dh"]).norm() / f["dh"].norm()).item()
+    assert float(f["dh"].norm()) < 1e-25 and rel < 1e-2, rel
+    assert torch.allclose(r.nll.double(), f["nll"], rtol=1e-3, atol=0) or float(f["nll"].max()) < 1e-12
+
+
+def test_nothing_of_an_ignored_row_is_used(ctx):
+    x, w, labels = make(140, 96, 700, seed=4, ignored=0.4)
+    dead = labels == -100
+    clean = call(ctx, x, w, labels)
+    for bad in (float("nan"), float("inf"), -torch.finfo(torch.bfloat16).max):
+        y = x.clone()
+        y[dead] = bad
+        r = call(ctx, y, w, labels)
+        for n in ("loss", "nll", "lse", "grad_hidden", "grad_weight"):
+            assert torch.equal(getattr(r, n), getattr(clean, n)), (bad, n)
+
+
+def test_every_row_ignored(ctx):
+    x, w, labels = make(65, 64, 300)
+    labels.fill_(-100)
+    for a, mean in ((0.0, True), (0.1, False)):
+        r = call(ctx, x, w, labels, a, mean)
+        assert float(r.loss) == 0 and not r.grad_hidden.any() and not r.grad_weight.any() and not r.lse.any()
+
+
+def test_nan_of_a_live_row_shows(ctx):
+    x, w, labels = make(40, 64, 300)
+    x[3, 5] = float("nan")
+    r = call(ctx, x, w, labels)
+    assert torch.isnan(r.loss) and torch.isnan(r.nll[3]) and torch.isnan(r.grad_hidden[3]).all()
+    assert torch.isfinite(r.nll[[i for i in range(40) if i != 3]]).all()
+
+
+def test_lowest_value_logits(ctx):
+    """Vocabulary entries that are masked by a large negative logit."""
+    x, w, labels = make(64, 64, 640, seed=6)
+    x[:, 0] = 1.0
+    w[:, 0] = 0.0
+    w[128:384, 0] = -3.0e38
+    labels[(labels >= 128) & (labels < 384)] = 5
+    r = call(ctx, x, w, labels, grad_dtype=torch.bfloat16)
+    keep = torch.cat([torch.arange(128), torch.arange(384, 640)]).cuda()
+    sub = torch.full((640,), 0, device="cuda")
+    sub[keep] = torch.arange(len(keep), device="cuda")
+    f = formula(x, w[keep].contiguous(), sub[labels])
+    assert torch.all((r.nll.double() - f["nll"]).abs() <= f["row_tol"])
+    assert not r.grad_weight[128:384].any()
+    assert ((r.grad_weight[keep].double() - f["dw"]).norm() / f["dw"].norm()) < 5e-3
+
+
+def test_label_out_of_range_is_reported(ctx):
+    import orda_b200 as ob
+    from orda_b200 import _abi
+    from orda_b200.device import linear_cross_entropy_device
+
+    x, w, labels = make(40, 64, 300)
+    for bad in (300, -1):
+        labels[7] = bad
+        linear_cross_entropy_device(ctx, x, w, labels)
+        with pytest.raises(ob.OrdaError) as e:
+            ctx.check()
+        assert e.value.code == _abi.ORDA_ERR_LABEL
+    labels[7] = 2
+    check(call(ctx, x, w, labels), formula(x, w, labels))
+
+
+def test_own_ignore_index_and_denominator(ctx):
+    x, w, labels = make(90, 64, 300, seed=8)
+    labels[::4] = 17
+    r = call(ctx, x, w, labels, ignore_index=17)
+    check(r, formula(x, w, labels, ignore=17))
+    r = call(ctx, x, w, labels, global_non_ignore=1000)
+    check(r, formula(x, w, labels, denom=1000))
+
+
+def test_gradient_against_differences(ctx):
+    """Directional derivatives of the 64-bit loss by central differences."""
+    x, w, labels = make(50, 72, 401, seed=12, ignored=0.2)
+    r = call(ctx, x, w, labels, 0.1)
+    gen = torch.Generator(device="cuda").manual_seed(1)
+    for i in range(4):
+        dx = torch.randn(x.shape, generator=gen, device="cuda", dtype=torch.float64)
+        dw = torch.randn(w.shape, generator=gen, device="cuda", dtype=torch.float64) / 72
+        eps = 1e-4
+        up = formula(x.double() + eps * dx, w.double() + eps * dw, labels, 0.1)["loss"]
+        down = formula(x.double() - eps * dx, w.double() - eps * dw, labels, 0.1)["loss"]
+        f = formula(x, w, labels, 0.1)
+        want = float((up - down) / (2 * eps))
+        got = float((r.grad_hidden.double() * dx).sum() + (r.grad_weight.double() * dw).sum())
+        tol = float((f["dh_tol"] * dx.abs()).sum() + (f["dw_tol"] * dw.abs()).sum()) + 1e-6
+        assert abs(got - want) <= tol, (got, want, tol)
+
+
+def test_same_bits_twice_and_on_another_stream(ctx):
+    x, w, labels = make(520, 200, 9000, seed=10, ignored=0.1)
+    for piece in (0, 520 * 2048 * 2):
+        a = call(ctx, x, w, labels, piece_bytes=piece)
+        side = torch.cuda.Stream()
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            b = call(ctx, x, w, labels, piece_bytes=piece)
+        torch.cuda.current_stream().wait_stream(side)
+        for n in ("loss", "nll", "lse", "grad_hidden", "grad_weight"):
+            assert torch.equal(getattr(a, n), getattr(b, n)), n
+
+
+def test_captured_call_replays_after_the_workspace_grew(ctx):
+    from orda_b200.device import DeviceContext, linear_cross_entropy_device
+
+    x, w, labels = make(100, 128, 2000, seed=11)
+    with DeviceContext(0) as own:
+        graph = torch.cuda.CUDAGraph()
+        with pytest.raises(Exception, match="before the capture"):
+            with torch.cuda.graph(torch.cuda.CUDAGraph()):
+                linear_cross_entropy_device(own, x, w, labels)
+        torch.cuda.synchronize()
+        call(own, x, w, labels)
+        out = {"loss": torch.zeros(1, device="cuda"), "grad_hidden": torch.zeros(100, 128, device="cuda"),
+               "grad_weight": torch.zeros(2000, 128, device="cuda")}
+        with torch.cuda.graph(graph):
+            linear_cross_entropy_device(own, x, w, labels, out=out)
+        big = make(400, 256, 5000, seed=13)
+        call(own, *big)
+        for seed in (21, 22):
+            x2, w2, l2 = make(100, 128, 2000, seed=seed, ignored=0.3)
+            x.copy_(x2), w.copy_(w2), labels.copy_(l2)
+            graph.replay()
+            torch.cuda.synchronize()
+            eager = call(own, x, w, labels)
+            assert torch.equal(eager.grad_weight, out["grad_weight"])
+            assert torch.equal(eager.grad_hidden, out["grad_hidden"]) and float(out["loss"]) == float(eager.loss)
+        del graph
+
+
+def test_allocation_failures_make_smaller_pieces(ctx):
+    from orda_b200.device import DeviceContext
+
+    x, w, labels = make(64, 64, 3000, seed=14)
+    with DeviceContext(0) as own:
+        own.inject_alloc_failures(2)
+        check(call(own, x, w, labels), formula(x, w, labels))
+        own.inject_alloc_failures(100)
+        with pytest.raises(RuntimeError, match="workspace"):
+            call(own, x, w, labels)
+        own.inject_alloc_failures(0)
+
+
+def test_agrees_with_the_distillation_losss_student_term(ctx):
+    """kd = 0 and no teacher CE leave the distillation loss its student term."""
+    import orda_b200 as ob
+    from orda_b200.device import distillation_loss_device
+
+    x, w, labels = make(200, 128, 1500, seed=15, ignored=0.2)
+    d = distillation_loss_device(ctx, x, w, labels, ob.TeacherMode.Tied, teacher_hidden=x,
+                                 opts=ob.LossOptions(kd_weight=0.0, teacher_ce_weight=0.0, label_smoothing=0.1))
+    torch.cuda.synchronize()
+    r = call(ctx, x, w, labels, 0.1)
+    f = formula(x, w, labels, 0.1)
+    tol = float(f["row_tol"].max())
+    assert abs(float(d.scalars[1]) - float(r.loss)) <= 2 * tol
+    for a, b, t in ((d.grad_student_hidden, r.grad_hidden, f["dh_tol"]), (d.grad_weight, r.grad_weight, f["dw_tol"])):
+        assert torch.all((a.double() - b.double()).abs() <= 2 * t + 1e-30)
+
+
+@pytest.mark.parametrize("pull", [0.5, 0.05])
+@pytest.mark.parametrize("bt,h,v", [(2048, 1024, 12000), (700, 2048, 20011)])
+def test_larger_products(ctx, bt, h, v, pull):
+    """Full tiles, wide tiles and slabs; relative L2 of three bf16 roundings (1.6e-3 rms each) at most.
+    pull = 0.05 lifts the labels' logits by about 13 (H = 1024), 0.5 by 128: there the gradients are
+    about e^-128 = 2.6e-56, below what bf16 and fp32 hold, so an element may be off by 2^-126, where the
+    arithmetic flushes to zero."""
+    x, w, labels = make(bt, h, v, seed=16, pull=pull, ignored=0.1)
+    for piece in (0, bt * v // 2):
+        r = call(ctx, x, w, labels, grad_dtype=torch.bfloat16, piece_bytes=piece)
+        f = formula(x, w, labels)
+        check(r, f)
+        for got, want in ((r.grad_hidden, f["dh"]), (r.grad_weight, f["dw"])):
+            flushed = math.sqrt(want.numel()) * 2.0**-126
+            assert (got.double() - want).norm() < 1.6e-3 * math.sqrt(3) * want.norm() + flushed
