@@ -497,6 +497,36 @@ ORDA_API int orda_linear_cross_entropy_device(OrdaContext* ctx, const OrdaDevice
                                               const OrdaLinearCeOptions* opts, const OrdaLinearCeOutputs* out,
                                               void* stream, char* err, size_t err_len);
 
+/* Embedding, the other end of a table that a model shares with its output
+ * head (no counterpart in the reference, which starts at the hidden states):
+ *   out[i, :] = scale * table[ids[i], :]                      i < n
+ * rounded once to out's type. bf16 or f32 on either side, any leading
+ * dimension >= H and any alignment of the elements (16-byte aligned rows are
+ * fastest). An id outside [0, V) gives a row of zeros and is reported by the
+ * next orda_context_check. n = 0 does nothing. */
+typedef struct OrdaDeviceMatMut {
+  void* data;
+  size_t rows;
+  size_t cols;
+  size_t ld;
+  OrdaDType dtype;
+} OrdaDeviceMatMut;
+ORDA_API int orda_embedding_device(OrdaContext* ctx, const OrdaDeviceMat* table, const int64_t* ids, size_t n,
+                                   float scale, const OrdaDeviceMatMut* out, void* stream, char* err, size_t err_len);
+/* Its gradient: grad_table[v, :] = scale * sum over {i : ids[i] = v} of
+ * grad_out[i, :], summed in fp32 in the order of i for runs of tokens and then
+ * run by run (the same bits on every call); rows of the table that no token
+ * names become 0. accumulate = 1 adds to what grad_table holds instead and
+ * touches the named rows only: after orda_linear_cross_entropy_device or
+ * orda_distillation_loss_device that is the gradient of the shared table. With
+ * has_padding_id, tokens of padding_id give no gradient. Ids out of range give
+ * none and are reported by the next orda_context_check. Stream capture as for
+ * orda_linear_cross_entropy_device. */
+ORDA_API int orda_embedding_grad_device(OrdaContext* ctx, const OrdaDeviceMat* grad_out, const int64_t* ids, size_t n,
+                                        float scale, int has_padding_id, int64_t padding_id,
+                                        const OrdaDeviceMatMut* grad_table, int accumulate, void* stream, char* err,
+                                        size_t err_len);
+
 /* Fused grad_W reduce-scatter for row-sharded runs on the GPUs of one node
  * (up to 8 ranks, one process per GPU). There is no counterpart in the
  * reference, which runs on one device; for data-parallel callers that

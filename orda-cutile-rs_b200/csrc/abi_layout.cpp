@@ -132,6 +132,13 @@ const OrdaFieldLayout kLayout[] = {
     ORDA_FIELD(OrdaLinearCeOutputs, grad_hidden_dtype),
     ORDA_FIELD(OrdaLinearCeOutputs, grad_weight_dtype),
 
+    ORDA_STRUCT(OrdaDeviceMatMut),
+    ORDA_FIELD(OrdaDeviceMatMut, data),
+    ORDA_FIELD(OrdaDeviceMatMut, rows),
+    ORDA_FIELD(OrdaDeviceMatMut, cols),
+    ORDA_FIELD(OrdaDeviceMatMut, ld),
+    ORDA_FIELD(OrdaDeviceMatMut, dtype),
+
     ORDA_STRUCT(OrdaIpcHandle),
     ORDA_FIELD(OrdaIpcHandle, bytes),
 

@@ -1,0 +1,583 @@
+// embedding.cu -- embedding lookup with scaling and its gradient by sorted
+// tokens (orda_embedding_device, orda_embedding_grad_device).
+//
+//   forward   out[i, :] = s T[id_i, :]
+//   gradient  dT[v, :] (+)= s sum over {i : id_i = v} of dout[i, :], in the order of i
+//
+// Both are bound by bandwidth. The gradient needs no float atomics: the token
+// positions are sorted by id (stable), the sorted positions are cut into tiles
+// of equal length, and each tile adds up the runs of equal ids that it holds, in
+// fp32 and in order. A run inside one tile is complete and is written at
+// once; a run that crosses tiles leaves one partial sum per tile, which a second
+// kernel adds in tile order. Work per tile does not depend on how often an id
+// occurs, and the result's bits do not depend on timing.
+#include <cuda_bf16.h>
+#include <cuda_runtime.h>
+
+#include <algorithm>
+#include <cstdint>
+#include <mutex>
+
+#include "kernels.h"
+#include "ptx.cuh"
+
+namespace orda {
+namespace {
+
+// VEC neighbouring elements as floats and back; VEC * sizeof(T) bytes are
+// aligned to themselves, 16 bytes at most.
+template <typename T, int VEC>
+struct Vec {
+  static constexpr int BYTES = VEC * static_cast<int>(sizeof(T));
+  static constexpr int WORDS = BYTES >= 4 ? BYTES / 4 : 1;
+  uint32_t w[WORDS];
+  __device__ __forceinline__ void load(const T* p) {
+    if constexpr (BYTES >= 16) {
+#pragma unroll
+      for (int i = 0; i < BYTES / 16; ++i) {
+        const uint4 q = __ldg(reinterpret_cast<const uint4*>(p) + i);
+        w[4 * i] = q.x, w[4 * i + 1] = q.y, w[4 * i + 2] = q.z, w[4 * i + 3] = q.w;
+      }
+    } else if constexpr (BYTES == 8) {
+      const uint2 q = __ldg(reinterpret_cast<const uint2*>(p));
+      w[0] = q.x, w[1] = q.y;
+    } else if constexpr (BYTES == 4) {
+      w[0] = __ldg(reinterpret_cast<const uint32_t*>(p));
+    } else {
+      w[0] = __ldg(reinterpret_cast<const uint16_t*>(p));
+    }
+  }
+  // for what this kernel writes too
+  __device__ __forceinline__ void load_own(const T* p) {
+    if constexpr (BYTES >= 16) {
+#pragma unroll
+      for (int i = 0; i < BYTES / 16; ++i) {
+        const uint4 q = reinterpret_cast<const uint4*>(p)[i];
+        w[4 * i] = q.x, w[4 * i + 1] = q.y, w[4 * i + 2] = q.z, w[4 * i + 3] = q.w;
+      }
+    } else if constexpr (BYTES == 8) {
+      const uint2 q = *reinterpret_cast<const uint2*>(p);
+      w[0] = q.x, w[1] = q.y;
+    } else if constexpr (BYTES == 4) {
+      w[0] = *reinterpret_cast<const uint32_t*>(p);
+    } else {
+      w[0] = *reinterpret_cast<const uint16_t*>(p);
+    }
+  }
+  __device__ __forceinline__ void store(T* p) const {
+    if constexpr (BYTES >= 16) {
+#pragma unroll
+      for (int i = 0; i < BYTES / 16; ++i)
+        reinterpret_cast<uint4*>(p)[i] = make_uint4(w[4 * i], w[4 * i + 1], w[4 * i + 2], w[4 * i + 3]);
+    } else if constexpr (BYTES == 8) {
+      *reinterpret_cast<uint2*>(p) = make_uint2(w[0], w[1]);
+    } else if constexpr (BYTES == 4) {
+      *reinterpret_cast<uint32_t*>(p) = w[0];
+    } else {
+      *reinterpret_cast<uint16_t*>(p) = static_cast<uint16_t>(w[0]);
+    }
+  }
+  __device__ __forceinline__ float get(int i) const {
+    if constexpr (sizeof(T) == 4) return __uint_as_float(w[i]);
+    return __uint_as_float((i & 1) ? (w[i >> 1] & 0xffff0000u) : (w[i >> 1] << 16));
+  }
+  __device__ __forceinline__ void set(const float (&f)[VEC]) {
+    if constexpr (sizeof(T) == 4) {
+#pragma unroll
+      for (int i = 0; i < VEC; ++i) w[i] = __float_as_uint(f[i]);
+    } else if constexpr (VEC == 1) {
+      w[0] = __bfloat16_as_ushort(__float2bfloat16_rn(f[0]));
+    } else {
+#pragma unroll
+      for (int i = 0; i < VEC / 2; ++i) {
+        const __nv_bfloat162 h = __floats2bfloat162_rn(f[2 * i], f[2 * i + 1]);
+        w[i] = *reinterpret_cast<const uint32_t*>(&h);
+      }
+    }
+  }
+};
+
+// ---------------------------------------------------------------- forward
+
+// blockDim.x threads along a row, blockDim.y rows per block.
+template <typename TI, typename TO, int VEC>
+__global__ void __launch_bounds__(256)
+    embed_kernel(const TI* __restrict__ table, long long ld, long long v, long long h, const int64_t* __restrict__ ids,
+                 long long n, float scale, TO* __restrict__ out, long long ldo, int* bad) {
+  const long long i = static_cast<long long>(blockIdx.x) * blockDim.y + threadIdx.y;
+  if (i >= n) return;
+  const int64_t id = ids[i];
+  const bool ok = id >= 0 && id < v;
+  if (!ok && threadIdx.x == 0) atomicExch(bad, DEV_ID_RANGE);
+  const TI* src = table + (ok ? id : 0) * ld;
+  TO* dst = out + i * ldo;
+  const long long step = static_cast<long long>(blockDim.x) * VEC;
+  for (long long c0 = static_cast<long long>(threadIdx.x) * VEC; c0 < h; c0 += 4 * step) {
+    Vec<TI, VEC> x[4];
+#pragma unroll
+    for (int k = 0; k < 4; ++k)
+      if (c0 + k * step < h && ok) x[k].load(src + c0 + k * step);
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      if (c0 + k * step >= h) continue;
+      float f[VEC];
+#pragma unroll
+      for (int j = 0; j < VEC; ++j) f[j] = ok ? x[k].get(j) * scale : 0.f;
+      Vec<TO, VEC> y;
+      y.set(f);
+      y.store(dst + c0 + k * step);
+    }
+  }
+}
+
+// --------------------------------------------------------------- the sort
+
+// Stable radix sort of the ids with their positions by one cluster of eight
+// CTAs, 9 bits a pass (two passes up to 262144 ids). Each of the 256 warps owns a
+// contiguous range and a histogram of its own: counting and placing need no
+// atomics and no order between warps. The CTAs exchange their 512 digit totals
+// through distributed shared memory, so a pass is one launch-free step of a few
+// microseconds. Ids out of range and the padding id get the key v, which sorts
+// behind every row. The other clusters of the grid clear the gradient meanwhile.
+constexpr int kSortCtas = 8;
+constexpr int kSortThreads = 1024;
+constexpr int kSortWarps = kSortThreads / 32;
+constexpr int kDigits = 512;
+constexpr int kDigitBits = 9;
+constexpr size_t kSortSmem = (kSortWarps * kDigits + 2 * kDigits) * sizeof(uint32_t);
+
+struct SortArgs {
+  const int64_t* ids;
+  int n;
+  int v;
+  int64_t padding_id;
+  int has_padding;
+  int passes;
+  int2* buf0;  // (key, position); the sorted pairs end in buf[passes & 1 ? 1 : 0]
+  int2* buf1;
+  int* bad;
+  uint8_t* clear;  // gradient rows to clear (null: none)
+  long long clear_rows, clear_row_bytes, clear_ld_bytes;
+};
+
+__device__ __forceinline__ uint32_t ld_cluster_u32(uint32_t addr) {
+  uint32_t v;
+  asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(v) : "r"(addr) : "memory");
+  return v;
+}
+
+// Clears [p, p + bytes) with the threads [t, t + nt); 16-byte stores where aligned.
+__device__ void clear_span(uint8_t* p, long long bytes, long long t, long long nt) {
+  const long long head = min(bytes, static_cast<long long>((16 - (reinterpret_cast<uintptr_t>(p) & 15)) & 15));
+  const long long vecs = (bytes - head) / 16;
+  const long long tail = bytes - head - vecs * 16;
+  uint4* q = reinterpret_cast<uint4*>(p + head);
+#pragma unroll 4
+  for (long long i = t; i < vecs; i += nt) __stcs(q + i, make_uint4(0, 0, 0, 0));
+  uint16_t* h = reinterpret_cast<uint16_t*>(p);  // elements are 2 or 4 bytes
+  for (long long i = t; i < head / 2; i += nt) h[i] = 0;
+  uint16_t* e = reinterpret_cast<uint16_t*>(p + head + vecs * 16);
+  for (long long i = t; i < tail / 2; i += nt) e[i] = 0;
+}
+
+__global__ void __cluster_dims__(kSortCtas, 1, 1) __launch_bounds__(kSortThreads, 1) sort_kernel(const SortArgs a) {
+  if (blockIdx.x >= kSortCtas) {
+    const long long nb = gridDim.x - kSortCtas, b = blockIdx.x - kSortCtas;
+    if (a.clear_ld_bytes == a.clear_row_bytes) {
+      clear_span(a.clear, a.clear_rows * a.clear_row_bytes, b * kSortThreads + threadIdx.x, nb * kSortThreads);
+    } else {
+      for (long long r = b; r < a.clear_rows; r += nb)
+        clear_span(a.clear + r * a.clear_ld_bytes, a.clear_row_bytes, threadIdx.x, kSortThreads);
+    }
+    return;
+  }
+  extern __shared__ uint32_t sort_smem[];
+  uint32_t* hist = sort_smem;                         // [warps][digits]
+  uint32_t* total = hist + kSortWarps * kDigits;      // this CTA's digit totals
+  uint32_t* scan = total + kDigits;                   // scratch of the scan over digits
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const uint32_t rank = cluster_ctarank();
+  uint32_t* mine = hist + warp * kDigits;
+  const long long tiles = (static_cast<long long>(a.n) + 31) / 32;
+  const long long per = (tiles + kSortCtas * kSortWarps - 1) / (kSortCtas * kSortWarps);
+  const long long first = (static_cast<long long>(rank) * kSortWarps + warp) * per * 32;
+  const uint32_t below = (1u << lane) - 1;
+
+  auto fetch = [&](int pass, long long i) -> int2 {
+    if (pass > 0) return __ldcg((pass & 1 ? a.buf1 : a.buf0) + i);
+    const int64_t id = a.ids[i];
+    const bool pad = a.has_padding && id == a.padding_id;
+    const bool ok = id >= 0 && id < a.v;
+    if (!ok && !pad) atomicExch(a.bad, DEV_ID_RANGE);
+    return make_int2(ok && !pad ? static_cast<int>(id) : a.v, static_cast<int>(i));
+  };
+
+  for (int pass = 0; pass < a.passes; ++pass) {
+    const int shift = pass * kDigitBits;
+    int2* dst = pass & 1 ? a.buf0 : a.buf1;
+    for (int d = lane; d < kDigits; d += 32) mine[d] = 0;
+    __syncwarp();
+    for (long long t = 0; t < per; ++t) {
+      const long long i = first + t * 32 + lane;
+      const bool in = i < a.n;
+      const int2 kv = in ? fetch(pass, i) : make_int2(0, 0);
+      const uint32_t d = in ? (static_cast<uint32_t>(kv.x) >> shift) & (kDigits - 1) : kDigits;
+      const uint32_t same = __match_any_sync(0xffffffffu, d);
+      if (in && (same & below) == 0) mine[d] += __popc(same);
+      __syncwarp();
+    }
+    __syncthreads();
+    // counts -> offsets among the CTA's warps, and the CTA's totals
+    if (threadIdx.x < kDigits) {
+      uint32_t s = 0;
+#pragma unroll 8
+      for (int w = 0; w < kSortWarps; ++w) {
+        const uint32_t c = hist[w * kDigits + threadIdx.x];
+        hist[w * kDigits + threadIdx.x] = s;
+        s += c;
+      }
+      total[threadIdx.x] = s;
+    }
+    __syncthreads();
+    cluster_sync();
+    uint32_t before = 0, all = 0;
+    if (threadIdx.x < kDigits) {
+#pragma unroll
+      for (uint32_t r = 0; r < kSortCtas; ++r) {
+        const uint32_t c = ld_cluster_u32(mapa_shared(smem_u32(&total[threadIdx.x]), r));
+        if (r < rank) before += c;
+        all += c;
+      }
+      scan[threadIdx.x] = all;
+    }
+    __syncthreads();
+    // inclusive scan over the digits: within warps, then the warps' sums
+    uint32_t inc = all;
+    if (threadIdx.x < kDigits) {
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const uint32_t up = __shfl_up_sync(0xffffffffu, inc, o);
+        if (lane >= o) inc += up;
+      }
+      if (lane == 31) scan[warp] = inc;
+    }
+    __syncthreads();
+    if (threadIdx.x < kDigits) {
+      uint32_t start = inc - all + before;
+      for (int w = 0; w < warp; ++w) start += scan[w];
+#pragma unroll 8
+      for (int w = 0; w < kSortWarps; ++w) hist[w * kDigits + threadIdx.x] += start;
+    }
+    __syncthreads();
+    for (long long t = 0; t < per; ++t) {
+      const long long i = first + t * 32 + lane;
+      const bool in = i < a.n;
+      const int2 kv = in ? fetch(pass, i) : make_int2(0, 0);
+      const uint32_t d = in ? (static_cast<uint32_t>(kv.x) >> shift) & (kDigits - 1) : kDigits;
+      const uint32_t same = __match_any_sync(0xffffffffu, d);
+      if (in) __stcg(dst + mine[d] + __popc(same & below), kv);
+      __syncwarp();
+      if (in && (same & below) == 0) mine[d] += __popc(same);
+      __syncwarp();
+    }
+    // the pairs are placed, and no CTA reads another's totals any more
+    __threadfence();
+    cluster_sync();
+  }
+}
+
+// ------------------------------------------------------------ the gradient
+
+struct GradArgs {
+  const int2* sorted;  // (key, position) by key, n of them
+  int n, v, len;       // len: sorted positions per tile
+  int tiles;
+  const void* g;
+  long long ldg;
+  long long h;
+  float scale;
+  void* out;
+  long long ldo;
+  int accumulate;
+  float* part;  // [tiles][2][ldp]: a tile's first run when it began before, its last run when it goes on
+  long long ldp;
+};
+
+template <typename TO, int VEC>
+__device__ __forceinline__ void put_row(const GradArgs& a, int key, long long c, const float (&s)[VEC]) {
+  TO* dst = static_cast<TO*>(a.out) + key * a.ldo + c;
+  float f[VEC];
+#pragma unroll
+  for (int j = 0; j < VEC; ++j) f[j] = s[j] * a.scale;
+  Vec<TO, VEC> y;
+  if (a.accumulate) {
+    Vec<TO, VEC> old;
+    old.load_own(dst);
+#pragma unroll
+    for (int j = 0; j < VEC; ++j) f[j] += old.get(j);
+  }
+  y.set(f);
+  y.store(dst);
+}
+
+// One tile per threadIdx.y: its sorted positions in order, eight rows of
+// grad_out in flight per thread.
+constexpr int kBatch = 8;
+
+template <typename TI, typename TO, int VEC>
+__global__ void __launch_bounds__(256) grad_tiles_kernel(const GradArgs a) {
+  const int tile = blockIdx.x * blockDim.y + threadIdx.y;
+  const long long c = (static_cast<long long>(blockIdx.y) * blockDim.x + threadIdx.x) * VEC;
+  if (tile >= a.tiles || c >= a.h) return;
+  const int p0 = tile * a.len, p1 = min(a.n, p0 + a.len);
+  const int before = p0 > 0 ? a.sorted[p0 - 1].x : -1;
+  const int after = p1 < a.n ? a.sorted[p1].x : -1;
+  float s[VEC];
+#pragma unroll
+  for (int j = 0; j < VEC; ++j) s[j] = 0.f;
+  int key = a.sorted[p0].x;
+  bool open_left = key == before;  // the current run began in an earlier tile
+  float* part = a.part + static_cast<long long>(tile) * 2 * a.ldp + c;
+  auto put_part = [&](int which) {
+    float* d = part + which * a.ldp;
+#pragma unroll
+    for (int j = 0; j < VEC; ++j) d[j] = s[j];
+  };
+  for (int p = p0; p < p1; p += kBatch) {
+    int2 kv[kBatch];
+    Vec<TI, VEC> x[kBatch];
+#pragma unroll
+    for (int k = 0; k < kBatch; ++k) kv[k] = p + k < p1 ? a.sorted[p + k] : make_int2(a.v, 0);
+#pragma unroll
+    for (int k = 0; k < kBatch; ++k)
+      if (kv[k].x < a.v) x[k].load(static_cast<const TI*>(a.g) + kv[k].y * a.ldg + c);
+#pragma unroll
+    for (int k = 0; k < kBatch; ++k) {
+      if (p + k >= p1) break;
+      if (kv[k].x != key) {
+        if (open_left) put_part(0);
+        else put_row<TO, VEC>(a, key, c, s);
+        open_left = false;
+        key = kv[k].x;
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) s[j] = 0.f;
+      }
+      if (kv[k].x >= a.v) return;  // padding and bad ids end the sorted list
+#pragma unroll
+      for (int j = 0; j < VEC; ++j) s[j] += x[k].get(j);
+    }
+  }
+  if (open_left) put_part(0);
+  else if (key == after) put_part(1);
+  else put_row<TO, VEC>(a, key, c, s);
+}
+
+// Runs that cross tiles: the tile in which a run begins adds its own partial
+// sum (slot 1) and the following tiles' (slot 0), split over the block's
+// threadIdx.y groups in contiguous parts that are added in order.
+template <typename TO, int VEC>
+__global__ void __launch_bounds__(256) grad_runs_kernel(const GradArgs a) {
+  const int tile = blockIdx.x;
+  const long long c = (static_cast<long long>(blockIdx.y) * blockDim.x + threadIdx.x) * VEC;
+  const int p0 = tile * a.len, p1 = p0 + a.len;
+  if (p1 >= a.n) return;
+  const int key = a.sorted[p1 - 1].x;
+  if (key >= a.v || a.sorted[p1].x != key) return;      // the last run ends here
+  if (a.sorted[p0].x == key && p0 > 0 && a.sorted[p0 - 1].x == key) return;  // it began earlier
+  // tiles [tile + 1, last] hold the rest of the run: the last tile whose first key is this one
+  int lo = tile + 1, hi = a.tiles - 1;
+  while (lo < hi) {
+    const int mid = (lo + hi + 1) >> 1;
+    if (a.sorted[mid * a.len].x == key) lo = mid;
+    else hi = mid - 1;
+  }
+  const int count = lo - tile + 1;  // partial sums, this tile's included
+  const int each = (count + blockDim.y - 1) / blockDim.y;
+  const int k0 = threadIdx.y * each, k1 = min(count, k0 + each);
+  float s[VEC];
+#pragma unroll
+  for (int j = 0; j < VEC; ++j) s[j] = 0.f;
+  if (c < a.h) {
+#pragma unroll 4
+    for (int k = k0; k < k1; ++k) {
+      const float* d = a.part + (static_cast<long long>(tile + k) * 2 + (k == 0 ? 1 : 0)) * a.ldp + c;
+#pragma unroll
+      for (int j = 0; j < VEC; ++j) s[j] += d[j];
+    }
+  }
+  extern __shared__ float run_smem[];  // [blockDim.y][blockDim.x][VEC]
+  float* sh = run_smem + (threadIdx.y * blockDim.x + threadIdx.x) * VEC;
+#pragma unroll
+  for (int j = 0; j < VEC; ++j) sh[j] = s[j];
+  __syncthreads();
+  if (threadIdx.y != 0 || c >= a.h) return;
+  for (int y = 1; y < static_cast<int>(blockDim.y); ++y)
+#pragma unroll
+    for (int j = 0; j < VEC; ++j) s[j] += run_smem[(y * blockDim.x + threadIdx.x) * VEC + j];
+  put_row<TO, VEC>(a, key, c, s);
+}
+
+// Largest VEC (8, 4, 2, 1 elements) such that rows and their pieces are
+// aligned for both matrices: VEC divides h, and VEC elements (at most 16 bytes
+// of them at a time) divide the address and the leading dimension.
+int pick_vec(long long h, const void* a, long long lda, int esa, const void* b, long long ldb, int esb) {
+  for (int vec = 8; vec > 1; vec /= 2) {
+    auto ok = [vec](const void* p, long long ld, int es) {
+      const long long bytes = std::min(16, vec * es);
+      return reinterpret_cast<uintptr_t>(p) % bytes == 0 && ld * es % bytes == 0;
+    };
+    if (h % vec == 0 && ok(a, lda, esa) && ok(b, ldb, esb)) return vec;
+  }
+  return 1;
+}
+
+// Threads along a row: a power of two, at least a warp, no more than 256 or than the row needs.
+int row_threads(long long h, int vec) {
+  int x = 32;
+  while (x < 256 && static_cast<long long>(x) * vec < h) x *= 2;
+  return x;
+}
+
+template <typename TI, typename TO, int VEC>
+void embed_t(const EmbedArgs& a, cudaStream_t st) {
+  const int x = row_threads(a.h, VEC), y = 256 / x;
+  embed_kernel<TI, TO, VEC><<<static_cast<unsigned>((a.n + y - 1) / y), dim3(x, y), 0, st>>>(
+      static_cast<const TI*>(a.table), a.ld, a.v, a.h, a.ids, a.n, a.scale, static_cast<TO*>(a.out), a.ldo, a.bad);
+}
+
+template <typename TI, typename TO, int VEC>
+void grad_t(const GradArgs& a, cudaStream_t st) {
+  const int x = row_threads(a.h, VEC), y = 256 / x;
+  const unsigned cols = static_cast<unsigned>((a.h + static_cast<long long>(x) * VEC - 1) / (static_cast<long long>(x) * VEC));
+  grad_tiles_kernel<TI, TO, VEC><<<dim3((a.tiles + y - 1) / y, cols), dim3(x, y), 0, st>>>(a);
+  if (a.tiles < 2) return;
+  // 32 threads along the row, 8 groups along the run
+  const unsigned run_cols = static_cast<unsigned>((a.h + 32 * VEC - 1) / (32 * VEC));
+  grad_runs_kernel<TO, VEC><<<dim3(a.tiles - 1, run_cols), dim3(32, 8), 256 * VEC * sizeof(float), st>>>(a);
+}
+
+template <typename F>
+void by_types(int in_bf16, int out_bf16, int vec, const F& f) {
+  auto go = [&](auto ti, auto to) {
+    using TI = decltype(ti);
+    using TO = decltype(to);
+    if (vec == 8) f.template operator()<TI, TO, 8>();
+    else if (vec == 4) f.template operator()<TI, TO, 4>();
+    else if (vec == 2) f.template operator()<TI, TO, 2>();
+    else f.template operator()<TI, TO, 1>();
+  };
+  if (in_bf16 && out_bf16) go(uint16_t{}, uint16_t{});
+  else if (in_bf16) go(uint16_t{}, float{});
+  else if (out_bf16) go(float{}, uint16_t{});
+  else go(float{}, float{});
+}
+
+struct EmbedCall {
+  const EmbedArgs& a;
+  cudaStream_t st;
+  template <typename TI, typename TO, int VEC>
+  void operator()() const {
+    embed_t<TI, TO, VEC>(a, st);
+  }
+};
+struct GradCall {
+  const GradArgs& a;
+  cudaStream_t st;
+  template <typename TI, typename TO, int VEC>
+  void operator()() const {
+    grad_t<TI, TO, VEC>(a, st);
+  }
+};
+
+// Sorted positions per tile: long tiles leave fewer partial sums, short ones
+// give few tokens enough blocks.
+int tile_len(long long n) { return n >= 8192 ? 32 : n >= 2048 ? 16 : 8; }
+
+struct EmbedGradLayout {
+  size_t buf0, buf1, part, total;
+  long long ldp;
+  int tiles, len;
+};
+EmbedGradLayout grad_layout(long long n, long long h) {
+  EmbedGradLayout L;
+  auto up = [](size_t x) { return (x + 255) / 256 * 256; };
+  L.len = tile_len(n);
+  L.tiles = static_cast<int>((n + L.len - 1) / L.len);
+  L.ldp = (h + 7) / 8 * 8;
+  L.buf0 = 0;
+  L.buf1 = up(n * sizeof(int2));
+  L.part = L.buf1 + up(n * sizeof(int2));
+  L.total = L.part + up(static_cast<size_t>(L.tiles) * 2 * L.ldp * sizeof(float));
+  return L;
+}
+
+}  // namespace
+
+void launch_embed(const EmbedArgs& a, cudaStream_t st) {
+  if (a.n == 0 || a.h == 0) return;
+  const int vec = pick_vec(a.h, a.table, a.ld, a.in_bf16 ? 2 : 4, a.out, a.ldo, a.out_bf16 ? 2 : 4);
+  by_types(a.in_bf16, a.out_bf16, vec, EmbedCall{a, st});
+}
+
+size_t embed_grad_workspace(long long n, long long h) { return grad_layout(n, h).total; }
+
+cudaError_t launch_embed_grad(const EmbedGradArgs& a, void* ws, int num_sms, cudaStream_t st, int* launches) {
+  if (a.n == 0 && a.accumulate) return cudaSuccess;
+  const int es_out = a.out_bf16 ? 2 : 4;
+  const EmbedGradLayout L = grad_layout(a.n, a.h);
+  uint8_t* w = static_cast<uint8_t*>(ws);
+  SortArgs s{};
+  s.ids = a.ids;
+  s.n = static_cast<int>(a.n);
+  s.v = static_cast<int>(a.v);
+  s.padding_id = a.padding_id;
+  s.has_padding = a.has_padding;
+  int bits = 1;
+  while ((a.v >> bits) != 0) ++bits;  // keys 0..v
+  s.passes = (bits + kDigitBits - 1) / kDigitBits;
+  s.buf0 = reinterpret_cast<int2*>(w + L.buf0);
+  s.buf1 = reinterpret_cast<int2*>(w + L.buf1);
+  s.bad = a.bad;
+  unsigned clusters = 1;
+  if (!a.accumulate) {
+    s.clear = static_cast<uint8_t*>(a.out);
+    s.clear_rows = a.v;
+    s.clear_row_bytes = a.h * es_out;
+    s.clear_ld_bytes = a.ldo * es_out;
+    // a small gradient needs few SMs; 64 KB each keep a CTA's threads busy
+    const long long want = (a.v * a.h * es_out + (65536ll * kSortCtas) - 1) / (65536ll * kSortCtas);
+    clusters += static_cast<unsigned>(std::max<long long>(1, std::min<long long>(want, num_sms / kSortCtas - 1)));
+  }
+  static std::once_flag once[64];
+  int dev = 0;
+  cudaGetDevice(&dev);
+  cudaError_t e = cudaSuccess;
+  std::call_once(once[dev & 63], [&] {
+    e = cudaFuncSetAttribute(sort_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(kSortSmem));
+  });
+  if (e != cudaSuccess) return e;
+  sort_kernel<<<clusters * kSortCtas, kSortThreads, kSortSmem, st>>>(s);
+  *launches += 1;
+  if (a.n == 0) return cudaGetLastError();
+  GradArgs g{};
+  g.sorted = s.passes & 1 ? s.buf1 : s.buf0;
+  g.n = s.n;
+  g.v = s.v;
+  g.len = L.len;
+  g.tiles = L.tiles;
+  g.g = a.g;
+  g.ldg = a.ldg;
+  g.h = a.h;
+  g.scale = a.scale;
+  g.out = a.out;
+  g.ldo = a.ldo;
+  g.accumulate = a.accumulate;
+  g.part = reinterpret_cast<float*>(w + L.part);
+  g.ldp = L.ldp;
+  const int vec = pick_vec(a.h, a.g, a.ldg, a.in_bf16 ? 2 : 4, a.out, a.ldo, es_out);
+  by_types(a.in_bf16, a.out_bf16, vec, GradCall{g, st});
+  *launches += L.tiles > 1 ? 2 : 1;
+  return cudaGetLastError();
+}
+
+}  // namespace orda

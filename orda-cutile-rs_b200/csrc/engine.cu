@@ -1212,11 +1212,17 @@ bool device_is_sm100(int dev) {
 }
 
 int check_status(OrdaContext* ctx, char* err, size_t len) {
-  int words[2] = {0, 0};
+  int words[4] = {0, 0, 0, 0};
   cudaError_t e = cudaStreamSynchronize(ctx->last_stream);
   if (e != cudaSuccess) return cuda_fail(e, "stream synchronize", err, len);
   e = cudaMemcpy(words, ctx->d_words, sizeof words, cudaMemcpyDeviceToHost);
   if (e != cudaSuccess) return cuda_fail(e, "status read", err, len);
+  if (words[3] != DEV_OK) {
+    // kept across calls until it is reported here
+    if ((e = cudaMemset(ctx->d_words + 3, 0, sizeof(int))) != cudaSuccess) return cuda_fail(e, "memset", err, len);
+    set_error(err, len, "a token id is out of range [0, V) (device id check)");
+    return ORDA_ERR_LABEL;
+  }
   if (words[0] == DEV_LABEL_RANGE) {
     set_error(err, len, "a label is out of range [0, V) and != ignore_index (device label check)");
     return ORDA_ERR_LABEL;
@@ -1775,6 +1781,116 @@ int orda_linear_cross_entropy_device(OrdaContext* ctx, const OrdaDeviceMat* hidd
   std::lock_guard<std::mutex> lock(ctx->mu);
   DeviceScope dev(ctx->device);
   return run_linear_ce(ctx, *hidden, *weight, labels, bt, *opts, *out, static_cast<cudaStream_t>(stream), err, err_len);
+}
+
+static bool elem_mat_ok(const void* data, size_t rows, size_t cols, size_t ld, OrdaDType dt) {
+  if (dt != ORDA_DTYPE_BF16 && dt != ORDA_DTYPE_F32) return false;
+  if (!data && rows > 0) return false;
+  return ld >= cols && reinterpret_cast<uintptr_t>(data) % (dt == ORDA_DTYPE_BF16 ? 2 : 4) == 0;
+}
+
+// Sizes and scale of the two embedding entries.
+static int embedding_args_ok(size_t v, size_t h, size_t n, const int64_t* ids, float scale, char* err, size_t err_len) {
+  constexpr size_t kMax = size_t{1} << 30;  // positions and keys are 32-bit
+  if (v == 0 || h == 0 || v > kMax || h > kMax || n > kMax) {
+    set_error(err, err_len, "V and H must be in [1, 2^30] and n at most 2^30, got %zu, %zu and %zu", v, h, n);
+    return ORDA_ERR_INVALID;
+  }
+  if (n > 0 && !ids) {
+    set_error(err, err_len, "null argument");
+    return ORDA_ERR_INVALID;
+  }
+  if (!(scale - scale == 0.0f)) {
+    set_error(err, err_len, "scale must be finite, got %s", fmt_f32(scale).c_str());
+    return ORDA_ERR_INVALID;
+  }
+  return ORDA_OK;
+}
+
+int orda_embedding_device(OrdaContext* ctx, const OrdaDeviceMat* table, const int64_t* ids, size_t n, float scale,
+                          const OrdaDeviceMatMut* out, void* stream, char* err, size_t err_len) {
+  if (!ctx || !table || !out) {
+    set_error(err, err_len, "null argument");
+    return ORDA_ERR_INVALID;
+  }
+  if (int rc = embedding_args_ok(table->rows, table->cols, n, ids, scale, err, err_len)) return rc;
+  if (out->rows != n || out->cols != table->cols) {
+    set_error(err, err_len, "out must be (%zu, %zu), got (%zu, %zu)", n, table->cols, out->rows, out->cols);
+    return ORDA_ERR_INVALID;
+  }
+  if (!elem_mat_ok(table->data, table->rows, table->cols, table->ld, table->dtype) ||
+      !elem_mat_ok(out->data, out->rows, out->cols, out->ld, out->dtype)) {
+    set_error(err, err_len, "table and out must be bf16 or f32, with ld >= H");
+    return ORDA_ERR_INVALID;
+  }
+  std::lock_guard<std::mutex> lock(ctx->mu);
+  DeviceScope dev(ctx->device);
+  EmbedArgs a;
+  a.table = table->data;
+  a.ld = static_cast<long long>(table->ld);
+  a.v = static_cast<long long>(table->rows);
+  a.h = static_cast<long long>(table->cols);
+  a.in_bf16 = table->dtype == ORDA_DTYPE_BF16;
+  a.out_bf16 = out->dtype == ORDA_DTYPE_BF16;
+  a.ids = ids;
+  a.n = static_cast<long long>(n);
+  a.scale = scale;
+  a.out = out->data;
+  a.ldo = static_cast<long long>(out->ld);
+  a.bad = ctx->d_words + 3;
+  ctx->last_stream = static_cast<cudaStream_t>(stream);
+  if (n == 0) return ORDA_OK;
+  launch_embed(a, static_cast<cudaStream_t>(stream));
+  ctx->launches += 1;
+  const cudaError_t e = cudaGetLastError();
+  return e == cudaSuccess ? ORDA_OK : cuda_fail(e, "embedding", err, err_len);
+}
+
+int orda_embedding_grad_device(OrdaContext* ctx, const OrdaDeviceMat* grad_out, const int64_t* ids, size_t n,
+                               float scale, int has_padding_id, int64_t padding_id, const OrdaDeviceMatMut* grad_table,
+                               int accumulate, void* stream, char* err, size_t err_len) {
+  if (!ctx || !grad_out || !grad_table) {
+    set_error(err, err_len, "null argument");
+    return ORDA_ERR_INVALID;
+  }
+  if (int rc = embedding_args_ok(grad_table->rows, grad_table->cols, n, ids, scale, err, err_len)) return rc;
+  if (grad_out->rows != n || grad_out->cols != grad_table->cols) {
+    set_error(err, err_len, "grad_out must be (%zu, %zu), got (%zu, %zu)", n, grad_table->cols, grad_out->rows,
+              grad_out->cols);
+    return ORDA_ERR_INVALID;
+  }
+  if (!elem_mat_ok(grad_out->data, grad_out->rows, grad_out->cols, grad_out->ld, grad_out->dtype) ||
+      !elem_mat_ok(grad_table->data, grad_table->rows, grad_table->cols, grad_table->ld, grad_table->dtype)) {
+    set_error(err, err_len, "grad_out and grad_table must be bf16 or f32, with ld >= H");
+    return ORDA_ERR_INVALID;
+  }
+  std::lock_guard<std::mutex> lock(ctx->mu);
+  DeviceScope dev(ctx->device);
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  EmbedGradArgs a;
+  a.g = grad_out->data;
+  a.ldg = static_cast<long long>(grad_out->ld);
+  a.v = static_cast<long long>(grad_table->rows);
+  a.h = static_cast<long long>(grad_table->cols);
+  a.in_bf16 = grad_out->dtype == ORDA_DTYPE_BF16;
+  a.out_bf16 = grad_table->dtype == ORDA_DTYPE_BF16;
+  a.ids = ids;
+  a.n = static_cast<long long>(n);
+  a.scale = scale;
+  a.has_padding = has_padding_id;
+  a.padding_id = padding_id;
+  a.out = grad_table->data;
+  a.ldo = static_cast<long long>(grad_table->ld);
+  a.accumulate = accumulate;
+  a.bad = ctx->d_words + 3;
+  ctx->vocab_ready = false;  // the workspace no longer holds a vocabulary forward phase
+  bool capturing = false;
+  if (int rc = call_ws(ctx, embed_grad_workspace(a.n, a.h), st, &capturing, err, err_len)) return rc;
+  int nl = 0;
+  const cudaError_t e = launch_embed_grad(a, ctx->ws, ctx->num_sms, st, &nl);
+  ctx->launches += static_cast<uint64_t>(nl);
+  ctx->last_stream = st;
+  return e == cudaSuccess ? ORDA_OK : cuda_fail(e, "embedding gradient", err, err_len);
 }
 
 int orda_quantize_grad_w_device(OrdaContext* ctx, float* grad_w, size_t v, size_t h, size_t ld, const int64_t* labels,

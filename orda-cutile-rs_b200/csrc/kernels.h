@@ -147,6 +147,37 @@ void launch_ce_rewrite(const CeArgs& a, uint16_t* piece, long long ld, long long
 void launch_slab_sum(const float* buf, int slabs, long long slab_rows, long long ldb, long long rows, long long cols,
                      void* out, long long ldo, int out_bf16, cudaStream_t stream);
 
+// ---------------------------------------------------- embedding (embedding.cu)
+struct EmbedArgs {
+  const void* table = nullptr;  // [v, h]
+  long long ld = 0, v = 0, h = 0;
+  int in_bf16 = 0, out_bf16 = 0;
+  const int64_t* ids = nullptr;
+  long long n = 0;
+  float scale = 1.0f;
+  void* out = nullptr;  // [n, h]
+  long long ldo = 0;
+  int* bad = nullptr;  // set to DEV_ID_RANGE for an id outside [0, v)
+};
+void launch_embed(const EmbedArgs& a, cudaStream_t st);
+
+struct EmbedGradArgs {
+  const void* g = nullptr;  // [n, h]
+  long long ldg = 0, v = 0, h = 0;
+  int in_bf16 = 0, out_bf16 = 0;
+  const int64_t* ids = nullptr;
+  long long n = 0;
+  float scale = 1.0f;
+  int has_padding = 0;
+  int64_t padding_id = 0;
+  void* out = nullptr;  // [v, h]
+  long long ldo = 0;
+  int accumulate = 0;
+  int* bad = nullptr;
+};
+size_t embed_grad_workspace(long long n, long long h);
+cudaError_t launch_embed_grad(const EmbedGradArgs& a, void* ws, int num_sms, cudaStream_t st, int* launches);
+
 // ------------------------------------------------------------ row kernels
 // Element type of a logits buffer the row kernels read.
 enum LogitType : int { kLogitF32 = 0, kLogitBF16 = 1, kLogitF16 = 2 };

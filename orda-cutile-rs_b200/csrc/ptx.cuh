@@ -24,6 +24,7 @@ enum DeviceStatus : int {
   DEV_TIMEOUT_EPILOGUE = 0x103,
   DEV_TIMEOUT_DRAIN = 0x104,
   DEV_LABEL_RANGE = 0x201,
+  DEV_ID_RANGE = 0x202,
   DEV_TIMEOUT_SELFTEST = 0x301,
 };
 

@@ -166,6 +166,16 @@ class OrdaLinearCeOutputs(C.Structure):
     ]
 
 
+class OrdaDeviceMatMut(C.Structure):
+    _fields_ = [
+        ("data", C.c_void_p),
+        ("rows", C.c_size_t),
+        ("cols", C.c_size_t),
+        ("ld", C.c_size_t),
+        ("dtype", C.c_int),
+    ]
+
+
 class OrdaIpcHandle(C.Structure):
     _fields_ = [("bytes", C.c_ubyte * 64)]  # opaque; c_ubyte so no NUL truncation
 
@@ -256,6 +266,12 @@ SIGNATURES = {
         C.c_int,
         [C.c_void_p, C.POINTER(OrdaDeviceMat), C.POINTER(OrdaDeviceMat), C.c_void_p, C.c_size_t,
          C.POINTER(OrdaLinearCeOptions), C.POINTER(OrdaLinearCeOutputs), C.c_void_p, C.c_char_p, C.c_size_t]),
+    "orda_embedding_device": (
+        C.c_int, [C.c_void_p, C.POINTER(OrdaDeviceMat), C.c_void_p, C.c_size_t, C.c_float, C.POINTER(OrdaDeviceMatMut),
+                  C.c_void_p, C.c_char_p, C.c_size_t]),
+    "orda_embedding_grad_device": (
+        C.c_int, [C.c_void_p, C.POINTER(OrdaDeviceMat), C.c_void_p, C.c_size_t, C.c_float, C.c_int, C.c_int64,
+                  C.POINTER(OrdaDeviceMatMut), C.c_int, C.c_void_p, C.c_char_p, C.c_size_t]),
     "orda_context_slots_create": (
         C.c_int, [C.c_void_p, C.c_int, C.c_int, C.c_size_t, C.c_size_t, C.c_int, C.POINTER(OrdaIpcHandle),
                   C.c_char_p, C.c_size_t]),

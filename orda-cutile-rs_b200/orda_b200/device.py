@@ -466,6 +466,106 @@ def linear_cross_entropy_device(
     return LinearCrossEntropyResult(loss=loss.view(-1)[0], nll=vectors["nll"], lse=vectors["lse"], **grads)
 
 
+def _ids(ids: torch.Tensor) -> torch.Tensor:
+    if ids.dtype != torch.int64 or not ids.is_contiguous():
+        raise ValueError("ids must be contiguous int64")
+    return ids
+
+
+def _rows_of(t: torch.Tensor, n: int, h: int, name: str) -> torch.Tensor:
+    """t [..., h] as [n, h] without a copy."""
+    if t.dim() < 1 or t.shape[-1] != h or t.numel() != n * h:
+        raise ValueError(f"{name} must have {n} rows of {h}, got {tuple(t.shape)}")
+    try:
+        m = t.view(n, h)
+    except RuntimeError:
+        raise ValueError(f"{name} must be viewable as ({n}, {h}) without a copy") from None
+    if h > 1 and n > 0 and m.stride(1) != 1:
+        raise ValueError(f"{name} must have unit column stride")
+    return m
+
+
+def _mat(cls, t: torch.Tensor, name: str):
+    m = cls()
+    m.dtype = _grad_dtype(t, name)
+    m.data = t.data_ptr()
+    m.rows, m.cols = t.shape
+    # a row stride means nothing for a single row
+    m.ld = t.stride(0) if t.shape[0] > 1 else max(t.stride(0), t.shape[1])
+    return m
+
+
+def embedding_device(
+    ctx: DeviceContext,
+    table: torch.Tensor,
+    ids: torch.Tensor,
+    scale: float = 1.0,
+    dtype: Optional[torch.dtype] = None,
+    out: Optional[torch.Tensor] = None,
+    stream=None,
+) -> torch.Tensor:
+    """`orda_embedding_device`: scale * table[ids] for table [V, H] (bf16 or
+    f32) and ids of any shape (int64); the result has ids' shape and H, in
+    `dtype` (default the table's) or written to `out`. Ids out of range give
+    zeros and are reported by ctx.check()."""
+    if table.dim() != 2 or (table.shape[1] > 1 and table.stride(1) != 1):
+        raise ValueError("table must be 2-D with unit column stride")
+    _ids(ids)
+    _on_context(ctx, table=table, ids=ids, out=out)
+    n, h = ids.numel(), table.shape[1]
+    if out is None:
+        out = torch.empty(*ids.shape, h, device=table.device, dtype=dtype or table.dtype)
+    elif dtype is not None and out.dtype != dtype:
+        raise ValueError(f"out is {out.dtype}, not {dtype}")
+    rows = _rows_of(out, n, h, "out")
+    buf = _abi.err_buf()
+    rc = _lib().orda_embedding_device(
+        ctx.handle, C.byref(_mat(_abi.OrdaDeviceMat, table, "table")), ids.data_ptr(), n, float(scale),
+        C.byref(_mat(_abi.OrdaDeviceMatMut, rows, "out")), _context_stream(ctx, stream), buf, len(buf))
+    _check(rc, buf)
+    return out
+
+
+def embedding_grad_device(
+    ctx: DeviceContext,
+    grad_out: torch.Tensor,
+    ids: torch.Tensor,
+    vocab: int,
+    scale: float = 1.0,
+    padding_id: Optional[int] = None,
+    dtype: Optional[torch.dtype] = None,
+    out: Optional[torch.Tensor] = None,
+    accumulate: bool = False,
+    stream=None,
+) -> torch.Tensor:
+    """`orda_embedding_grad_device`: the gradient [vocab, H] of the table, from
+    grad_out (ids' shape and H, bf16 or f32). It is allocated in `dtype`
+    (default grad_out's) or written to `out`; accumulate=True adds to what
+    `out` holds (a shared table's output head gradient, say). Tokens of
+    padding_id give no gradient. Ids out of range are reported by ctx.check()."""
+    _ids(ids)
+    _on_context(ctx, grad_out=grad_out, ids=ids, out=out)
+    if grad_out.dim() < 1 or vocab < 1:
+        raise ValueError("grad_out must have a last dimension H and vocab must be at least 1")
+    n, h = ids.numel(), grad_out.shape[-1]
+    g = _rows_of(grad_out, n, h, "grad_out")
+    if out is None:
+        if accumulate:
+            raise ValueError("accumulate needs out")
+        out = torch.empty(vocab, h, device=grad_out.device, dtype=dtype or grad_out.dtype)
+    elif tuple(out.shape) != (vocab, h) or (h > 1 and out.stride(1) != 1):
+        raise ValueError(f"out must be ({vocab}, {h}) with unit column stride")
+    elif dtype is not None and out.dtype != dtype:
+        raise ValueError(f"out is {out.dtype}, not {dtype}")
+    buf = _abi.err_buf()
+    rc = _lib().orda_embedding_grad_device(
+        ctx.handle, C.byref(_mat(_abi.OrdaDeviceMat, g, "grad_out")), ids.data_ptr(), n, float(scale),
+        int(padding_id is not None), int(padding_id or 0), C.byref(_mat(_abi.OrdaDeviceMatMut, out, "out")),
+        int(accumulate), _context_stream(ctx, stream), buf, len(buf))
+    _check(rc, buf)
+    return out
+
+
 def gemm_bf16(
     ctx: DeviceContext,
     a: torch.Tensor,

@@ -227,6 +227,16 @@ pub struct OrdaLinearCeOutputs {
 }
 
 #[repr(C)]
+#[derive(Clone, Copy, Debug)]
+pub struct OrdaDeviceMatMut {
+    pub data: *mut c_void,
+    pub rows: usize,
+    pub cols: usize,
+    pub ld: usize,
+    pub dtype: c_int,
+}
+
+#[repr(C)]
 #[derive(Clone, Copy)]
 pub struct OrdaIpcHandle {
     pub bytes: [c_char; 64],
@@ -306,6 +316,14 @@ extern "C" {
                                             weight: *const OrdaDeviceMat, labels: *const i64, bt: usize,
                                             opts: *const OrdaLinearCeOptions, out: *const OrdaLinearCeOutputs,
                                             stream: *mut c_void, err: *mut c_char, err_len: usize) -> c_int;
+
+    pub fn orda_embedding_device(ctx: *mut OrdaContext, table: *const OrdaDeviceMat, ids: *const i64, n: usize,
+                                 scale: f32, out: *const OrdaDeviceMatMut, stream: *mut c_void, err: *mut c_char,
+                                 err_len: usize) -> c_int;
+    pub fn orda_embedding_grad_device(ctx: *mut OrdaContext, grad_out: *const OrdaDeviceMat, ids: *const i64,
+                                      n: usize, scale: f32, has_padding_id: c_int, padding_id: i64,
+                                      grad_table: *const OrdaDeviceMatMut, accumulate: c_int, stream: *mut c_void,
+                                      err: *mut c_char, err_len: usize) -> c_int;
 
     pub fn orda_context_slots_create(ctx: *mut OrdaContext, world: c_int, rank: c_int, total_rows: usize, h: usize,
                                      copies: c_int, handle_out: *mut OrdaIpcHandle, err: *mut c_char,

@@ -46,3 +46,29 @@ def test_linear_ce_python_refusals(ob, change, what):
     args.update(change)
     with pytest.raises(ValueError, match=what):
         linear_cross_entropy_device(_Handle(), **args)
+
+
+def test_embedding_null_arguments(ob):
+    from orda_b200 import _abi
+
+    buf = _abi.err_buf()
+    lib = ob.load_library()
+    assert lib.orda_embedding_device(None, None, None, 0, 1.0, None, None, buf, len(buf)) == _abi.ORDA_ERR_INVALID
+    assert b"null" in buf.value
+    buf = _abi.err_buf()
+    rc = lib.orda_embedding_grad_device(None, None, None, 0, 1.0, 0, 0, None, 0, None, buf, len(buf))
+    assert rc == _abi.ORDA_ERR_INVALID and b"null" in buf.value
+
+
+def test_embedding_python_refusals(ob):
+    from orda_b200.device import embedding_device, embedding_grad_device
+
+    table, ids = torch.zeros(6, 8), torch.zeros(4, dtype=torch.int64)
+    for args, what in [((table[0], ids), "2-D"), ((table.T, ids), "unit column stride"), ((table, ids.int()), "int64"),
+                       ((table, torch.zeros(8, dtype=torch.int64)[::2]), "contiguous"), ((table, ids), "device")]:
+        with pytest.raises(ValueError, match=what):
+            embedding_device(_Handle(), *args)
+    g = torch.zeros(4, 8)
+    for args, what in [((g, ids.int(), 6), "int64"), ((g, ids, 6), "device")]:
+        with pytest.raises(ValueError, match=what):
+            embedding_grad_device(_Handle(), *args)
