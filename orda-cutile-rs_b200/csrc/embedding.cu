@@ -133,18 +133,18 @@ __global__ void __launch_bounds__(256)
 // --------------------------------------------------------------- the sort
 
 // Stable radix sort of the ids with their positions by one cluster of eight
-// CTAs, 9 bits a pass (two passes up to 262144 ids). Each of the 256 warps owns a
-// contiguous range and a histogram of its own: counting and placing need no
-// atomics and no order between warps. The CTAs exchange their 512 digit totals
-// through distributed shared memory, so a pass is one launch-free step of a few
-// microseconds. Ids out of range and the padding id get the key v, which sorts
-// behind every row. The other clusters of the grid clear the gradient meanwhile.
+// CTAs, at most 9 bits a pass (two passes up to 262144 ids). Each of the 256 warps
+// owns a contiguous range and a histogram of its own: counting and placing need
+// no atomics and no order between warps. The CTAs exchange their digit totals
+// through distributed shared memory, so a pass needs no launch of its own. Ids
+// out of range and the padding id get the key v, which sorts behind every row.
 constexpr int kSortCtas = 8;
 constexpr int kSortThreads = 1024;
 constexpr int kSortWarps = kSortThreads / 32;
-constexpr int kDigits = 512;
-constexpr int kDigitBits = 9;
-constexpr size_t kSortSmem = (kSortWarps * kDigits + 2 * kDigits) * sizeof(uint32_t);
+constexpr int kMaxDigits = 512;
+constexpr int kMaxDigitBits = 9;
+constexpr int kHeld = 4;  // 32-key tiles of a warp that stay in registers over a pass
+constexpr size_t kSortSmem = (kSortWarps * kMaxDigits + 2 * kMaxDigits) * sizeof(uint32_t);
 
 struct SortArgs {
   const int64_t* ids;
@@ -152,12 +152,10 @@ struct SortArgs {
   int v;
   int64_t padding_id;
   int has_padding;
-  int passes;
+  int passes, digit_bits;
   int2* buf0;  // (key, position); the sorted pairs end in buf[passes & 1 ? 1 : 0]
   int2* buf1;
   int* bad;
-  uint8_t* clear;  // gradient rows to clear (null: none)
-  long long clear_rows, clear_row_bytes, clear_ld_bytes;
 };
 
 __device__ __forceinline__ uint32_t ld_cluster_u32(uint32_t addr) {
@@ -166,42 +164,20 @@ __device__ __forceinline__ uint32_t ld_cluster_u32(uint32_t addr) {
   return v;
 }
 
-// Clears [p, p + bytes) with the threads [t, t + nt); 16-byte stores where aligned.
-__device__ void clear_span(uint8_t* p, long long bytes, long long t, long long nt) {
-  const long long head = min(bytes, static_cast<long long>((16 - (reinterpret_cast<uintptr_t>(p) & 15)) & 15));
-  const long long vecs = (bytes - head) / 16;
-  const long long tail = bytes - head - vecs * 16;
-  uint4* q = reinterpret_cast<uint4*>(p + head);
-#pragma unroll 4
-  for (long long i = t; i < vecs; i += nt) __stcs(q + i, make_uint4(0, 0, 0, 0));
-  uint16_t* h = reinterpret_cast<uint16_t*>(p);  // elements are 2 or 4 bytes
-  for (long long i = t; i < head / 2; i += nt) h[i] = 0;
-  uint16_t* e = reinterpret_cast<uint16_t*>(p + head + vecs * 16);
-  for (long long i = t; i < tail / 2; i += nt) e[i] = 0;
-}
-
 __global__ void __cluster_dims__(kSortCtas, 1, 1) __launch_bounds__(kSortThreads, 1) sort_kernel(const SortArgs a) {
-  if (blockIdx.x >= kSortCtas) {
-    const long long nb = gridDim.x - kSortCtas, b = blockIdx.x - kSortCtas;
-    if (a.clear_ld_bytes == a.clear_row_bytes) {
-      clear_span(a.clear, a.clear_rows * a.clear_row_bytes, b * kSortThreads + threadIdx.x, nb * kSortThreads);
-    } else {
-      for (long long r = b; r < a.clear_rows; r += nb)
-        clear_span(a.clear + r * a.clear_ld_bytes, a.clear_row_bytes, threadIdx.x, kSortThreads);
-    }
-    return;
-  }
   extern __shared__ uint32_t sort_smem[];
-  uint32_t* hist = sort_smem;                         // [warps][digits]
-  uint32_t* total = hist + kSortWarps * kDigits;      // this CTA's digit totals
-  uint32_t* scan = total + kDigits;                   // scratch of the scan over digits
+  const int digits = 1 << a.digit_bits;
+  uint32_t* hist = sort_smem;                    // [warps][digits]
+  uint32_t* total = hist + kSortWarps * digits;  // this CTA's digit totals
+  uint32_t* scan = total + digits;               // scratch of the scan over digits
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const uint32_t rank = cluster_ctarank();
-  uint32_t* mine = hist + warp * kDigits;
+  uint32_t* mine = hist + warp * digits;
   const long long tiles = (static_cast<long long>(a.n) + 31) / 32;
   const long long per = (tiles + kSortCtas * kSortWarps - 1) / (kSortCtas * kSortWarps);
   const long long first = (static_cast<long long>(rank) * kSortWarps + warp) * per * 32;
   const uint32_t below = (1u << lane) - 1;
+  pdl_trigger();
 
   auto fetch = [&](int pass, long long i) -> int2 {
     if (pass > 0) return __ldcg((pass & 1 ? a.buf1 : a.buf0) + i);
@@ -213,76 +189,133 @@ __global__ void __cluster_dims__(kSortCtas, 1, 1) __launch_bounds__(kSortThreads
   };
 
   for (int pass = 0; pass < a.passes; ++pass) {
-    const int shift = pass * kDigitBits;
+    const int shift = pass * a.digit_bits;
     int2* dst = pass & 1 ? a.buf0 : a.buf1;
-    for (int d = lane; d < kDigits; d += 32) mine[d] = 0;
-    __syncwarp();
-    for (long long t = 0; t < per; ++t) {
-      const long long i = first + t * 32 + lane;
-      const bool in = i < a.n;
-      const int2 kv = in ? fetch(pass, i) : make_int2(0, 0);
-      const uint32_t d = in ? (static_cast<uint32_t>(kv.x) >> shift) & (kDigits - 1) : kDigits;
-      const uint32_t same = __match_any_sync(0xffffffffu, d);
+    // the same digit in other lanes of the warp's tile (lanes past the end share none)
+    auto digit_of = [&](int2 kv, bool in) {
+      return in ? (static_cast<uint32_t>(kv.x) >> shift) & (digits - 1) : static_cast<uint32_t>(digits);
+    };
+    auto count = [&](uint32_t d, uint32_t same, bool in) {
       if (in && (same & below) == 0) mine[d] += __popc(same);
       __syncwarp();
+    };
+    auto place = [&](int2 kv, uint32_t d, uint32_t same, bool in) {
+      if (in) __stcg(dst + mine[d] + __popc(same & below), kv);
+      __syncwarp();
+      count(d, same, in);
+    };
+    int2 held[kHeld];
+    uint32_t held_same[kHeld];
+    const bool hold = per <= kHeld;
+#pragma unroll
+    for (int t = 0; t < kHeld; ++t) {
+      const long long i = first + t * 32 + lane;
+      if (hold && t < per && i < a.n) held[t] = fetch(pass, i);
+    }
+    for (int d = lane; d < digits; d += 32) mine[d] = 0;
+    __syncwarp();
+    if (hold) {
+#pragma unroll
+      for (int t = 0; t < kHeld; ++t) {
+        if (t >= per) break;
+        const bool in = first + t * 32 + lane < a.n;
+        const uint32_t d = digit_of(held[t], in);
+        held_same[t] = __match_any_sync(0xffffffffu, d);
+        count(d, held_same[t], in);
+      }
+    } else {
+      for (long long t = 0; t < per; ++t) {
+        const long long i = first + t * 32 + lane;
+        const bool in = i < a.n;
+        const uint32_t d = digit_of(in ? fetch(pass, i) : make_int2(0, 0), in);
+        count(d, __match_any_sync(0xffffffffu, d), in);
+      }
     }
     __syncthreads();
     // counts -> offsets among the CTA's warps, and the CTA's totals
-    if (threadIdx.x < kDigits) {
+    const int td = threadIdx.x;
+    if (td < digits) {
       uint32_t s = 0;
 #pragma unroll 8
       for (int w = 0; w < kSortWarps; ++w) {
-        const uint32_t c = hist[w * kDigits + threadIdx.x];
-        hist[w * kDigits + threadIdx.x] = s;
+        const uint32_t c = hist[w * digits + td];
+        hist[w * digits + td] = s;
         s += c;
       }
-      total[threadIdx.x] = s;
+      total[td] = s;
     }
-    __syncthreads();
     cluster_sync();
     uint32_t before = 0, all = 0;
-    if (threadIdx.x < kDigits) {
+    if (td < digits) {
 #pragma unroll
       for (uint32_t r = 0; r < kSortCtas; ++r) {
-        const uint32_t c = ld_cluster_u32(mapa_shared(smem_u32(&total[threadIdx.x]), r));
+        const uint32_t c = ld_cluster_u32(mapa_shared(smem_u32(&total[td]), r));
         if (r < rank) before += c;
         all += c;
       }
-      scan[threadIdx.x] = all;
     }
-    __syncthreads();
     // inclusive scan over the digits: within warps, then the warps' sums
     uint32_t inc = all;
-    if (threadIdx.x < kDigits) {
 #pragma unroll
-      for (int o = 1; o < 32; o <<= 1) {
-        const uint32_t up = __shfl_up_sync(0xffffffffu, inc, o);
-        if (lane >= o) inc += up;
-      }
-      if (lane == 31) scan[warp] = inc;
+    for (int o = 1; o < 32; o <<= 1) {
+      const uint32_t up = __shfl_up_sync(0xffffffffu, inc, o);
+      if (lane >= o) inc += up;
     }
+    if (lane == 31 && warp * 32 < digits) scan[warp] = inc;
     __syncthreads();
-    if (threadIdx.x < kDigits) {
+    if (td < digits) {
       uint32_t start = inc - all + before;
       for (int w = 0; w < warp; ++w) start += scan[w];
 #pragma unroll 8
-      for (int w = 0; w < kSortWarps; ++w) hist[w * kDigits + threadIdx.x] += start;
+      for (int w = 0; w < kSortWarps; ++w) hist[w * digits + td] += start;
     }
     __syncthreads();
-    for (long long t = 0; t < per; ++t) {
-      const long long i = first + t * 32 + lane;
-      const bool in = i < a.n;
-      const int2 kv = in ? fetch(pass, i) : make_int2(0, 0);
-      const uint32_t d = in ? (static_cast<uint32_t>(kv.x) >> shift) & (kDigits - 1) : kDigits;
-      const uint32_t same = __match_any_sync(0xffffffffu, d);
-      if (in) __stcg(dst + mine[d] + __popc(same & below), kv);
-      __syncwarp();
-      if (in && (same & below) == 0) mine[d] += __popc(same);
-      __syncwarp();
+    if (hold) {
+#pragma unroll
+      for (int t = 0; t < kHeld; ++t) {
+        if (t >= per) break;
+        const bool in = first + t * 32 + lane < a.n;
+        place(held[t], digit_of(held[t], in), held_same[t], in);
+      }
+    } else {
+      for (long long t = 0; t < per; ++t) {
+        const long long i = first + t * 32 + lane;
+        const bool in = i < a.n;
+        const int2 kv = in ? fetch(pass, i) : make_int2(0, 0);
+        const uint32_t d = digit_of(kv, in);
+        place(kv, d, __match_any_sync(0xffffffffu, d), in);
+      }
     }
     // the pairs are placed, and no CTA reads another's totals any more
     __threadfence();
     cluster_sync();
+  }
+  // the clearing kernel that runs beside this one is part of what comes before the next
+  pdl_wait();
+}
+
+// Clears the gradient's rows. 1024 threads per SM leave room for the sort's
+// CTAs beside it; 32-byte stores where aligned (172 us for 1 GiB, 6.2 TB/s).
+constexpr int kClearBlocks = 4;  // per SM
+
+__device__ __forceinline__ void clear_span(uint8_t* p, long long bytes, long long t, long long nt) {
+  const long long head = min(bytes, static_cast<long long>((32 - (reinterpret_cast<uintptr_t>(p) & 31)) & 31));
+  const long long vecs = (bytes - head) / 32;
+  uint8_t* q = p + head;
+  for (long long i = t; i < vecs; i += nt)
+    asm volatile("st.global.v8.b32 [%0], {%1, %1, %1, %1, %1, %1, %1, %1};" ::"l"(q + i * 32), "r"(0) : "memory");
+  // elements are 2 or 4 bytes
+  for (long long i = t; i < head / 2; i += nt) reinterpret_cast<uint16_t*>(p)[i] = 0;
+  uint8_t* e = q + vecs * 32;
+  for (long long i = t; i < (p + bytes - e) / 2; i += nt) reinterpret_cast<uint16_t*>(e)[i] = 0;
+}
+
+__global__ void __launch_bounds__(256) clear_kernel(uint8_t* p, long long rows, long long row_bytes, long long ld_bytes) {
+  pdl_trigger();
+  if (ld_bytes == row_bytes) {
+    clear_span(p, rows * row_bytes, blockIdx.x * 256ll + threadIdx.x, gridDim.x * 256ll);
+  } else {
+    for (long long r = blockIdx.x; r < rows; r += gridDim.x) clear_span(p + r * ld_bytes, row_bytes, threadIdx.x, 256);
   }
 }
 
@@ -326,6 +359,8 @@ constexpr int kBatch = 8;
 
 template <typename TI, typename TO, int VEC>
 __global__ void __launch_bounds__(256) grad_tiles_kernel(const GradArgs a) {
+  pdl_trigger();
+  pdl_wait();
   const int tile = blockIdx.x * blockDim.y + threadIdx.y;
   const long long c = (static_cast<long long>(blockIdx.y) * blockDim.x + threadIdx.x) * VEC;
   if (tile >= a.tiles || c >= a.h) return;
@@ -375,25 +410,32 @@ __global__ void __launch_bounds__(256) grad_tiles_kernel(const GradArgs a) {
 // Runs that cross tiles: the tile in which a run begins adds its own partial
 // sum (slot 1) and the following tiles' (slot 0), split over the block's
 // threadIdx.y groups in contiguous parts that are added in order.
+constexpr int kRunX = 64, kRunY = 4;
+
 template <typename TO, int VEC>
-__global__ void __launch_bounds__(256) grad_runs_kernel(const GradArgs a) {
+__global__ void __launch_bounds__(kRunX* kRunY) grad_runs_kernel(const GradArgs a) {
+  __shared__ float sum_s[kRunY][kRunX * VEC];
+  pdl_wait();
   const int tile = blockIdx.x;
-  const long long c = (static_cast<long long>(blockIdx.y) * blockDim.x + threadIdx.x) * VEC;
-  const int p0 = tile * a.len, p1 = p0 + a.len;
-  if (p1 >= a.n) return;
-  const int key = a.sorted[p1 - 1].x;
-  if (key >= a.v || a.sorted[p1].x != key) return;      // the last run ends here
-  if (a.sorted[p0].x == key && p0 > 0 && a.sorted[p0 - 1].x == key) return;  // it began earlier
-  // tiles [tile + 1, last] hold the rest of the run: the last tile whose first key is this one
-  int lo = tile + 1, hi = a.tiles - 1;
-  while (lo < hi) {
-    const int mid = (lo + hi + 1) >> 1;
-    if (a.sorted[mid * a.len].x == key) lo = mid;
-    else hi = mid - 1;
+  const int p0 = tile * a.len, p1 = p0 + a.len;  // p1 < n: the last tile has no block
+  const int key = a.sorted[p1 - 1].x, next = a.sorted[p1].x, head = a.sorted[p0].x;
+  const int prev = p0 > 0 ? a.sorted[p0 - 1].x : -1;
+  if (key >= a.v || next != key) return;     // the last run ends here
+  if (head == key && prev == key) return;    // it began earlier
+  // tiles [tile + 1, last] hold the rest of the run: those whose first key is this
+  // one, looked up side by side
+  const int tid = threadIdx.y * kRunX + threadIdx.x;
+  int last = tile + 1;
+  for (int t0 = tile + 2;; t0 += kRunX * kRunY) {
+    const int t = t0 + tid;
+    const int more = __syncthreads_count(t < a.tiles && a.sorted[static_cast<long long>(t) * a.len].x == key);
+    last += more;
+    if (more < kRunX * kRunY) break;
   }
-  const int count = lo - tile + 1;  // partial sums, this tile's included
-  const int each = (count + blockDim.y - 1) / blockDim.y;
+  const int count = last - tile + 1;  // partial sums, this tile's included
+  const int each = (count + kRunY - 1) / kRunY;
   const int k0 = threadIdx.y * each, k1 = min(count, k0 + each);
+  const long long c = (static_cast<long long>(blockIdx.y) * kRunX + threadIdx.x) * VEC;
   float s[VEC];
 #pragma unroll
   for (int j = 0; j < VEC; ++j) s[j] = 0.f;
@@ -405,15 +447,14 @@ __global__ void __launch_bounds__(256) grad_runs_kernel(const GradArgs a) {
       for (int j = 0; j < VEC; ++j) s[j] += d[j];
     }
   }
-  extern __shared__ float run_smem[];  // [blockDim.y][blockDim.x][VEC]
-  float* sh = run_smem + (threadIdx.y * blockDim.x + threadIdx.x) * VEC;
 #pragma unroll
-  for (int j = 0; j < VEC; ++j) sh[j] = s[j];
+  for (int j = 0; j < VEC; ++j) sum_s[threadIdx.y][threadIdx.x * VEC + j] = s[j];
   __syncthreads();
   if (threadIdx.y != 0 || c >= a.h) return;
-  for (int y = 1; y < static_cast<int>(blockDim.y); ++y)
 #pragma unroll
-    for (int j = 0; j < VEC; ++j) s[j] += run_smem[(y * blockDim.x + threadIdx.x) * VEC + j];
+  for (int y = 1; y < kRunY; ++y)
+#pragma unroll
+    for (int j = 0; j < VEC; ++j) s[j] += sum_s[y][threadIdx.x * VEC + j];
   put_row<TO, VEC>(a, key, c, s);
 }
 
@@ -431,29 +472,30 @@ int pick_vec(long long h, const void* a, long long lda, int esa, const void* b, 
   return 1;
 }
 
-// Threads along a row: a power of two, at least a warp, no more than 256 or than the row needs.
-int row_threads(long long h, int vec) {
+// Threads along a row: a power of two, at least a warp, no more than 256 or
+// than the row needs at `each` vectors per thread.
+int row_threads(long long h, int vec, int each) {
   int x = 32;
-  while (x < 256 && static_cast<long long>(x) * vec < h) x *= 2;
+  while (x < 256 && static_cast<long long>(x) * vec * each < h) x *= 2;
   return x;
 }
 
 template <typename TI, typename TO, int VEC>
 void embed_t(const EmbedArgs& a, cudaStream_t st) {
-  const int x = row_threads(a.h, VEC), y = 256 / x;
+  // four vectors of a row in flight per thread; with few rows all threads of a block on one row
+  const int x = row_threads(a.h, VEC, a.n < 592 ? 1 : 4), y = 256 / x;
   embed_kernel<TI, TO, VEC><<<static_cast<unsigned>((a.n + y - 1) / y), dim3(x, y), 0, st>>>(
       static_cast<const TI*>(a.table), a.ld, a.v, a.h, a.ids, a.n, a.scale, static_cast<TO*>(a.out), a.ldo, a.bad);
 }
 
 template <typename TI, typename TO, int VEC>
-void grad_t(const GradArgs& a, cudaStream_t st) {
-  const int x = row_threads(a.h, VEC), y = 256 / x;
-  const unsigned cols = static_cast<unsigned>((a.h + static_cast<long long>(x) * VEC - 1) / (static_cast<long long>(x) * VEC));
-  grad_tiles_kernel<TI, TO, VEC><<<dim3((a.tiles + y - 1) / y, cols), dim3(x, y), 0, st>>>(a);
-  if (a.tiles < 2) return;
-  // 32 threads along the row, 8 groups along the run
-  const unsigned run_cols = static_cast<unsigned>((a.h + 32 * VEC - 1) / (32 * VEC));
-  grad_runs_kernel<TO, VEC><<<dim3(a.tiles - 1, run_cols), dim3(32, 8), 256 * VEC * sizeof(float), st>>>(a);
+cudaError_t grad_t(const GradArgs& a, cudaStream_t st) {
+  const int x = row_threads(a.h, VEC, 1), y = 256 / x;
+  auto groups = [&a](long long cols) { return static_cast<unsigned>((a.h + cols - 1) / cols); };
+  cudaError_t e = launch_pdl(grad_tiles_kernel<TI, TO, VEC>,
+                             dim3((a.tiles + y - 1) / y, groups(static_cast<long long>(x) * VEC)), dim3(x, y), 0, st, a);
+  if (e != cudaSuccess || a.tiles < 2) return e;
+  return launch_pdl(grad_runs_kernel<TO, VEC>, dim3(a.tiles - 1, groups(kRunX * VEC)), dim3(kRunX, kRunY), 0, st, a);
 }
 
 template <typename F>
@@ -483,9 +525,10 @@ struct EmbedCall {
 struct GradCall {
   const GradArgs& a;
   cudaStream_t st;
+  cudaError_t* e;
   template <typename TI, typename TO, int VEC>
   void operator()() const {
-    grad_t<TI, TO, VEC>(a, st);
+    *e = grad_t<TI, TO, VEC>(a, st);
   }
 };
 
@@ -534,19 +577,19 @@ cudaError_t launch_embed_grad(const EmbedGradArgs& a, void* ws, int num_sms, cud
   s.has_padding = a.has_padding;
   int bits = 1;
   while ((a.v >> bits) != 0) ++bits;  // keys 0..v
-  s.passes = (bits + kDigitBits - 1) / kDigitBits;
+  s.passes = (bits + kMaxDigitBits - 1) / kMaxDigitBits;
+  s.digit_bits = (bits + s.passes - 1) / s.passes;
   s.buf0 = reinterpret_cast<int2*>(w + L.buf0);
   s.buf1 = reinterpret_cast<int2*>(w + L.buf1);
   s.bad = a.bad;
-  unsigned clusters = 1;
   if (!a.accumulate) {
-    s.clear = static_cast<uint8_t*>(a.out);
-    s.clear_rows = a.v;
-    s.clear_row_bytes = a.h * es_out;
-    s.clear_ld_bytes = a.ldo * es_out;
-    // a small gradient needs few SMs; 64 KB each keep a CTA's threads busy
-    const long long want = (a.v * a.h * es_out + (65536ll * kSortCtas) - 1) / (65536ll * kSortCtas);
-    clusters += static_cast<unsigned>(std::max<long long>(1, std::min<long long>(want, num_sms / kSortCtas - 1)));
+    const long long bytes = a.v * a.h * es_out;
+    const long long blocks = std::max<long long>(1, std::min<long long>((bytes + 8191) / 8192, num_sms * kClearBlocks));
+    clear_kernel<<<static_cast<unsigned>(blocks), 256, 0, st>>>(static_cast<uint8_t*>(a.out), a.v, a.h * es_out,
+                                                                a.ldo * es_out);
+    *launches += 1;
+    const cudaError_t e = cudaGetLastError();
+    if (e != cudaSuccess || a.n == 0) return e;
   }
   static std::once_flag once[64];
   int dev = 0;
@@ -556,9 +599,13 @@ cudaError_t launch_embed_grad(const EmbedGradArgs& a, void* ws, int num_sms, cud
     e = cudaFuncSetAttribute(sort_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(kSortSmem));
   });
   if (e != cudaSuccess) return e;
-  sort_kernel<<<clusters * kSortCtas, kSortThreads, kSortSmem, st>>>(s);
+  // beside the clearing kernel, which reads and writes none of the sort's data
+  const size_t smem = (kSortWarps + 2) * sizeof(uint32_t) << s.digit_bits;
+  if (a.accumulate) sort_kernel<<<kSortCtas, kSortThreads, smem, st>>>(s);
+  else e = launch_pdl(sort_kernel, dim3(kSortCtas), dim3(kSortThreads), smem, st, s);
+  if (e == cudaSuccess) e = cudaGetLastError();
+  if (e != cudaSuccess) return e;
   *launches += 1;
-  if (a.n == 0) return cudaGetLastError();
   GradArgs g{};
   g.sorted = s.passes & 1 ? s.buf1 : s.buf0;
   g.n = s.n;
@@ -575,9 +622,9 @@ cudaError_t launch_embed_grad(const EmbedGradArgs& a, void* ws, int num_sms, cud
   g.part = reinterpret_cast<float*>(w + L.part);
   g.ldp = L.ldp;
   const int vec = pick_vec(a.h, a.g, a.ldg, a.in_bf16 ? 2 : 4, a.out, a.ldo, es_out);
-  by_types(a.in_bf16, a.out_bf16, vec, GradCall{g, st});
+  by_types(a.in_bf16, a.out_bf16, vec, GradCall{g, st, &e});
   *launches += L.tiles > 1 ? 2 : 1;
-  return cudaGetLastError();
+  return e;
 }
 
 }  // namespace orda

@@ -47,8 +47,9 @@
 struct OrdaContext {
   int device = 0;
   int num_sms = 148;
-  // [0] status, [1] n_non_ignore, [2] finished blocks of the cross entropy's
-  // combining kernel, [3] token ids out of range (kept until it is reported)
+  // [0] status, [1] n_non_ignore, [2] a label, [3] a token id out of range (both
+  // kept until they are reported), [4] live tokens and [5] finished blocks of a
+  // linear cross entropy call (0 between calls)
   int* d_words = nullptr;
   float* d_mean_scale = nullptr;
   void* ws = nullptr;
@@ -983,7 +984,7 @@ CeLayout ce_layout(size_t bt, size_t h, size_t v, size_t cols, bool smooth, cons
   const bool grads = o.grad_hidden || o.grad_weight;
   L.cols = cols;
   L.n_parts = ceil_div(v, kCePartCols);
-  L.rec_ld = round_up(bt, 32);
+  L.rec_ld = round_up(L.n_parts, 4);  // rows of records start on 32-byte sectors
   L.ld_clean = round_up(h, 8);
   L.ld_piece = round_up(cols, 8);
   size_t off = 0;
@@ -994,8 +995,8 @@ CeLayout ce_layout(size_t bt, size_t h, size_t v, size_t cols, bool smooth, cons
   };
   L.h_clean = take(bt * L.ld_clean * 2);
   L.ref = take(bt * sizeof(float2));
-  L.rec = take(L.n_parts * L.rec_ld * sizeof(float2));
-  L.sx = take(smooth ? L.n_parts * L.rec_ld * sizeof(float) : 0);
+  L.rec = take(bt * L.rec_ld * sizeof(float2));
+  L.sx = take(smooth ? bt * L.rec_ld * sizeof(float) : 0);
   L.row_const = take(bt * sizeof(float4));
   L.nll = take(o.nll ? 0 : bt * sizeof(float));
   L.piece = take(grads ? bt * L.ld_piece * 2 : 0);
@@ -1071,8 +1072,9 @@ int run_linear_ce(OrdaContext* ctx, const OrdaDeviceMat& hm, const OrdaDeviceMat
   a.lse = out.lse;
   a.loss = out.loss;
   a.status = ctx->d_words;
-  a.count = ctx->d_words + 1;
-  a.done = ctx->d_words + 2;
+  a.bad_label = ctx->d_words + 2;
+  a.count = ctx->d_words + 4;
+  a.done = ctx->d_words + 5;
   uint16_t* piece = grads ? reinterpret_cast<uint16_t*>(ws + L.piece) : nullptr;
 
   cudaError_t e;
@@ -1080,10 +1082,7 @@ int run_linear_ce(OrdaContext* ctx, const OrdaDeviceMat& hm, const OrdaDeviceMat
   {
     Phase ph(ctx, 5, st);
     ph.launched();
-    if ((e = cudaMemsetAsync(ctx->d_words, 0, 3 * sizeof(int), st)) != cudaSuccess)
-      return cuda_fail(e, "memset", err, len);
-    launch_ce_prep(a, st);
-    if ((e = cudaGetLastError()) != cudaSuccess) return cuda_fail(e, "label pass", err, len);
+    if ((e = launch_ce_prep(a, st)) != cudaSuccess) return cuda_fail(e, "label pass", err, len);
   }
   const MatRef hmat{a.h_clean, a.bt, a.hd, a.ld_clean};
   // logits of vocabulary columns [v0, v0 + n): statistics (and kept 16-bit logits), or the gradients
@@ -1102,10 +1101,11 @@ int run_linear_ce(OrdaContext* ctx, const OrdaDeviceMat& hm, const OrdaDeviceMat
     gd.args.ld16 = static_cast<long long>(L.ld_piece);
     gd.args.ce_v0 = static_cast<long long>(v0);
     gd.args.ce_ref = a.ref;
-    gd.args.ce_rec = a.rec + v0 / kCePartCols * L.rec_ld;
-    gd.args.ce_sx = smooth ? a.sx + v0 / kCePartCols * L.rec_ld : nullptr;
+    gd.args.ce_rec = a.rec + v0 / kCePartCols;
+    gd.args.ce_sx = smooth ? a.sx + v0 / kCePartCols : nullptr;
     gd.args.ce_rec_ld = a.rec_ld;
     gd.args.ce_const = a.row_const;
+    gd.args.pdl = kPdlWaitFirst;
     gd.demote_kept = ctx->l2_set;
     gd.launches = &nl;
     if ((e = gemm_launch(gd, ctx->num_sms, st, &why)) != cudaSuccess)
@@ -1120,18 +1120,14 @@ int run_linear_ce(OrdaContext* ctx, const OrdaDeviceMat& hm, const OrdaDeviceMat
   {
     Phase ph(ctx, 1, st);
     ph.launched();
-    launch_ce_combine(a, st);
-    if ((e = cudaGetLastError()) != cudaSuccess) return cuda_fail(e, "row kernels", err, len);
+    if ((e = launch_ce_rows(a, piece, static_cast<long long>(L.ld_piece),
+                            grads ? static_cast<long long>(std::min(cols, v)) : 0, st)) != cudaSuccess)
+      return cuda_fail(e, "row kernel", err, len);
   }
   for (size_t v0 = 0; grads && v0 < v; v0 += cols) {
     const size_t n = std::min(cols, v - v0);
-    if (v0 == 0) {
-      Phase ph(ctx, 1, st);
-      ph.launched();
-      launch_ce_rewrite(a, piece, static_cast<long long>(L.ld_piece), 0, static_cast<long long>(n), st);
-      if ((e = cudaGetLastError()) != cudaSuccess) return cuda_fail(e, "row kernels", err, len);
-    } else if (int rc = logits(v0, n, Epi::CeGrad, piece)) {
-      return rc;
+    if (v0 > 0) {
+      if (int rc = logits(v0, n, Epi::CeGrad, piece)) return rc;
     }
     const MatRef dl{piece, a.bt, static_cast<long long>(n), static_cast<long long>(L.ld_piece)};
     if (out.grad_hidden) {
@@ -1158,6 +1154,7 @@ int run_linear_ce(OrdaContext* ctx, const OrdaDeviceMat& hm, const OrdaDeviceMat
         gd.args.slabs = std::min<int>(L.slabs, static_cast<int>(ceil_div(n, 64)));
         gd.args.slab_rows = static_cast<long long>(L.slab_rows);
       }
+      gd.args.pdl = kPdlWaitFirst;
       gd.demote_kept = ctx->l2_set;
       gd.launches = &nl;
       if ((e = gemm_launch(gd, ctx->num_sms, st, &why)) != cudaSuccess)
@@ -1181,6 +1178,8 @@ int run_linear_ce(OrdaContext* ctx, const OrdaDeviceMat& hm, const OrdaDeviceMat
         gd.epi = Epi::StoreBf16;
         gd.args.out16 = static_cast<uint16_t*>(out.grad_weight) + v0 * out.ld_grad_weight;
         gd.args.ld16 = static_cast<long long>(out.ld_grad_weight);
+        // it may run beside the dgrad product, which began with the gradients complete
+        gd.args.pdl = out.grad_hidden ? kPdlWaitLast : kPdlWaitFirst;
       } else {
         gd.args.out0 = static_cast<float*>(out.grad_weight) + v0 * out.ld_grad_weight;
         gd.args.ld0 = static_cast<long long>(out.ld_grad_weight);
@@ -1195,10 +1194,11 @@ int run_linear_ce(OrdaContext* ctx, const OrdaDeviceMat& hm, const OrdaDeviceMat
   if (out.grad_hidden && !L.dgrad_direct) {
     Phase ph(ctx, 2, st);
     ph.launched();
-    launch_slab_sum(reinterpret_cast<const float*>(ws + L.dgrad), L.slabs, static_cast<long long>(L.slab_rows),
-                    static_cast<long long>(L.ld_dgrad), a.bt, a.hd, out.grad_hidden,
-                    static_cast<long long>(out.ld_grad_hidden), out.grad_hidden_dtype == ORDA_DTYPE_BF16, st);
-    if ((e = cudaGetLastError()) != cudaSuccess) return cuda_fail(e, "dgrad sum", err, len);
+    if ((e = launch_slab_sum(reinterpret_cast<const float*>(ws + L.dgrad), L.slabs,
+                             static_cast<long long>(L.slab_rows), static_cast<long long>(L.ld_dgrad), a.bt, a.hd,
+                             out.grad_hidden, static_cast<long long>(out.ld_grad_hidden),
+                             out.grad_hidden_dtype == ORDA_DTYPE_BF16, st)) != cudaSuccess)
+      return cuda_fail(e, "dgrad sum", err, len);
   }
   ctx->last_stream = st;
   return ORDA_OK;
@@ -1217,13 +1217,15 @@ int check_status(OrdaContext* ctx, char* err, size_t len) {
   if (e != cudaSuccess) return cuda_fail(e, "stream synchronize", err, len);
   e = cudaMemcpy(words, ctx->d_words, sizeof words, cudaMemcpyDeviceToHost);
   if (e != cudaSuccess) return cuda_fail(e, "status read", err, len);
+  if (words[2] != DEV_OK || words[3] != DEV_OK) {
+    // kept across calls until they are reported here
+    if ((e = cudaMemset(ctx->d_words + 2, 0, 2 * sizeof(int))) != cudaSuccess) return cuda_fail(e, "memset", err, len);
+  }
   if (words[3] != DEV_OK) {
-    // kept across calls until it is reported here
-    if ((e = cudaMemset(ctx->d_words + 3, 0, sizeof(int))) != cudaSuccess) return cuda_fail(e, "memset", err, len);
     set_error(err, len, "a token id is out of range [0, V) (device id check)");
     return ORDA_ERR_LABEL;
   }
-  if (words[0] == DEV_LABEL_RANGE) {
+  if (words[0] == DEV_LABEL_RANGE || words[2] != DEV_OK) {
     set_error(err, len, "a label is out of range [0, V) and != ignore_index (device label check)");
     return ORDA_ERR_LABEL;
   }
@@ -1340,10 +1342,10 @@ int orda_context_create(int device, OrdaContext** out, char* err, size_t err_len
   std::unique_ptr<OrdaContext> ctx(new OrdaContext());
   ctx->device = device;
   cudaDeviceGetAttribute(&ctx->num_sms, cudaDevAttrMultiProcessorCount, device);
-  if ((e = cudaMalloc(&ctx->d_words, 4 * sizeof(int))) != cudaSuccess) return cuda_fail(e, "cudaMalloc", err, err_len);
+  if ((e = cudaMalloc(&ctx->d_words, 8 * sizeof(int))) != cudaSuccess) return cuda_fail(e, "cudaMalloc", err, err_len);
   if ((e = cudaMalloc(&ctx->d_mean_scale, 4 * sizeof(float))) != cudaSuccess)
     return cuda_fail(e, "cudaMalloc", err, err_len);
-  cudaMemset(ctx->d_words, 0, 4 * sizeof(int));
+  cudaMemset(ctx->d_words, 0, 8 * sizeof(int));
   *out = ctx.release();
   return ORDA_OK;
 }
@@ -1780,7 +1782,11 @@ int orda_linear_cross_entropy_device(OrdaContext* ctx, const OrdaDeviceMat* hidd
   }
   std::lock_guard<std::mutex> lock(ctx->mu);
   DeviceScope dev(ctx->device);
-  return run_linear_ce(ctx, *hidden, *weight, labels, bt, *opts, *out, static_cast<cudaStream_t>(stream), err, err_len);
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  const int rc = run_linear_ce(ctx, *hidden, *weight, labels, bt, *opts, *out, st, err, err_len);
+  // a call that broke off leaves its counters as a whole one does
+  if (rc == ORDA_ERR_CUDA) cudaMemsetAsync(ctx->d_words + 4, 0, 2 * sizeof(int), st);
+  return rc;
 }
 
 static bool elem_mat_ok(const void* data, size_t rows, size_t cols, size_t ld, OrdaDType dt) {

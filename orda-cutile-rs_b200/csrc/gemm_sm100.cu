@@ -496,7 +496,7 @@ __device__ __forceinline__ void ce_epilogue(const KParams& p, const CUtensorMap*
     }
     release_tmem();
     if (row_ok && colh < p.N) {
-      const long long ri = static_cast<long long>(part) * p.e.ce_rec_ld + grow;
+      const long long ri = grow * p.e.ce_rec_ld + part;
       p.e.ce_rec[ri] = make_float2(d, ref2);
       if (SX) p.e.ce_sx[ri] = sx;
     }
@@ -563,6 +563,10 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
   if constexpr (PAIR) cluster_sync();  // peer barriers initialised before any remote arrival
   tc_fence_after();
   const uint32_t tmem_base = *tmem_slot;
+  if constexpr (EPI >= kEpiStoreBf16) {
+    if (p.e.pdl == kPdlWaitFirst) pdl_wait();
+    pdl_trigger();
+  }
 
   if (warp == 0) {
     // ---------------------------------------------------------- producer
@@ -893,6 +897,9 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
     __syncwarp();
   }
 
+  if constexpr (EPI >= kEpiStoreBf16) {
+    if (p.e.pdl == kPdlWaitLast) pdl_wait();
+  }
   tc_fence_before();
   __syncthreads();
   // A pair stays resident until the leader's MMAs (which read the peer's
@@ -1099,7 +1106,7 @@ cudaError_t launch_t(const CUtensorMap* maps, const KParams& kp_in, int num_sms,
     kp.num_items = kp.num_tiles * kp.e.slabs;
   }
   if (kp.num_items < units) units = kp.num_items;
-  if (CG == 1) {
+  if (CG == 1 && !kp.e.pdl) {
     kern<<<units, NUM_THREADS, T::SMEM, stream>>>(maps[0], maps[1], maps[2], maps[3], maps[4], kp);
     return cudaGetLastError();
   }
@@ -1108,13 +1115,15 @@ cudaError_t launch_t(const CUtensorMap* maps, const KParams& kp_in, int num_sms,
   cfg.blockDim = dim3(NUM_THREADS, 1, 1);
   cfg.dynamicSmemBytes = T::SMEM;
   cfg.stream = stream;
-  cudaLaunchAttribute attr[1];
+  cudaLaunchAttribute attr[2];
   attr[0].id = cudaLaunchAttributeClusterDimension;
   attr[0].val.clusterDim.x = CG;
   attr[0].val.clusterDim.y = 1;
   attr[0].val.clusterDim.z = 1;
+  attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[1].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
-  cfg.numAttrs = 1;
+  cfg.numAttrs = kp.e.pdl && EPI >= kEpiStoreBf16 ? 2 : 1;
   return cudaLaunchKernelEx(&cfg, kern, maps[0], maps[1], maps[2], maps[3], maps[4], kp);
 }
 
@@ -1240,6 +1249,11 @@ cudaError_t gemm_launch(const GemmDesc& d, int num_sms, cudaStream_t stream, con
     const int src = s < d.nseg ? s : 0;
     kp.seg_kblocks[s] = s < d.nseg ? static_cast<int>((d.k_seg[s] + BK - 1) / BK) : 0;
     if (s < d.nseg) k_total += d.k_seg[s];
+    if (s > 0 && s >= d.nseg) {  // no second segment: the first one's maps
+      maps[s] = maps[0];
+      maps[2 + s] = maps[2];
+      continue;
+    }
     const MatRef& a = d.a[src];
     const MatRef& b = d.b[src];
     for (const MatRef* m : {&a, &b}) {

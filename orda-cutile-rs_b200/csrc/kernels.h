@@ -7,6 +7,24 @@
 
 namespace orda {
 
+// Launch of a kernel that calls pdl_wait before it touches what earlier
+// kernels of the stream write (or still read): its launch and prologue overlap
+// their end.
+template <typename... P, typename... A>
+cudaError_t launch_pdl(void (*kern)(P...), dim3 grid, dim3 block, size_t smem, cudaStream_t stream, A&&... args) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = grid;
+  cfg.blockDim = block;
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, kern, static_cast<P>(args)...);
+}
+
 // ---------------------------------------------------------------- GEMM
 // One operand segment: a bf16 matrix as stored in memory, rows x cols with
 // leading dimension ld (elements).
@@ -26,6 +44,7 @@ enum class Epi : int { Store = 0, Logits = 1, StoreBf16 = 2, CeStats = 3, CeGrad
 // StoreBf16: out16 = acc rounded to bf16.
 // CeStats / CeGrad: the two passes of the linear cross entropy over a piece
 // of the vocabulary (see linear_ce.cu).
+constexpr int kPdlWaitFirst = 1, kPdlWaitLast = 2;
 constexpr int kMaxSlotRanks = 8;  // ranks of one node that a scattered grad_W store can address
 
 struct EpiArgs {
@@ -61,14 +80,19 @@ struct EpiArgs {
   // multiple of 32 and >= M.
   int slabs = 1;
   long long slab_rows = 0;
+  // Programmatic dependent launch (StoreBf16, slabs, CeStats, CeGrad):
+  // kPdlWaitFirst waits for the kernels before this one ahead of its loads;
+  // kPdlWaitLast does so at its end, for a kernel whose inputs were complete
+  // before the kernel in front of it began (it runs beside that one).
+  int pdl = 0;
   // StoreBf16, and the 16-bit piece that CeStats (optionally) and CeGrad write
   void* out16 = nullptr;
   long long ld16 = 0;
   // CeStats, CeGrad: column c is vocabulary index ce_v0 + c
   long long ce_v0 = 0;
   const float2* ce_ref = nullptr;    // CeStats: per row (reference logit * log2 e, label as int bits)
-  float2* ce_rec = nullptr;          // CeStats: [parts][ce_rec_ld] records, from column 0 of this launch
-  float* ce_sx = nullptr;            // CeStats, optional: [parts][ce_rec_ld] sums of the logits
+  float2* ce_rec = nullptr;          // CeStats: [rows][ce_rec_ld] records of the parts, from column 0 of this launch
+  float* ce_sx = nullptr;            // CeStats, optional: [rows][ce_rec_ld] sums of the logits
   long long ce_rec_ld = 0;
   const float4* ce_const = nullptr;  // CeGrad: per row constants (CeRowConst)
 };
@@ -125,26 +149,26 @@ struct CeArgs {
   uint16_t* h_clean = nullptr;  // bf16 [bt, ld_clean]
   long long ld_clean = 0;
   float2* ref = nullptr;       // [bt]
-  float2* rec = nullptr;       // [n_parts][rec_ld]
-  float* sx = nullptr;         // [n_parts][rec_ld], with label smoothing
+  float2* rec = nullptr;       // [bt][rec_ld]
+  float* sx = nullptr;         // [bt][rec_ld], with label smoothing
   long long rec_ld = 0;
   int n_parts = 0;
   float4* row_const = nullptr;  // [bt]
   float* nll = nullptr;         // [bt]
   float* lse = nullptr;         // [bt], optional
   float* loss = nullptr;        // [1]
-  int* status = nullptr;
-  int* count = nullptr;  // live tokens; zero before the call
-  int* done = nullptr;   // finished blocks of the combining kernel; zero before the call
+  int* status = nullptr;        // cleared by the first kernel
+  int* bad_label = nullptr;     // set to DEV_LABEL_RANGE
+  int* count = nullptr;         // live tokens; 0 between calls
+  int* done = nullptr;          // ended blocks of ce_rows_kernel; 0 between calls
 };
 // Labels, reference logits and the copy of the hidden states with ignored rows cleared.
-void launch_ce_prep(const CeArgs& a, cudaStream_t stream);
-// Records -> nll, lse, the gradient's row constants and the loss.
-void launch_ce_combine(const CeArgs& a, cudaStream_t stream);
-// The kept 16-bit logits of vocabulary columns [v0, v0 + n) -> bf16 logit gradients, in place.
-void launch_ce_rewrite(const CeArgs& a, uint16_t* piece, long long ld, long long v0, long long n, cudaStream_t stream);
+cudaError_t launch_ce_prep(const CeArgs& a, cudaStream_t stream);
+// Records -> nll, lse, the gradient's row constants and the loss; and with a
+// piece the kept 16-bit logits of its n first columns -> bf16 logit gradients.
+cudaError_t launch_ce_rows(const CeArgs& a, uint16_t* piece, long long ld, long long n, cudaStream_t stream);
 // out = the sum over slabs of buf (fp32 [slabs][slab_rows][ldb]) for rows x cols, as bf16 or fp32.
-void launch_slab_sum(const float* buf, int slabs, long long slab_rows, long long ldb, long long rows, long long cols,
+cudaError_t launch_slab_sum(const float* buf, int slabs, long long slab_rows, long long ldb, long long rows, long long cols,
                      void* out, long long ldo, int out_bf16, cudaStream_t stream);
 
 // ---------------------------------------------------- embedding (embedding.cu)

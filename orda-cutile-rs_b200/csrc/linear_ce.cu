@@ -56,10 +56,12 @@ constexpr int kPrepThreads = 128;
 
 __global__ void __launch_bounds__(kPrepThreads) ce_prep_kernel(const CeArgs a) {
   const long long row = blockIdx.x;
+  pdl_trigger();
   const int64_t y = a.labels[row];
   bool live = y != a.ignore_index;
+  if (row == 0 && threadIdx.x == 0) *a.status = DEV_OK;
   if (live && (y < 0 || y >= a.v)) {
-    if (threadIdx.x == 0) atomicCAS(a.status, DEV_OK, DEV_LABEL_RANGE);
+    if (threadIdx.x == 0) *a.bad_label = DEV_LABEL_RANGE;
     live = false;
   }
   const uint16_t* h = static_cast<const uint16_t*>(a.h) + row * a.ldh;
@@ -120,147 +122,192 @@ __device__ __forceinline__ void acc_add(Acc& a, double d, float r) {
   }
 }
 
-// R rows per block, 256 / R threads per row over the parts (their records lie
-// [part][row], so R rows are read together); then the row's loss and constants
-// in 64 bits. The block that finishes last sums the losses in row order.
-constexpr int kCombineThreads = 256;
+// The row's loss and gradient constants from its parts' records, in 64 bits;
+// every block of the row does the same.
+struct RowResult {
+  float4 c;  // -lse log2 e + log2 g, label, a / V g, the label's gradient
+  float nll, lse;
+};
 
-template <int R>
-__global__ void __launch_bounds__(kCombineThreads) ce_combine_kernel(const CeArgs a) {
-  constexpr int T = kCombineThreads / R;
-  __shared__ Acc acc_s[kCombineThreads];
-  __shared__ double sx_s[kCombineThreads];
-  __shared__ bool last;
-  const int r = threadIdx.x % R, t = threadIdx.x / R;
-  const long long row = static_cast<long long>(blockIdx.x) * R + r;
-  const float2 ref = row < a.bt ? a.ref[row] : make_float2(0.f, __int_as_float(-1));
-  const bool live = __float_as_int(ref.y) >= 0;
-  Acc acc{0.0, ref.x};
-  double sx = 0.0;
-  if (live) {
-#pragma unroll 8
-    for (int p = t; p < a.n_parts; p += T) {
-      const float2 c = a.rec[p * a.rec_ld + row];
-      acc_add(acc, static_cast<double>(c.x), c.y);
-    }
-    if (a.alpha > 0.f)
-#pragma unroll 8
-      for (int p = t; p < a.n_parts; p += T) sx += static_cast<double>(a.sx[p * a.rec_ld + row]);
+__device__ __forceinline__ RowResult row_result(const CeArgs& a, float2 ref, const Acc& m, double sx) {
+  RowResult r;
+  const long long n = a.denom_override > 0 ? a.denom_override : max(*static_cast<volatile int*>(a.count), 1);
+  const double g = a.reduction_sum ? 1.0 : 1.0 / static_cast<double>(n);
+  const double up = static_cast<double>(m.r) - static_cast<double>(ref.x);
+  double gap, miss, l;  // lse - z_y, 1 - p_y and lse
+  if (m.r == ref.x) {
+    gap = log1p(m.d);
+    miss = m.d / (1.0 + m.d);
+    l = static_cast<double>(ref.x) * kLn2 + gap;
+  } else {
+    const double own = exp2(-up);  // the label's term next to m.d
+    gap = up * kLn2 + log(m.d + own);
+    miss = m.d / (m.d + own);
+    l = static_cast<double>(m.r) * kLn2 + log(m.d + own);
   }
-  acc_s[threadIdx.x] = acc;
-  sx_s[threadIdx.x] = sx;
-  __syncthreads();
-#pragma unroll
-  for (int o = T / 2; o > 0; o >>= 1) {
-    if (t < o) {
-      Acc m = acc_s[threadIdx.x];
-      const Acc other = acc_s[threadIdx.x + o * R];
-      acc_add(m, other.d, other.r);
-      acc_s[threadIdx.x] = m;
-      sx_s[threadIdx.x] += sx_s[threadIdx.x + o * R];
-    }
-    __syncthreads();
-  }
-  if (t == 0 && row < a.bt) {
-    float nll = 0.f, lse = 0.f;
-    float4 c = make_float4(-INFINITY, __int_as_float(-1), 0.f, 0.f);
-    if (live) {
-      const long long n = a.denom_override > 0 ? a.denom_override : max(*static_cast<volatile int*>(a.count), 1);
-      const double g = a.reduction_sum ? 1.0 : 1.0 / static_cast<double>(n);
-      const Acc m = acc_s[threadIdx.x];
-      // Z_o = m.d 2^(m.r - ref): everything but the label
-      const double up = static_cast<double>(m.r) - static_cast<double>(ref.x);
-      double gap, miss, l;  // lse - z_y, 1 - p_y and lse
-      if (m.r == ref.x) {
-        gap = log1p(m.d);
-        miss = m.d / (1.0 + m.d);
-        l = static_cast<double>(ref.x) * kLn2 + gap;
-      } else {
-        const double own = exp2(-up);  // the label's term next to m.d
-        gap = up * kLn2 + log(m.d + own);
-        miss = m.d / (m.d + own);
-        l = static_cast<double>(m.r) * kLn2 + log(m.d + own);
-      }
-      const double al = static_cast<double>(a.alpha), uni = al / static_cast<double>(a.v);
-      nll = static_cast<float>(al > 0.0 ? (1.0 - al) * gap + al * l - uni * sx_s[threadIdx.x] : gap);
-      lse = static_cast<float>(l);
-      c.x = static_cast<float>(log2(g) - l / kLn2);
-      c.y = ref.y;
-      c.z = static_cast<float>(g * uni);
-      c.w = static_cast<float>(g * (al - uni - miss));
-    }
-    a.row_const[row] = c;
-    a.nll[row] = nll;
-    if (a.lse) a.lse[row] = lse;
-    __threadfence();
-  }
-  __syncthreads();
-  if (threadIdx.x == 0) last = atomicAdd(a.done, 1) == static_cast<int>(gridDim.x) - 1;
-  __syncthreads();
-  if (last) {
-    __threadfence();
-    double s = 0.0;
-#pragma unroll 4
-    for (long long i = threadIdx.x; i < a.bt; i += kCombineThreads) s += static_cast<double>(__ldcg(a.nll + i));
-    sx_s[threadIdx.x] = s;
-    __syncthreads();
-    for (int o = kCombineThreads / 2; o > 0; o >>= 1) {
-      if (static_cast<int>(threadIdx.x) < o) sx_s[threadIdx.x] += sx_s[threadIdx.x + o];
-      __syncthreads();
-    }
-    if (threadIdx.x == 0) {
-      const long long n = a.denom_override > 0 ? a.denom_override : max(*static_cast<volatile int*>(a.count), 1);
-      *a.loss = static_cast<float>(a.reduction_sum ? sx_s[0] : sx_s[0] / static_cast<double>(n));
-    }
-  }
+  const double al = static_cast<double>(a.alpha), uni = al / static_cast<double>(a.v);
+  r.nll = static_cast<float>(al > 0.0 ? (1.0 - al) * gap + al * l - uni * sx : gap);
+  r.lse = static_cast<float>(l);
+  r.c.x = static_cast<float>(-l / kLn2) + (a.reduction_sum ? 0.f : -log2f(static_cast<float>(n)));
+  r.c.y = ref.y;
+  r.c.z = static_cast<float>(g * uni);
+  r.c.w = static_cast<float>(g * (al - uni - miss));
+  return r;
 }
 
-// Kept 16-bit logits -> bf16 logit gradients, in place: 2^(t + c) - a / V g,
-// with c = (the part's reference - lse) log2 e + log2 g. Bound by bandwidth
-// (4 bytes per element); each thread holds 8 neighbouring columns.
-constexpr int kRewriteThreads = 256;
-constexpr int kRewriteSteps = 4;
-constexpr int kRewriteCols = kRewriteThreads * 8 * kRewriteSteps;
+// One block per row, or several along the columns where the rows are few:
+//   * the row's records (coalesced, 8 bytes per 128 columns) -> constants;
+//   * 16-bit logits -> bf16 logit gradients, in place: 2^(t + c) - a g / V with
+//     c = (the part's reference - lse) log2 e + log2 g. Bound by bandwidth, 4 bytes
+//     per element; a thread holds 8 neighbouring columns, and the first loads
+//     are under way while the constants are formed.
+// The block that ends last sums the losses in row order.
+constexpr int kRowThreads = 256;
+constexpr int kRowSteps = 4;
+constexpr int kRowChunk = kRowThreads * 8 * kRowSteps;
 
-__global__ void __launch_bounds__(kRewriteThreads)
-    ce_rewrite_kernel(const float4* __restrict__ row_const, const float2* __restrict__ rec, long long rec_ld,
-                      uint16_t* piece, long long ld, long long v0, long long n, int segs) {
+__global__ void __launch_bounds__(kRowThreads) ce_rows_kernel(const CeArgs a, uint16_t* piece, long long ld, long long n,
+                                                              int segs, long long seg_cols) {
+  __shared__ Acc acc_s[kRowThreads];
+  __shared__ double d_s[kRowThreads / 32], x_s[kRowThreads / 32];
+  __shared__ float4 const_s;
+  __shared__ bool last;
+  pdl_trigger();
+  pdl_wait();
   const long long row = blockIdx.x / segs;
   const int seg = static_cast<int>(blockIdx.x - row * segs);
-  const float4 c = row_const[row];
-  const long long label = static_cast<long long>(__float_as_int(c.y)) - v0;
+  const long long c0 = seg * seg_cols, c1 = min(n, c0 + seg_cols);
   uint16_t* base = piece + row * ld;
-  uint4 v[kRewriteSteps];
-  float off[kRewriteSteps];
+  const float2* rec = a.rec + row * a.rec_ld;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+
+  uint4 v[kRowSteps];
+  auto load = [&](long long at) {
 #pragma unroll
-  for (int i = 0; i < kRewriteSteps; ++i) {
-    const long long col = static_cast<long long>(seg) * kRewriteCols + i * (kRewriteThreads * 8) + threadIdx.x * 8;
-    if (col < n) {
-      v[i] = __ldcs(reinterpret_cast<const uint4*>(base + col));
-      off[i] = rec[((v0 + col) / kCePartCols) * rec_ld + row].y + c.x;
+    for (int i = 0; i < kRowSteps; ++i) {
+      const long long col = at + i * (kRowThreads * 8) + threadIdx.x * 8;
+      if (col < c1) v[i] = __ldcs(reinterpret_cast<const uint4*>(base + col));
+    }
+  };
+  if (c0 < c1) load(c0);
+
+  const float2 ref = a.ref[row];
+  const bool live = __float_as_int(ref.y) >= 0;
+  // parts against the row's reference, the usual case, are a plain sum
+  double d = 0.0, sx = 0.0;
+  bool other = false;
+  if (live) {
+#pragma unroll 4
+    for (int p = threadIdx.x; p < a.n_parts; p += kRowThreads) {
+      const float2 c = rec[p];
+      d += static_cast<double>(c.x);
+      other |= c.y != ref.x;
+    }
+    if (a.alpha > 0.f) {
+#pragma unroll 4
+      for (int p = threadIdx.x; p < a.n_parts; p += kRowThreads) sx += static_cast<double>(a.sx[row * a.rec_ld + p]);
     }
   }
 #pragma unroll
-  for (int i = 0; i < kRewriteSteps; ++i) {
-    const long long col = static_cast<long long>(seg) * kRewriteCols + i * (kRewriteThreads * 8) + threadIdx.x * 8;
-    if (col >= n) continue;
-    uint32_t w[4] = {v[i].x, v[i].y, v[i].z, v[i].w};
-#pragma unroll
-    for (int k = 0; k < 4; ++k) {
-      // 2^23 + u as a float, from u's 16 bits
-      const float q0 = __uint_as_float(__byte_perm(w[k], 0x4B000000u, 0x7610)) - (8388608.0f + kCeQBias);
-      const float q1 = __uint_as_float(__byte_perm(w[k], 0x4B000000u, 0x7632)) - (8388608.0f + kCeQBias);
-      const float e0 = ex2(fmaf(q0, 1.0f / kCeQScale, off[i]));
-      const float e1 = ex2(fmaf(q1, 1.0f / kCeQScale, off[i]));
-      float d0 = (q0 == -kCeQBias ? 0.f : e0) - c.z;
-      float d1 = (q1 == -kCeQBias ? 0.f : e1) - c.z;
-      const long long l = label - col - 2 * k;
-      if (l == 0) d0 = c.w;
-      if (l == 1) d1 = c.w;
-      const __nv_bfloat162 b = __floats2bfloat162_rn(d0, d1);
-      w[k] = *reinterpret_cast<const uint32_t*>(&b);
+  for (int o = 16; o > 0; o >>= 1) {
+    d += __shfl_xor_sync(0xffffffffu, d, o);
+    if (a.alpha > 0.f) sx += __shfl_xor_sync(0xffffffffu, sx, o);
+  }
+  if (lane == 0) {
+    d_s[warp] = d;
+    x_s[warp] = sx;
+  }
+  const bool mixed = __syncthreads_or(other);
+  if (mixed) {
+    Acc acc{0.0, ref.x};
+    for (int p = threadIdx.x; p < a.n_parts; p += kRowThreads) {
+      const float2 c = rec[p];
+      acc_add(acc, static_cast<double>(c.x), c.y);
     }
-    *reinterpret_cast<uint4*>(base + col) = make_uint4(w[0], w[1], w[2], w[3]);
+    acc_s[threadIdx.x] = acc;
+    __syncthreads();
+    for (int o = kRowThreads / 2; o > 0; o >>= 1) {
+      if (static_cast<int>(threadIdx.x) < o) {
+        Acc m = acc_s[threadIdx.x];
+        acc_add(m, acc_s[threadIdx.x + o].d, acc_s[threadIdx.x + o].r);
+        acc_s[threadIdx.x] = m;
+      }
+      __syncthreads();
+    }
+  }
+  if (threadIdx.x == 0) {
+    RowResult r{make_float4(-INFINITY, __int_as_float(-1), 0.f, 0.f), 0.f, 0.f};
+    if (live) {
+      Acc m{0.0, ref.x};
+      double x = 0.0;
+#pragma unroll
+      for (int w = 0; w < kRowThreads / 32; ++w) {
+        m.d += d_s[w];
+        x += x_s[w];
+      }
+      if (mixed) m = acc_s[0];
+      r = row_result(a, ref, m, x);
+    }
+    const_s = r.c;
+    if (seg == 0) {
+      a.row_const[row] = r.c;
+      a.nll[row] = r.nll;
+      if (a.lse) a.lse[row] = r.lse;
+      __threadfence();
+    }
+  }
+  __syncthreads();
+  const float4 c = const_s;
+
+  if (c0 < c1) {
+    const long long label = static_cast<long long>(__float_as_int(c.y));
+    for (long long at = c0; at < c1; at += kRowChunk) {
+      if (at > c0) load(at);
+#pragma unroll
+      for (int i = 0; i < kRowSteps; ++i) {
+        const long long col = at + i * (kRowThreads * 8) + threadIdx.x * 8;
+        if (col >= c1) continue;
+        const float off = rec[col / kCePartCols].y + c.x;
+        uint32_t w[4] = {v[i].x, v[i].y, v[i].z, v[i].w};
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          // 2^23 + u as a float, from u's 16 bits
+          const float q0 = __uint_as_float(__byte_perm(w[k], 0x4B000000u, 0x7610)) - (8388608.0f + kCeQBias);
+          const float q1 = __uint_as_float(__byte_perm(w[k], 0x4B000000u, 0x7632)) - (8388608.0f + kCeQBias);
+          const float e0 = ex2(fmaf(q0, 1.0f / kCeQScale, off));
+          const float e1 = ex2(fmaf(q1, 1.0f / kCeQScale, off));
+          float d0 = (q0 == -kCeQBias ? 0.f : e0) - c.z;
+          float d1 = (q1 == -kCeQBias ? 0.f : e1) - c.z;
+          const long long l = label - col - 2 * k;
+          if (l == 0) d0 = c.w;
+          if (l == 1) d1 = c.w;
+          const __nv_bfloat162 b = __floats2bfloat162_rn(d0, d1);
+          w[k] = *reinterpret_cast<const uint32_t*>(&b);
+        }
+        *reinterpret_cast<uint4*>(base + col) = make_uint4(w[0], w[1], w[2], w[3]);
+      }
+    }
+  }
+
+  // every block has read the count of live tokens when the last one is here
+  if (threadIdx.x == 0) last = atomicAdd(a.done, 1) == static_cast<int>(gridDim.x) - 1;
+  __syncthreads();
+  if (!last) return;
+  __threadfence();
+  double s = 0.0;
+#pragma unroll 4
+  for (long long i = threadIdx.x; i < a.bt; i += kRowThreads) s += static_cast<double>(__ldcg(a.nll + i));
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+  if (lane == 0) d_s[warp] = s;
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    s = 0.0;
+    for (int w = 0; w < kRowThreads / 32; ++w) s += d_s[w];
+    const long long live_n = a.denom_override > 0 ? a.denom_override : max(*static_cast<volatile int*>(a.count), 1);
+    *a.loss = static_cast<float>(a.reduction_sum ? s : s / static_cast<double>(live_n));
+    *a.count = 0;
+    *a.done = 0;
   }
 }
 
@@ -269,11 +316,13 @@ template <bool BF16>
 __global__ void __launch_bounds__(256)
     slab_sum_kernel(const float* __restrict__ buf, int slabs, long long slab_rows, long long ldb, long long rows,
                     long long cols, void* out, long long ldo, int vec_ok) {
+  pdl_trigger();
+  pdl_wait();
   const long long groups = (cols + 3) / 4;
   for (long long i = blockIdx.x * 256ll + threadIdx.x; i < rows * groups; i += gridDim.x * 256ll) {
     const long long r = i / groups, c = (i - r * groups) * 4;
     float4 s = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 4
+#pragma unroll 8
     for (int k = 0; k < slabs; ++k) {
       const float4 x = *reinterpret_cast<const float4*>(buf + (k * slab_rows + r) * ldb + c);
       s.x += x.x;
@@ -302,37 +351,27 @@ __global__ void __launch_bounds__(256)
 
 }  // namespace
 
-void launch_ce_prep(const CeArgs& a, cudaStream_t stream) {
+cudaError_t launch_ce_prep(const CeArgs& a, cudaStream_t stream) {
   ce_prep_kernel<<<static_cast<unsigned>(a.bt), kPrepThreads, 0, stream>>>(a);
+  return cudaGetLastError();
 }
 
-// Eight rows per block read whole 64-byte sectors of the records; fewer rows
-// per block where that would leave SMs without a block.
-void launch_ce_combine(const CeArgs& a, cudaStream_t stream) {
-  if (a.bt >= 2048)
-    ce_combine_kernel<8><<<static_cast<unsigned>((a.bt + 7) / 8), kCombineThreads, 0, stream>>>(a);
-  else if (a.bt >= 512)
-    ce_combine_kernel<4><<<static_cast<unsigned>((a.bt + 3) / 4), kCombineThreads, 0, stream>>>(a);
-  else
-    ce_combine_kernel<1><<<static_cast<unsigned>(a.bt), kCombineThreads, 0, stream>>>(a);
+// Several blocks per row, of 8192 columns at least, while that gives the SMs up to eight blocks each.
+cudaError_t launch_ce_rows(const CeArgs& a, uint16_t* piece, long long ld, long long n, cudaStream_t stream) {
+  long long segs = std::max<long long>(1, std::min((148 * 8) / a.bt, n / kRowChunk));
+  const long long seg_cols = ((n + segs - 1) / segs + kRowThreads * 8 - 1) / (kRowThreads * 8) * (kRowThreads * 8);
+  return launch_pdl(ce_rows_kernel, dim3(static_cast<unsigned>(a.bt * segs)), dim3(kRowThreads), 0, stream, a, piece,
+                    ld, n, static_cast<int>(segs), seg_cols);
 }
 
-void launch_ce_rewrite(const CeArgs& a, uint16_t* piece, long long ld, long long v0, long long n, cudaStream_t stream) {
-  const int segs = static_cast<int>((n + kRewriteCols - 1) / kRewriteCols);
-  ce_rewrite_kernel<<<static_cast<unsigned>(a.bt * segs), kRewriteThreads, 0, stream>>>(a.row_const, a.rec, a.rec_ld,
-                                                                                        piece, ld, v0, n, segs);
-}
-
-void launch_slab_sum(const float* buf, int slabs, long long slab_rows, long long ldb, long long rows, long long cols,
-                     void* out, long long ldo, int out_bf16, cudaStream_t stream) {
+cudaError_t launch_slab_sum(const float* buf, int slabs, long long slab_rows, long long ldb, long long rows,
+                            long long cols, void* out, long long ldo, int out_bf16, cudaStream_t stream) {
   const long long n = rows * ((cols + 3) / 4);
   const unsigned blocks = static_cast<unsigned>(std::min<long long>((n + 255) / 256, 148 * 16));
   const int esz = out_bf16 ? 2 : 4;
   const int vec_ok = reinterpret_cast<uintptr_t>(out) % (4 * esz) == 0 && ldo % 4 == 0;
-  if (out_bf16)
-    slab_sum_kernel<true><<<blocks, 256, 0, stream>>>(buf, slabs, slab_rows, ldb, rows, cols, out, ldo, vec_ok);
-  else
-    slab_sum_kernel<false><<<blocks, 256, 0, stream>>>(buf, slabs, slab_rows, ldb, rows, cols, out, ldo, vec_ok);
+  return launch_pdl(out_bf16 ? slab_sum_kernel<true> : slab_sum_kernel<false>, dim3(blocks), dim3(256), 0, stream, buf,
+                    slabs, slab_rows, ldb, rows, cols, out, ldo, vec_ok);
 }
 
 }  // namespace orda

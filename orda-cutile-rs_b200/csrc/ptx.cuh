@@ -138,6 +138,14 @@ __device__ __forceinline__ void mbar_arrive_cluster(uint32_t cluster_addr) {
   asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr) : "memory");
 }
 
+// ------------------------------------------- programmatic dependent launch
+// pdl_trigger: the next kernel of the stream may be placed on free SMs once
+// every CTA of this grid has called it (or ended). pdl_wait: returns when every
+// kernel before this one has completed and its writes are visible. Both do
+// nothing in a kernel launched without the attribute (see launch_pdl).
+__device__ __forceinline__ void pdl_trigger() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+__device__ __forceinline__ void pdl_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+
 // ------------------------------------------------------- L2 cache policies
 // 64-bit access policies for the .L2::cache_hint operand of bulk copies.
 __device__ __forceinline__ uint64_t l2_policy_evict_first() {

@@ -4,6 +4,7 @@ device memory and streams; every computation runs in liborda_b200.so).
 from __future__ import annotations
 
 import ctypes as C
+import threading
 from dataclasses import dataclass
 from typing import Optional
 
@@ -359,26 +360,40 @@ def vocab_backward_device(
 def _on_context(ctx: DeviceContext, **tensors: Optional[torch.Tensor]) -> None:
     """Every tensor lies on the context's GPU."""
     for name, t in tensors.items():
-        if t is not None and (not t.is_cuda or t.device.index != ctx.device):
+        if t is not None and t.get_device() != ctx.device:
             raise ValueError(f"{name} must be on cuda:{ctx.device}, the context's device, got {t.device}")
 
 
 def _context_stream(ctx: DeviceContext, stream) -> int:
-    """The given stream, else the current one of the context's device."""
-    return torch.cuda.current_stream(ctx.device).cuda_stream if stream is None else _stream(stream)
+    """The given stream, else the current one of the context's device (the raw
+    handle: a Stream object costs as much as a small kernel's launch)."""
+    return torch._C._cuda_getCurrentRawStream(ctx.device) if stream is None else _stream(stream)
+
+
+_DTYPE_CODES = {torch.bfloat16: _abi.DTYPE_BF16, torch.float32: _abi.DTYPE_F32}
+_thread = threading.local()
+
+
+def _err():
+    """This thread's error buffer."""
+    buf = getattr(_thread, "err", None)
+    if buf is None:
+        buf = _thread.err = _abi.err_buf()
+    return buf
 
 
 def _grad_dtype(t: torch.Tensor, name: str) -> int:
-    if t.dtype == torch.bfloat16:
-        return _abi.DTYPE_BF16
-    if t.dtype == torch.float32:
-        return _abi.DTYPE_F32
-    raise ValueError(f"{name}: unsupported dtype {t.dtype}")
+    code = _DTYPE_CODES.get(t.dtype)
+    if code is None:
+        raise ValueError(f"{name}: unsupported dtype {t.dtype}")
+    return code
 
 
 def _row_major(rows: int, cols: int, dtype: torch.dtype, device) -> torch.Tensor:
     """[rows, cols] whose rows start on 16 bytes (what TMA stores address)."""
-    step = 16 // torch.empty(0, dtype=dtype).element_size()
+    step = 16 // dtype.itemsize
+    if cols % step == 0:
+        return torch.empty(rows, cols, device=device, dtype=dtype)
     return torch.empty(rows, -(-cols // step) * step, device=device, dtype=dtype)[:, :cols]
 
 
@@ -423,47 +438,52 @@ def linear_cross_entropy_device(
         raise ValueError("hidden and weight must be 2-D and labels 1-D")
     if labels.dtype != torch.int64 or not labels.is_contiguous():
         raise ValueError("labels must be contiguous int64")
-    out = dict(out or {})
-    unknown = set(out) - {"loss", "nll", "lse", "grad_hidden", "grad_weight"}
-    if unknown:
+    if out and not out.keys() <= {"loss", "nll", "lse", "grad_hidden", "grad_weight"}:
+        unknown = set(out) - {"loss", "nll", "lse", "grad_hidden", "grad_weight"}
         raise ValueError(f"unknown outputs {sorted(unknown)}")
+    out = out or {}
     _on_context(ctx, hidden=hidden, weight=weight, labels=labels, **out)
-    (bt, h), v, dev = hidden.shape, weight.shape[0], hidden.device
-    loss = out.get("loss")
+    bt, h = hidden.shape
+    v, dev = weight.shape[0], hidden.device
+    loss, nll, lse = out.get("loss"), out.get("nll"), out.get("lse")
+    for name, t, n in (("loss", loss, 1), ("nll", nll, bt), ("lse", lse, bt)):
+        if t is not None and (t.dtype != torch.float32 or t.numel() != n or not t.is_contiguous()):
+            raise ValueError(f"{name} must be contiguous float32 of {n} element(s)")
+    if loss is None and nll is None and lse is None:
+        # one allocation for the three
+        store = torch.empty(2 * bt + 1, device=dev, dtype=torch.float32)
+        nll, lse, loss = store[:bt], store[bt:2 * bt], store[2 * bt:]
     if loss is None:
         loss = torch.empty(1, device=dev, dtype=torch.float32)
-    vectors = {}
-    for name in ("nll", "lse"):
-        t = out.get(name)
-        vectors[name] = torch.empty(bt, device=dev, dtype=torch.float32) if t is None else t
-    for name, t, n in (("loss", loss, 1), ("nll", vectors["nll"], bt), ("lse", vectors["lse"], bt)):
-        if t.dtype != torch.float32 or t.numel() != n or not t.is_contiguous():
-            raise ValueError(f"{name} must be contiguous float32 of {n} element(s)")
-    o = _abi.OrdaLinearCeOutputs()
-    o.loss, o.nll, o.lse = loss.data_ptr(), vectors["nll"].data_ptr(), vectors["lse"].data_ptr()
-    grads = {"grad_hidden": None, "grad_weight": None}
+    if nll is None:
+        nll = torch.empty(bt, device=dev, dtype=torch.float32)
+    if lse is None:
+        lse = torch.empty(bt, device=dev, dtype=torch.float32)
+    grads = []
     for name, rows, need in (("grad_hidden", bt, need_grad_hidden), ("grad_weight", v, need_grad_weight)):
-        if not need:
-            if name in out:
-                raise ValueError(f"out holds {name}, which need_{name}=False leaves out")
-            continue
         t = out.get(name)
+        if not need:
+            if t is not None:
+                raise ValueError(f"out holds {name}, which need_{name}=False leaves out")
+            grads.append((None, None, 0, 0))
+            continue
         if t is None:
             t = _row_major(rows, h, grad_dtype, dev)
-        if tuple(t.shape) != (rows, h) or t.stride(1) != 1:
+        elif tuple(t.shape) != (rows, h) or (h > 1 and t.stride(1) != 1):
             raise ValueError(f"{name} must be ({rows}, {h}) with unit column stride")
-        grads[name] = t
-        setattr(o, name, t.data_ptr())
-        setattr(o, f"ld_{name}", max(t.stride(0), h))
-        setattr(o, f"{name}_dtype", _grad_dtype(t, name))
-    opts = _abi.OrdaLinearCeOptions(int(ignore_index), float(label_smoothing), int(reduction),
-                                    int(global_non_ignore), int(piece_bytes))
-    buf = _abi.err_buf()
+        # a row stride means nothing for a single row
+        grads.append((t, t.data_ptr(), t.stride(0) if rows > 1 else max(t.stride(0), h), _grad_dtype(t, name)))
+    (gh, gh_ptr, gh_ld, gh_type), (gw, gw_ptr, gw_ld, gw_type) = grads
+    o = _abi.OrdaLinearCeOutputs(loss.data_ptr(), nll.data_ptr(), lse.data_ptr(), gh_ptr, gh_ld, gw_ptr, gw_ld,
+                                 gh_type, gw_type)
+    opts = _abi.OrdaLinearCeOptions(ignore_index, label_smoothing, reduction, global_non_ignore, piece_bytes)
+    buf = _err()
     rc = _lib().orda_linear_cross_entropy_device(
-        ctx.handle, C.byref(dev_mat(hidden)), C.byref(dev_mat(weight)), labels.data_ptr(), labels.numel(),
-        C.byref(opts), C.byref(o), _context_stream(ctx, stream), buf, len(buf))
+        ctx.handle, C.byref(_mat(_abi.OrdaDeviceMat, hidden, "hidden")),
+        C.byref(_mat(_abi.OrdaDeviceMat, weight, "weight")), labels.data_ptr(), labels.numel(), C.byref(opts),
+        C.byref(o), _context_stream(ctx, stream), buf, len(buf))
     _check(rc, buf)
-    return LinearCrossEntropyResult(loss=loss.view(-1)[0], nll=vectors["nll"], lse=vectors["lse"], **grads)
+    return LinearCrossEntropyResult(loss.view(-1)[0], nll, lse, gh, gw)
 
 
 def _ids(ids: torch.Tensor) -> torch.Tensor:
@@ -477,22 +497,20 @@ def _rows_of(t: torch.Tensor, n: int, h: int, name: str) -> torch.Tensor:
     if t.dim() < 1 or t.shape[-1] != h or t.numel() != n * h:
         raise ValueError(f"{name} must have {n} rows of {h}, got {tuple(t.shape)}")
     try:
-        m = t.view(n, h)
+        return t.view(n, h)
     except RuntimeError:
         raise ValueError(f"{name} must be viewable as ({n}, {h}) without a copy") from None
-    if h > 1 and n > 0 and m.stride(1) != 1:
-        raise ValueError(f"{name} must have unit column stride")
-    return m
 
 
 def _mat(cls, t: torch.Tensor, name: str):
-    m = cls()
-    m.dtype = _grad_dtype(t, name)
-    m.data = t.data_ptr()
-    m.rows, m.cols = t.shape
-    # a row stride means nothing for a single row
-    m.ld = t.stride(0) if t.shape[0] > 1 else max(t.stride(0), t.shape[1])
-    return m
+    """The C struct of a 2-D tensor with unit column stride."""
+    rows, cols = t.shape
+    ld, step = t.stride()
+    if cols > 1 and step != 1:
+        raise ValueError(f"{name} must have unit column stride")
+    if rows <= 1 and ld < cols:  # a row stride means nothing for a single row
+        ld = cols
+    return cls(t.data_ptr(), rows, cols, ld, _grad_dtype(t, name))
 
 
 def embedding_device(
@@ -508,20 +526,22 @@ def embedding_device(
     f32) and ids of any shape (int64); the result has ids' shape and H, in
     `dtype` (default the table's) or written to `out`. Ids out of range give
     zeros and are reported by ctx.check()."""
-    if table.dim() != 2 or (table.shape[1] > 1 and table.stride(1) != 1):
-        raise ValueError("table must be 2-D with unit column stride")
+    if table.dim() != 2:
+        raise ValueError("table must be 2-D")
     _ids(ids)
+    src = _mat(_abi.OrdaDeviceMat, table, "table")
     _on_context(ctx, table=table, ids=ids, out=out)
     n, h = ids.numel(), table.shape[1]
     if out is None:
-        out = torch.empty(*ids.shape, h, device=table.device, dtype=dtype or table.dtype)
+        out = torch.empty((*ids.shape, h), device=table.device, dtype=dtype or table.dtype)
+        dst = _abi.OrdaDeviceMatMut(out.data_ptr(), n, h, h, _grad_dtype(out, "out"))
     elif dtype is not None and out.dtype != dtype:
         raise ValueError(f"out is {out.dtype}, not {dtype}")
-    rows = _rows_of(out, n, h, "out")
-    buf = _abi.err_buf()
-    rc = _lib().orda_embedding_device(
-        ctx.handle, C.byref(_mat(_abi.OrdaDeviceMat, table, "table")), ids.data_ptr(), n, float(scale),
-        C.byref(_mat(_abi.OrdaDeviceMatMut, rows, "out")), _context_stream(ctx, stream), buf, len(buf))
+    else:
+        dst = _mat(_abi.OrdaDeviceMatMut, _rows_of(out, n, h, "out"), "out")
+    buf = _err()
+    rc = _lib().orda_embedding_device(ctx.handle, C.byref(src), ids.data_ptr(), n, scale, C.byref(dst),
+                                      _context_stream(ctx, stream), buf, len(buf))
     _check(rc, buf)
     return out
 
@@ -548,7 +568,7 @@ def embedding_grad_device(
     if grad_out.dim() < 1 or vocab < 1:
         raise ValueError("grad_out must have a last dimension H and vocab must be at least 1")
     n, h = ids.numel(), grad_out.shape[-1]
-    g = _rows_of(grad_out, n, h, "grad_out")
+    g = grad_out if grad_out.dim() == 2 and grad_out.shape[0] == n else _rows_of(grad_out, n, h, "grad_out")
     if out is None:
         if accumulate:
             raise ValueError("accumulate needs out")
@@ -557,11 +577,11 @@ def embedding_grad_device(
         raise ValueError(f"out must be ({vocab}, {h}) with unit column stride")
     elif dtype is not None and out.dtype != dtype:
         raise ValueError(f"out is {out.dtype}, not {dtype}")
-    buf = _abi.err_buf()
+    buf = _err()
     rc = _lib().orda_embedding_grad_device(
-        ctx.handle, C.byref(_mat(_abi.OrdaDeviceMat, g, "grad_out")), ids.data_ptr(), n, float(scale),
-        int(padding_id is not None), int(padding_id or 0), C.byref(_mat(_abi.OrdaDeviceMatMut, out, "out")),
-        int(accumulate), _context_stream(ctx, stream), buf, len(buf))
+        ctx.handle, C.byref(_mat(_abi.OrdaDeviceMat, g, "grad_out")), ids.data_ptr(), n, scale,
+        padding_id is not None, padding_id or 0, C.byref(_mat(_abi.OrdaDeviceMatMut, out, "out")),
+        accumulate, _context_stream(ctx, stream), buf, len(buf))
     _check(rc, buf)
     return out
 
