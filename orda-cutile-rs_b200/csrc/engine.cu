@@ -985,8 +985,10 @@ CeLayout ce_layout(size_t bt, size_t h, size_t v, size_t cols, bool smooth, cons
   L.cols = cols;
   L.n_parts = ceil_div(v, kCePartCols);
   L.rec_ld = round_up(L.n_parts, 4);  // rows of records start on 32-byte sectors
-  L.ld_clean = round_up(h, 8);
-  L.ld_piece = round_up(cols, 8);
+  // rows on 128-byte lines: a TMA box row (128 bytes) then is one line, not two
+  // (1999 x 1000 x 100003 with gradients: 1.42 ms, 1.67 ms with 16-byte rows)
+  L.ld_clean = round_up(h, 64);
+  L.ld_piece = round_up(cols, 64);
   size_t off = 0;
   auto take = [&](size_t bytes) {
     const size_t at = off;
