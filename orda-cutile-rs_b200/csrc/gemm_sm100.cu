@@ -57,7 +57,7 @@ namespace {
 
 constexpr int BN = 256;  // tile columns (N)
 constexpr int BK = 64;   // K slice per stage (128 bytes of bf16)
-constexpr int NUM_THREADS = 384;  // warp 0 TMA, 1 MMA, 2 TMEM, 3 idle, 4..11 epilogue
+constexpr int NUM_THREADS = 384;  // warp 0 TMA, 1 MMA, 2 TMEM, 3 idle, 4.. epilogue (8 warps; see epi_warps)
 constexpr int EPI_WARP0 = 4;
 constexpr int NUM_EPI_WARPS = 8;
 constexpr int TMEM_COLS = 512;
@@ -344,33 +344,36 @@ constexpr int kEpiStoreSlab = 33;
 constexpr int kEpiCeStats = 64;  // + 1: keep the 16-bit logits, + 2: sums of the logits
 constexpr int kEpiCeGrad = 68;
 
+// Epilogue warps. The 16-bit epilogues of the linear cross entropy take 16
+// (four per scheduler): one warp's chain of TMEM load, exponentials, staging
+// and proxy fence leaves its scheduler idle most of the time (two warps each
+// issued in 31 % of the cycles at H = 64), and with a short K loop the epilogue
+// is the tile's time.
+constexpr int epi_warps(int epi) { return epi == kEpiStoreBf16 || epi >= kEpiCeStats ? 16 : 8; }
+constexpr int epi_threads(int epi) { return NUM_THREADS - 256 + 32 * epi_warps(epi); }
+
 // Two fp32 values as a bf16 pair (round to nearest even), the first in the low half.
 __device__ __forceinline__ uint32_t pack_bf16x2(float a, float b) {
   const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
   return *reinterpret_cast<const uint32_t*>(&h);
 }
 
-// Stages this row's 32 16-bit values (16 packed words) as half `side` of a
-// 64-column row (128 bytes, 128-byte swizzle); after side 1 the 32 x 64 block
-// goes out in one TMA store, clipped at the tensor bounds. All lanes call it
-// for side 0 and then side 1.
-__device__ __forceinline__ void stage16(uint8_t* buf, int lane, int side, const uint32_t (&w)[16],
-                                        const CUtensorMap* map, int x, int y, bool store, uint64_t policy) {
-  if (side == 0) {
-    if (lane == 0) bulk_wait_read_all();
-    __syncwarp();
-  }
+// Stages this row's 32 16-bit values (16 packed words) and sends the warp's
+// 32 x 32 block (64-byte rows, 64-byte swizzle) out in one TMA store, clipped
+// at the tensor bounds.
+__device__ __forceinline__ void stage16(uint8_t* buf, int lane, const uint32_t (&w)[16], const CUtensorMap* map, int x,
+                                        int y, bool store, uint64_t policy) {
+  if (lane == 0) bulk_wait_read_all();
+  __syncwarp();
 #pragma unroll
   for (int k = 0; k < 4; ++k)
-    *reinterpret_cast<uint4*>(buf + lane * 128 + (((side * 4 + k) ^ (lane & 7)) << 4)) =
+    *reinterpret_cast<uint4*>(buf + lane * 64 + ((k ^ ((lane >> 1) & 3)) << 4)) =
         make_uint4(w[4 * k], w[4 * k + 1], w[4 * k + 2], w[4 * k + 3]);
-  if (side == 1) {
-    fence_proxy_async_smem();
-    __syncwarp();
-    if (lane == 0 && store) {
-      tma_store_2d_hint(map, buf, x, y, policy);
-      bulk_commit();
-    }
+  fence_proxy_async_smem();
+  __syncwarp();
+  if (lane == 0 && store) {
+    tma_store_2d_hint(map, buf, x, y, policy);
+    bulk_commit();
   }
 }
 
@@ -402,7 +405,7 @@ __device__ __forceinline__ void ce_stats_chunk(const uint32_t (&r)[32], float re
   if (SX) sx += (ax[0] + ax[1]) + (ax[2] + ax[3]);
 }
 
-// Linear cross entropy, one warp's 32 rows x 128 columns of a tile.
+// Linear cross entropy, one warp's 32 rows x 64 columns of a tile.
 // CeStats: one record (sum of 2^t, reference) per row and part, and (+ 1) the
 // 16-bit t of the part. The sum is taken against the row's reference logit;
 // only when it leaves the range that the fixed point resolves (every logit 27
@@ -426,7 +429,7 @@ __device__ __forceinline__ void ce_epilogue(const KParams& p, const CUtensorMap*
   float ref2 = row_c.x;
   auto chunk = [&](int c, const uint32_t(&r)[32]) {
     const int nvalid = p.N - (colh + c * 32);
-    const int lc = lab - c * 32;
+    const int lc = lab - c * 32;  // below 0 without a label here
     const bool has_label = __any_sync(0xffffffffu, lc >= 0 && lc < 32);
     uint32_t q[16];
     if constexpr (GRAD) {
@@ -446,32 +449,27 @@ __device__ __forceinline__ void ce_epilogue(const KParams& p, const CUtensorMap*
       ce_stats_chunk<false, STORE, SX>(r, ref2, lc, 32, d, sx, q);
     }
     if constexpr (STORE) {
-      const int x = colh + (c & ~1) * 32;
-      stage16(buf, lane, c & 1, q, map, x, row0, row0 < p.M && x < p.N, pol_c);
+      const int x = colh + c * 32;
+      stage16(buf, lane, q, map, x, row0, row0 < p.M && x < p.N, pol_c);
     }
   };
-  uint32_t ra[32], rb[32];
+  static_assert(kCePartCols == 64, "two chunks of 32 columns");
+  uint32_t ra[32];
   tmem_ld_32x32b_x32(t_row, ra);
   tmem_ld_wait();
-  tmem_ld_32x32b_x32(t_row + 32, rb);
   chunk(0, ra);
-  tmem_ld_wait();
-  tmem_ld_32x32b_x32(t_row + 64, ra);
-  chunk(1, rb);
-  tmem_ld_wait();
-  tmem_ld_32x32b_x32(t_row + 96, rb);
-  chunk(2, ra);
+  tmem_ld_32x32b_x32(t_row + 32, ra);
   tmem_ld_wait();
   if constexpr (GRAD) {
     release_tmem();
-    chunk(3, rb);
+    chunk(1, ra);
   } else {
-    chunk(3, rb);
+    chunk(1, ra);
     const bool out_of_range = !(d >= kCeSumLow && d < kCeSumHigh);  // NaN too
     if (__any_sync(0xffffffffu, out_of_range)) {
       float m = -INFINITY;
 #pragma unroll 1
-      for (int c = 0; c < 4; ++c) {
+      for (int c = 0; c < 2; ++c) {
         tmem_ld_32x32b_x32(t_row + c * 32, ra);
         tmem_ld_wait();
         const int nvalid = p.N - (colh + c * 32);
@@ -488,7 +486,7 @@ __device__ __forceinline__ void ce_epilogue(const KParams& p, const CUtensorMap*
       if (STORE && lane == 0) bulk_wait_all();
       __syncwarp();
 #pragma unroll 1
-      for (int c = 0; c < 4; ++c) {
+      for (int c = 0; c < 2; ++c) {
         tmem_ld_32x32b_x32(t_row + c * 32, ra);
         tmem_ld_wait();
         chunk(c, ra);
@@ -506,7 +504,7 @@ __device__ __forceinline__ void ce_epilogue(const KParams& p, const CUtensorMap*
 // ------------------------------------------------------------------ kernel
 
 template <int CG, bool A_MN, bool B_MN, int EPI, bool WIDE>
-__global__ void __launch_bounds__(NUM_THREADS, 1)
+__global__ void __launch_bounds__(epi_threads(EPI), 1)
     gemm_kernel(const __grid_constant__ CUtensorMap mapA0, const __grid_constant__ CUtensorMap mapA1,
                 const __grid_constant__ CUtensorMap mapB0, const __grid_constant__ CUtensorMap mapB1,
                 const __grid_constant__ CUtensorMap mapC, const __grid_constant__ KParams p) {
@@ -514,6 +512,8 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
   static_assert(!WIDE || EPI == static_cast<int>(Epi::Store) || EPI == kEpiStoreBf16,
                 "wide tiles take the store epilogues");
   constexpr bool PAIR = CG == 2;
+  constexpr int EW = epi_warps(EPI);
+  constexpr int SLICE = T::TILE_N / (EW / 4);  // tile columns of one epilogue warp
   extern __shared__ uint8_t smem_raw[];
   // Same static layout in both CTAs of a pair: the MMA reads the peer's
   // operands at the leader's offsets.
@@ -541,7 +541,7 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
     }
     for (int i = 0; i < 2; ++i) {
       mbar_init(&tfull[i], 1);
-      mbar_init(&tempty[i], NUM_EPI_WARPS * CG);  // both CTAs' epilogues release the leader's MMA
+      mbar_init(&tempty[i], EW * CG);  // both CTAs' epilogues release the leader's MMA
     }
     mbar_init(drain, 1);
     fence_mbarrier_init();
@@ -699,7 +699,7 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
     // ---------------------------------------------------------- epilogue
     const int ew = warp - EPI_WARP0;
     const int quad = warp & 3;  // TMEM lane quadrant this warp may access
-    const int half = ew >> 2;   // which 128-column half of the tile
+    const int part = ew >> 2;   // which SLICE of the tile's columns
     const int row_in_tile = static_cast<int>(rank) * 128 + quad * 32 + lane;
     const uint64_t pol_c = l2_policy(p.pol_c);
     const uint32_t tempty_leader0 = PAIR ? mapa_shared(smem_u32(&tempty[0]), 0) : 0u;
@@ -724,24 +724,26 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
       }
       if (!mbar_wait<PAIR>(&tfull[acc], acc_phase, p.status, DEV_TIMEOUT_EPILOGUE)) break;
       tc_fence_after();
-      // this warp's half of the tile's columns: TMEM column j holds tile column j
+      // this warp's part of the tile's columns: TMEM column j holds tile column j
       const uint32_t t_row = tmem_base + (static_cast<uint32_t>(quad * 32) << 16) +
-                             static_cast<uint32_t>(acc * BN + half * (T::TILE_N / 2));
-      const int colh = nb * T::TILE_N + half * (T::TILE_N / 2);
+                             static_cast<uint32_t>(acc * BN + part * SLICE);
+      const int colh = nb * T::TILE_N + part * SLICE;
       const int row0 = mb * T::TILE_M + static_cast<int>(rank) * 128 + quad * 32;
-      uint8_t* buf = sOut + ew * OUT_STAGE_BYTES;
+      uint8_t* buf = sOut + ew * (OUT_BYTES / EW);
       // Releases the accumulator to the (leader's) MMA warp as soon as its
       // last TMEM load has completed (the remaining work uses registers only).
       auto release_tmem = [&]() {
         tc_fence_before();
         __syncwarp();
         if (lane == 0) {
-          if constexpr (PAIR) mbar_arrive_cluster(tempty_leader0 + static_cast<uint32_t>(acc * 8));
+          // the release at cluster scope waits for the records that the thread stored before
+          if constexpr (PAIR && EPI >= kEpiStoreBf16) mbar_arrive_remote(tempty_leader0 + static_cast<uint32_t>(acc * 8));
+          else if constexpr (PAIR) mbar_arrive_cluster(tempty_leader0 + static_cast<uint32_t>(acc * 8));
           else mbar_arrive(&tempty[acc]);
         }
       };
       if constexpr (EPI >= kEpiCeStats) {
-        ce_epilogue<EPI>(p, &mapC, buf, lane, t_row, colh, row0, grow, row_ok, nb * 2 + half, row_c, pol_c,
+        ce_epilogue<EPI>(p, &mapC, buf, lane, t_row, colh, row0, grow, row_ok, colh / kCePartCols, row_c, pol_c,
                          release_tmem);
       } else if constexpr (EPI == kEpiStoreBf16) {
         auto store = [&](int c, const uint32_t(&r)[32]) {
@@ -750,8 +752,7 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
             uint32_t q[16];
 #pragma unroll
             for (int j = 0; j < 16; ++j) q[j] = pack_bf16x2(__uint_as_float(r[2 * j]), __uint_as_float(r[2 * j + 1]));
-            const int x = colh + (c & ~1) * 32;
-            stage16(buf, lane, c & 1, q, &mapC, x, row0, row0 < p.M && x < p.N, pol_c);
+            stage16(buf, lane, q, &mapC, col0, row0, row0 < p.M && col0 < p.N, pol_c);
           } else if (row_ok) {
             __nv_bfloat16* dst = static_cast<__nv_bfloat16*>(p.e.out16) + grow * p.e.ld16 + col0;
 #pragma unroll
@@ -759,19 +760,13 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
               if (col0 + j < p.N) dst[j] = __float2bfloat16_rn(__uint_as_float(r[j]));
           }
         };
-        constexpr int NCH = T::TILE_N / 2 / 32;
-        uint32_t ra[32], rb[32];
-        tmem_ld_32x32b_x32(t_row, ra);
-        tmem_ld_wait();
+        uint32_t r[32];
 #pragma unroll
-        for (int c = 0; c < NCH; c += 2) {
-          tmem_ld_32x32b_x32(t_row + (c + 1) * 32, rb);
-          store(c, ra);
+        for (int c = 0; c < SLICE / 32; ++c) {
+          tmem_ld_32x32b_x32(t_row + c * 32, r);
           tmem_ld_wait();
-          if (c + 2 < NCH) tmem_ld_32x32b_x32(t_row + (c + 2) * 32, ra);
-          else release_tmem();
-          store(c + 1, rb);
-          if (c + 2 < NCH) tmem_ld_wait();
+          if (c == SLICE / 32 - 1) release_tmem();
+          store(c, r);
         }
       } else if constexpr (EPI == kEpiStoreSlab) {
         const int y = row0 + (w / p.rem_tiles) * static_cast<int>(p.e.slab_rows);
@@ -882,7 +877,7 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
         release_tmem();
         chunk(3, rb);
         if (row_ok && colh < p.N) {
-          const long long ri = grow * e.n_parts + nb * 2 + half;
+          const long long ri = grow * e.n_parts + nb * 2 + part;
           reinterpret_cast<float4*>(e.rec_own)[ri] = make_float4(os.m, os.d1, os.dT, os.sx);
         }
       }
@@ -997,14 +992,14 @@ bool encode_out_map_f16(CUtensorMap* map, void* ptr, long long rows, long long c
   return r == CUDA_SUCCESS;
 }
 
-// bf16 (or other 16-bit) output map: the box and swizzle of stage16's 32 x 64 blocks.
+// bf16 (or other 16-bit) output map: the box and swizzle of stage16's 32 x 32 blocks.
 bool encode_out_map_16(CUtensorMap* map, void* ptr, long long rows, long long cols, long long ld) {
   cuuint64_t dims[2] = {static_cast<cuuint64_t>(cols), static_cast<cuuint64_t>(rows)};
   cuuint64_t strides[1] = {static_cast<cuuint64_t>(ld) * 2};
-  cuuint32_t box[2] = {64, 32};
+  cuuint32_t box[2] = {32, 32};
   cuuint32_t estr[2] = {1, 1};
   CUresult r = g_encode(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, ptr, dims, strides, box, estr,
-                        CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_NONE,
+                        CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_64B, CU_TENSOR_MAP_L2_PROMOTION_NONE,
                         CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   return r == CUDA_SUCCESS;
 }
@@ -1055,7 +1050,7 @@ cudaError_t launch_t(const CUtensorMap* maps, const KParams& kp_in, int num_sms,
       if (CG > 1) {
         cudaLaunchConfig_t q = {};
         q.gridDim = dim3(static_cast<unsigned>(units * CG), 1, 1);
-        q.blockDim = dim3(NUM_THREADS, 1, 1);
+        q.blockDim = dim3(epi_threads(EPI), 1, 1);
         q.dynamicSmemBytes = T::SMEM;
         cudaLaunchAttribute qa[1];
         qa[0].id = cudaLaunchAttributeClusterDimension;
@@ -1107,12 +1102,12 @@ cudaError_t launch_t(const CUtensorMap* maps, const KParams& kp_in, int num_sms,
   }
   if (kp.num_items < units) units = kp.num_items;
   if (CG == 1 && !kp.e.pdl) {
-    kern<<<units, NUM_THREADS, T::SMEM, stream>>>(maps[0], maps[1], maps[2], maps[3], maps[4], kp);
+    kern<<<units, epi_threads(EPI), T::SMEM, stream>>>(maps[0], maps[1], maps[2], maps[3], maps[4], kp);
     return cudaGetLastError();
   }
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(static_cast<unsigned>(units * CG), 1, 1);
-  cfg.blockDim = dim3(NUM_THREADS, 1, 1);
+  cfg.blockDim = dim3(epi_threads(EPI), 1, 1);
   cfg.dynamicSmemBytes = T::SMEM;
   cfg.stream = stream;
   cudaLaunchAttribute attr[2];

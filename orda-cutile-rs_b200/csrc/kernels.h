@@ -133,7 +133,7 @@ constexpr float kCeQLow = -64.0f;
 // A part whose sum of 2^t lies outside [2^-40, 2^62) is stored relative to its own maximum.
 constexpr float kCeSumLow = 9.094947017729282e-13f;
 constexpr float kCeSumHigh = 4611686018427387904.0f;
-constexpr int kCePartCols = 128;
+constexpr int kCePartCols = 64;  // columns of one epilogue warp
 
 struct CeArgs {
   const void* h = nullptr;  // bf16 [bt, hd]

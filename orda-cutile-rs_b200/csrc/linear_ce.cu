@@ -6,7 +6,7 @@
 //   nll = (1 - a) (lse - z_y) + a (lse - mean_v z_v)
 //   dz_v = g (e^{z_v - lse} - (1 - a) [v = y] - a / V),  dh = dz W,  dW = dz^T h
 // The label's logit is the reference of its row: the logits product sums
-// Z_o = sum_{v != y} e^{z_v - z_y} per 128-column part, so that
+// Z_o = sum_{v != y} e^{z_v - z_y} per 64-column part, so that
 //   lse - z_y = log(1 + Z_o),  1 - p_y = Z_o / (1 + Z_o)
 // lose nothing to cancellation when the label's probability nears 1.
 //
@@ -32,6 +32,7 @@ namespace {
 
 constexpr float kLog2E = 1.4426950408889634f;
 constexpr double kLn2 = 0.6931471805599453;
+constexpr float kLn2f = 0.6931471805599453f;
 
 __device__ __forceinline__ float bf16_lo(uint32_t w) { return __uint_as_float(w << 16); }
 __device__ __forceinline__ float bf16_hi(uint32_t w) { return __uint_as_float(w & 0xffff0000u); }
@@ -122,43 +123,47 @@ __device__ __forceinline__ void acc_add(Acc& a, double d, float r) {
   }
 }
 
-// The row's loss and gradient constants from its parts' records, in 64 bits;
-// every block of the row does the same.
+// The row's loss and gradient constants from its parts' sum m; every block of
+// the row does the same. Results are fp32, and so is the arithmetic where no
+// two large numbers cancel.
 struct RowResult {
   float4 c;  // -lse log2 e + log2 g, label, a / V g, the label's gradient
   float nll, lse;
 };
 
-__device__ __forceinline__ RowResult row_result(const CeArgs& a, float2 ref, const Acc& m, double sx) {
+__device__ __forceinline__ RowResult row_result(const CeArgs& a, float2 ref, const Acc& m, float sx) {
   RowResult r;
   const long long n = a.denom_override > 0 ? a.denom_override : max(*static_cast<volatile int*>(a.count), 1);
-  const double g = a.reduction_sum ? 1.0 : 1.0 / static_cast<double>(n);
-  const double up = static_cast<double>(m.r) - static_cast<double>(ref.x);
-  double gap, miss, l;  // lse - z_y, 1 - p_y and lse
+  const float nf = a.reduction_sum ? 1.f : static_cast<float>(n);
+  const float g = 1.f / nf;
+  float gap, miss, l;  // lse - z_y, 1 - p_y and lse
   if (m.r == ref.x) {
-    gap = log1p(m.d);
-    miss = m.d / (1.0 + m.d);
-    l = static_cast<double>(ref.x) * kLn2 + gap;
+    const float z = static_cast<float>(m.d);
+    gap = log1pf(z);
+    miss = z < INFINITY ? z / (1.f + z) : 1.f;
+    l = fmaf(ref.x, kLn2f, gap);
   } else {
+    const double up = static_cast<double>(m.r) - static_cast<double>(ref.x);
     const double own = exp2(-up);  // the label's term next to m.d
-    gap = up * kLn2 + log(m.d + own);
-    miss = m.d / (m.d + own);
-    l = static_cast<double>(m.r) * kLn2 + log(m.d + own);
+    const double lg = log(m.d + own);
+    gap = static_cast<float>(up * kLn2 + lg);
+    miss = static_cast<float>(m.d / (m.d + own));
+    l = static_cast<float>(static_cast<double>(m.r) * kLn2 + lg);
   }
-  const double al = static_cast<double>(a.alpha), uni = al / static_cast<double>(a.v);
-  r.nll = static_cast<float>(al > 0.0 ? (1.0 - al) * gap + al * l - uni * sx : gap);
-  r.lse = static_cast<float>(l);
-  r.c.x = static_cast<float>(-l / kLn2) + (a.reduction_sum ? 0.f : -log2f(static_cast<float>(n)));
+  const float uni = a.alpha / static_cast<float>(a.v);
+  r.nll = a.alpha > 0.f ? (1.f - a.alpha) * gap + a.alpha * (l - sx / static_cast<float>(a.v)) : gap;
+  r.lse = l;
+  r.c.x = fmaf(-l, kLog2E, -log2f(nf));
   r.c.y = ref.y;
-  r.c.z = static_cast<float>(g * uni);
-  r.c.w = static_cast<float>(g * (al - uni - miss));
+  r.c.z = g * uni;
+  r.c.w = g * (a.alpha - uni - miss);
   return r;
 }
 
 // One block per row, or several along the columns where the rows are few:
-//   * the row's records (coalesced, 8 bytes per 128 columns) -> constants;
-//   * 16-bit logits -> bf16 logit gradients, in place: 2^(t + c) - a g / V with
-//     c = (the part's reference - lse) log2 e + log2 g. Bound by bandwidth, 4 bytes
+//   * the row's records (coalesced, 8 bytes per 64 columns) -> constants;
+//   * 16-bit logits -> bf16 logit gradients, in place: 2^(t + off) - a g / V with
+//     off = (the part's reference - lse) log2 e + log2 g. Bound by bandwidth, 4 bytes
 //     per element; a thread holds 8 neighbouring columns, and the first loads
 //     are under way while the constants are formed.
 // The block that ends last sums the losses in row order.
@@ -246,7 +251,7 @@ __global__ void __launch_bounds__(kRowThreads) ce_rows_kernel(const CeArgs a, ui
         x += x_s[w];
       }
       if (mixed) m = acc_s[0];
-      r = row_result(a, ref, m, x);
+      r = row_result(a, ref, m, static_cast<float>(x));
     }
     const_s = r.c;
     if (seg == 0) {
@@ -260,29 +265,34 @@ __global__ void __launch_bounds__(kRowThreads) ce_rows_kernel(const CeArgs a, ui
   const float4 c = const_s;
 
   if (c0 < c1) {
-    const long long label = static_cast<long long>(__float_as_int(c.y));
+    const int label = __float_as_int(c.y);  // -1: none
+    const int label8 = label < 0 ? -1 : label & ~7, label_in = label & 7;
     for (long long at = c0; at < c1; at += kRowChunk) {
       if (at > c0) load(at);
 #pragma unroll
       for (int i = 0; i < kRowSteps; ++i) {
         const long long col = at + i * (kRowThreads * 8) + threadIdx.x * 8;
         if (col >= c1) continue;
-        const float off = rec[col / kCePartCols].y + c.x;
+        // 2^(t + off) = 2^(t - 62.5) 2^(off + 62.5): the first factor is an exact
+        // argument from u's bits (2^23 + u as a float, over 512, less the bias), and
+        // flushes to zero for code 0, so the code needs no test of its own
+        const float up = ex2(rec[col / kCePartCols].y + (c.x + 62.5f));
         uint32_t w[4] = {v[i].x, v[i].y, v[i].z, v[i].w};
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
-          // 2^23 + u as a float, from u's 16 bits
-          const float q0 = __uint_as_float(__byte_perm(w[k], 0x4B000000u, 0x7610)) - (8388608.0f + kCeQBias);
-          const float q1 = __uint_as_float(__byte_perm(w[k], 0x4B000000u, 0x7632)) - (8388608.0f + kCeQBias);
-          const float e0 = ex2(fmaf(q0, 1.0f / kCeQScale, off));
-          const float e1 = ex2(fmaf(q1, 1.0f / kCeQScale, off));
-          float d0 = (q0 == -kCeQBias ? 0.f : e0) - c.z;
-          float d1 = (q1 == -kCeQBias ? 0.f : e1) - c.z;
-          const long long l = label - col - 2 * k;
-          if (l == 0) d0 = c.w;
-          if (l == 1) d1 = c.w;
-          const __nv_bfloat162 b = __floats2bfloat162_rn(d0, d1);
+          constexpr float kBias = -(8388608.0f + kCeQBias) / kCeQScale - 62.5f;
+          const float x0 = fmaf(__uint_as_float(__byte_perm(w[k], 0x4B000000u, 0x7610)), 1.0f / kCeQScale, kBias);
+          const float x1 = fmaf(__uint_as_float(__byte_perm(w[k], 0x4B000000u, 0x7632)), 1.0f / kCeQScale, kBias);
+          const __nv_bfloat162 b = __floats2bfloat162_rn(fmaf(ex2(x0), up, -c.z), fmaf(ex2(x1), up, -c.z));
           w[k] = *reinterpret_cast<const uint32_t*>(&b);
+        }
+        if (col == label8) {
+          const uint32_t dy = __bfloat16_as_ushort(__float2bfloat16_rn(c.w));
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            if (2 * k == label_in) w[k] = (w[k] & 0xffff0000u) | dy;
+            if (2 * k + 1 == label_in) w[k] = (w[k] & 0xffffu) | (dy << 16);
+          }
         }
         *reinterpret_cast<uint4*>(base + col) = make_uint4(w[0], w[1], w[2], w[3]);
       }

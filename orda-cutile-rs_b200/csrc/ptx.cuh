@@ -138,6 +138,13 @@ __device__ __forceinline__ void mbar_arrive_cluster(uint32_t cluster_addr) {
   asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr) : "memory");
 }
 
+// The same with the default CTA-scope release: hands over nothing in memory
+// (TMEM reads are ordered by tcgen05.wait::ld and the fence before), so it does
+// not wait until earlier global stores of the thread are performed.
+__device__ __forceinline__ void mbar_arrive_remote(uint32_t cluster_addr) {
+  asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr) : "memory");
+}
+
 // ------------------------------------------- programmatic dependent launch
 // pdl_trigger: the next kernel of the stream may be placed on free SMs once
 // every CTA of this grid has called it (or ended). pdl_wait: returns when every
