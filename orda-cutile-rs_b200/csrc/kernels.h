@@ -146,8 +146,8 @@ struct CeArgs {
   float alpha = 0.0f;  // label smoothing
   int reduction_sum = 0;
   long long denom_override = 0;
-  uint16_t* h_clean = nullptr;  // bf16 [bt, ld_clean]
-  long long ld_clean = 0;
+  uint16_t* h_clean = nullptr;  // bf16 [clean_rows, ld_clean], zeros from row bt
+  long long clean_rows = 0, ld_clean = 0;
   float2* ref = nullptr;       // [bt]
   float2* rec = nullptr;       // [bt][rec_ld]
   float* sx = nullptr;         // [bt][rec_ld], with label smoothing

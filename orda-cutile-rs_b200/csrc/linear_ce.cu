@@ -58,8 +58,9 @@ constexpr int kPrepThreads = 128;
 __global__ void __launch_bounds__(kPrepThreads) ce_prep_kernel(const CeArgs a) {
   const long long row = blockIdx.x;
   pdl_trigger();
-  const int64_t y = a.labels[row];
-  bool live = y != a.ignore_index;
+  const bool token = row < a.bt;
+  const int64_t y = token ? a.labels[row] : a.ignore_index;
+  bool live = token && y != a.ignore_index;
   if (row == 0 && threadIdx.x == 0) *a.status = DEV_OK;
   if (live && (y < 0 || y >= a.v)) {
     if (threadIdx.x == 0) *a.bad_label = DEV_LABEL_RANGE;
@@ -91,6 +92,7 @@ __global__ void __launch_bounds__(kPrepThreads) ce_prep_kernel(const CeArgs a) {
     for (int i = threadIdx.x; i < nvec; i += kPrepThreads) reinterpret_cast<uint4*>(out)[i] = make_uint4(0, 0, 0, 0);
     for (long long i = 8ll * nvec + threadIdx.x; i < a.hd; i += kPrepThreads) out[i] = 0;
   }
+  if (!token) return;
   s = warp_sum(s);
   __shared__ float part[kPrepThreads / 32];
   if ((threadIdx.x & 31) == 0) part[threadIdx.x >> 5] = s;
@@ -362,7 +364,7 @@ __global__ void __launch_bounds__(256)
 }  // namespace
 
 cudaError_t launch_ce_prep(const CeArgs& a, cudaStream_t stream) {
-  ce_prep_kernel<<<static_cast<unsigned>(a.bt), kPrepThreads, 0, stream>>>(a);
+  ce_prep_kernel<<<static_cast<unsigned>(a.clean_rows), kPrepThreads, 0, stream>>>(a);
   return cudaGetLastError();
 }
 
