@@ -133,18 +133,22 @@ __global__ void __launch_bounds__(256)
 // --------------------------------------------------------------- the sort
 
 // Stable radix sort of the ids with their positions by one cluster of eight
-// CTAs, at most 9 bits a pass (two passes up to 262144 ids). Each of the 256 warps
-// owns a contiguous range and a histogram of its own: counting and placing need
-// no atomics and no order between warps. The CTAs exchange their digit totals
+// CTAs, at most 9 bits a pass (two passes up to 262144 ids). Each warp owns a
+// contiguous range and a histogram of its own: counting and placing need no
+// atomics and no order between warps. The CTAs exchange their digit totals
 // through distributed shared memory, so a pass needs no launch of its own. Ids
 // out of range and the padding id get the key v, which sorts behind every row.
 constexpr int kSortCtas = 8;
-constexpr int kSortThreads = 1024;
-constexpr int kSortWarps = kSortThreads / 32;
+// Threads per CTA: 512 up to 16384 ids, where clearing and summing the warps'
+// histograms is the time (two passes over 8192 ids: 14.4 us, 16.4 us with 1024),
+// 1024 above (65536 ids and their gradient: 80 us, 90 us with 512).
+constexpr int kFewIds = 16384;
 constexpr int kMaxDigits = 512;
 constexpr int kMaxDigitBits = 9;
 constexpr int kHeld = 4;  // 32-key tiles of a warp that stay in registers over a pass
-constexpr size_t kSortSmem = (kSortWarps * kMaxDigits + 2 * kMaxDigits) * sizeof(uint32_t);
+constexpr size_t sort_smem_bytes(int threads, int digit_bits) {
+  return (threads / 32 + 2) * sizeof(uint32_t) << digit_bits;
+}
 
 struct SortArgs {
   const int64_t* ids;
@@ -164,12 +168,16 @@ __device__ __forceinline__ uint32_t ld_cluster_u32(uint32_t addr) {
   return v;
 }
 
-__global__ void __cluster_dims__(kSortCtas, 1, 1) __launch_bounds__(kSortThreads, 1) sort_kernel(const SortArgs a) {
+template <int THREADS>
+__global__ void __cluster_dims__(kSortCtas, 1, 1) __launch_bounds__(THREADS, 1) sort_kernel(const SortArgs a) {
+  constexpr int kSortWarps = THREADS / 32;
+  static_assert(kMaxDigits <= THREADS && kSortWarps <= 32, "a thread per digit, a lane per warp");
   extern __shared__ uint32_t sort_smem[];
   const int digits = 1 << a.digit_bits;
   uint32_t* hist = sort_smem;                    // [warps][digits]
   uint32_t* total = hist + kSortWarps * digits;  // this CTA's digit totals
-  uint32_t* scan = total + digits;               // scratch of the scan over digits
+  uint32_t* start = total + digits;              // where this CTA's keys of a digit go
+  __shared__ uint32_t scan[kSortWarps];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const uint32_t rank = cluster_ctarank();
   uint32_t* mine = hist + warp * digits;
@@ -200,7 +208,7 @@ __global__ void __cluster_dims__(kSortCtas, 1, 1) __launch_bounds__(kSortThreads
       __syncwarp();
     };
     auto place = [&](int2 kv, uint32_t d, uint32_t same, bool in) {
-      if (in) __stcg(dst + mine[d] + __popc(same & below), kv);
+      if (in) __stcg(dst + start[d] + mine[d] + __popc(same & below), kv);
       __syncwarp();
       count(d, same, in);
     };
@@ -255,20 +263,20 @@ __global__ void __cluster_dims__(kSortCtas, 1, 1) __launch_bounds__(kSortThreads
       }
     }
     // inclusive scan over the digits: within warps, then the warps' sums
-    uint32_t inc = all;
+    auto warp_scan = [lane](uint32_t x) {
 #pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const uint32_t up = __shfl_up_sync(0xffffffffu, inc, o);
-      if (lane >= o) inc += up;
-    }
-    if (lane == 31 && warp * 32 < digits) scan[warp] = inc;
+      for (int o = 1; o < 32; o <<= 1) {
+        const uint32_t up = __shfl_up_sync(0xffffffffu, x, o);
+        if (lane >= o) x += up;
+      }
+      return x;
+    };
+    const uint32_t inc = warp_scan(all);
+    if (lane == 31) scan[warp] = inc;
     __syncthreads();
-    if (td < digits) {
-      uint32_t start = inc - all + before;
-      for (int w = 0; w < warp; ++w) start += scan[w];
-#pragma unroll 8
-      for (int w = 0; w < kSortWarps; ++w) hist[w * digits + td] += start;
-    }
+    const uint32_t sums = warp_scan(lane < kSortWarps ? scan[lane] : 0);
+    const uint32_t ahead = __shfl_sync(0xffffffffu, sums, max(warp - 1, 0));
+    if (td < digits) start[td] = (warp > 0 ? ahead : 0) + inc - all + before;
     __syncthreads();
     if (hold) {
 #pragma unroll
@@ -287,7 +295,6 @@ __global__ void __cluster_dims__(kSortCtas, 1, 1) __launch_bounds__(kSortThreads
       }
     }
     // the pairs are placed, and no CTA reads another's totals any more
-    __threadfence();
     cluster_sync();
   }
   // the clearing kernel that runs beside this one is part of what comes before the next
@@ -336,12 +343,37 @@ struct GradArgs {
   long long ldp;
 };
 
+// Adds to fp32 elements in L2 without waiting for them. Each element of the
+// gradient gets one addition per call, so the order of the additions cannot
+// matter; a read, add and write here would put a memory latency at each run's
+// end (72 us instead of 58 us for 8192 tokens on top of an fp32 gradient).
+template <int VEC>
+__device__ __forceinline__ void red_add(float* p, const float (&f)[VEC]) {
+  if constexpr (VEC % 4 == 0) {
+#pragma unroll
+    for (int j = 0; j < VEC; j += 4)
+      asm volatile("red.global.add.v4.f32 [%0], {%1, %2, %3, %4};" ::"l"(p + j), "f"(f[j]), "f"(f[j + 1]), "f"(f[j + 2]),
+                   "f"(f[j + 3])
+                   : "memory");
+  } else if constexpr (VEC == 2) {
+    asm volatile("red.global.add.v2.f32 [%0], {%1, %2};" ::"l"(p), "f"(f[0]), "f"(f[1]) : "memory");
+  } else {
+    asm volatile("red.global.add.f32 [%0], %1;" ::"l"(p), "f"(f[0]) : "memory");
+  }
+}
+
 template <typename TO, int VEC>
 __device__ __forceinline__ void put_row(const GradArgs& a, int key, long long c, const float (&s)[VEC]) {
   TO* dst = static_cast<TO*>(a.out) + key * a.ldo + c;
   float f[VEC];
 #pragma unroll
   for (int j = 0; j < VEC; ++j) f[j] = s[j] * a.scale;
+  if constexpr (sizeof(TO) == 4) {
+    if (a.accumulate) {
+      red_add<VEC>(dst, f);
+      return;
+    }
+  }
   Vec<TO, VEC> y;
   if (a.accumulate) {
     Vec<TO, VEC> old;
@@ -354,7 +386,7 @@ __device__ __forceinline__ void put_row(const GradArgs& a, int key, long long c,
 }
 
 // One tile per threadIdx.y: its sorted positions in order, eight rows of
-// grad_out in flight per thread.
+// grad_out in flight per thread (sixteen leave too few warps: 68 us for 62 us).
 constexpr int kBatch = 8;
 
 template <typename TI, typename TO, int VEC>
@@ -386,6 +418,15 @@ __global__ void __launch_bounds__(256) grad_tiles_kernel(const GradArgs a) {
 #pragma unroll
     for (int k = 0; k < kBatch; ++k)
       if (kv[k].x < a.v) x[k].load(static_cast<const TI*>(a.g) + kv[k].y * a.ldg + c);
+    if constexpr (sizeof(TO) == 2) {
+      // rows that will be read and added to
+      if (a.accumulate) {
+#pragma unroll
+        for (int k = 0; k < kBatch; ++k)
+          if (kv[k].x < a.v)
+            asm volatile("prefetch.global.L2 [%0];" ::"l"(static_cast<const TO*>(a.out) + kv[k].x * a.ldo + c));
+      }
+    }
 #pragma unroll
     for (int k = 0; k < kBatch; ++k) {
       if (p + k >= p1) break;
@@ -458,11 +499,12 @@ __global__ void __launch_bounds__(kRunX* kRunY) grad_runs_kernel(const GradArgs 
   put_row<TO, VEC>(a, key, c, s);
 }
 
-// Largest VEC (8, 4, 2, 1 elements) such that rows and their pieces are
-// aligned for both matrices: VEC divides h, and VEC elements (at most 16 bytes
-// of them at a time) divide the address and the leading dimension.
+// Largest VEC (8, 4, 2, 1 elements, 16 bytes of the first matrix) such that
+// rows and their pieces are aligned for both matrices: VEC divides h, and VEC
+// elements (at most 16 bytes of them at a time) divide the address and the
+// leading dimension.
 int pick_vec(long long h, const void* a, long long lda, int esa, const void* b, long long ldb, int esb) {
-  for (int vec = 8; vec > 1; vec /= 2) {
+  for (int vec = 16 / esa; vec > 1; vec /= 2) {
     auto ok = [vec](const void* p, long long ld, int es) {
       const long long bytes = std::min(16, vec * es);
       return reinterpret_cast<uintptr_t>(p) % bytes == 0 && ld * es % bytes == 0;
@@ -562,6 +604,29 @@ void launch_embed(const EmbedArgs& a, cudaStream_t st) {
   by_types(a.in_bf16, a.out_bf16, vec, EmbedCall{a, st});
 }
 
+// beside_clear: next to the clearing kernel, which reads and writes none of the sort's data.
+template <int THREADS>
+cudaError_t launch_sort(const SortArgs& s, bool beside_clear, cudaStream_t st) {
+  static std::mutex mu;
+  static uint64_t ready = 0;
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e != cudaSuccess) return e;
+  {
+    std::lock_guard<std::mutex> lock(mu);
+    if (!(ready >> (dev & 63) & 1)) {
+      e = cudaFuncSetAttribute(sort_kernel<THREADS>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                               static_cast<int>(sort_smem_bytes(THREADS, kMaxDigitBits)));
+      if (e != cudaSuccess) return e;
+      ready |= 1ull << (dev & 63);
+    }
+  }
+  const size_t smem = sort_smem_bytes(THREADS, s.digit_bits);
+  if (beside_clear) return launch_pdl(sort_kernel<THREADS>, dim3(kSortCtas), dim3(THREADS), smem, st, s);
+  sort_kernel<THREADS><<<kSortCtas, THREADS, smem, st>>>(s);
+  return cudaGetLastError();
+}
+
 size_t embed_grad_workspace(long long n, long long h) { return grad_layout(n, h).total; }
 
 cudaError_t launch_embed_grad(const EmbedGradArgs& a, void* ws, int num_sms, cudaStream_t st, int* launches) {
@@ -591,19 +656,7 @@ cudaError_t launch_embed_grad(const EmbedGradArgs& a, void* ws, int num_sms, cud
     const cudaError_t e = cudaGetLastError();
     if (e != cudaSuccess || a.n == 0) return e;
   }
-  static std::once_flag once[64];
-  int dev = 0;
-  cudaGetDevice(&dev);
-  cudaError_t e = cudaSuccess;
-  std::call_once(once[dev & 63], [&] {
-    e = cudaFuncSetAttribute(sort_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(kSortSmem));
-  });
-  if (e != cudaSuccess) return e;
-  // beside the clearing kernel, which reads and writes none of the sort's data
-  const size_t smem = (kSortWarps + 2) * sizeof(uint32_t) << s.digit_bits;
-  if (a.accumulate) sort_kernel<<<kSortCtas, kSortThreads, smem, st>>>(s);
-  else e = launch_pdl(sort_kernel, dim3(kSortCtas), dim3(kSortThreads), smem, st, s);
-  if (e == cudaSuccess) e = cudaGetLastError();
+  cudaError_t e = a.n <= kFewIds ? launch_sort<512>(s, !a.accumulate, st) : launch_sort<1024>(s, !a.accumulate, st);
   if (e != cudaSuccess) return e;
   *launches += 1;
   GradArgs g{};
