@@ -385,12 +385,16 @@ __device__ __forceinline__ void put_row(const GradArgs& a, int key, long long c,
   y.store(dst);
 }
 
-// One tile per threadIdx.y: its sorted positions in order, eight rows of
-// grad_out in flight per thread (sixteen leave too few warps: 68 us for 62 us).
-constexpr int kBatch = 8;
+// One tile per threadIdx.y: its sorted positions in order, four rows of grad_out
+// in flight per thread; eight leave fewer warps (32768 x 2048 bf16: 98 us, 110 us
+// with eight) except for fp32 sums of bf16 rows, where the adds to L2 are the
+// slower part (8192 x 4096: 65 us with four, 60 us).
+template <typename TI, typename TO>
+constexpr int kBatchOf = sizeof(TI) == 2 && sizeof(TO) == 4 ? 8 : 4;
 
 template <typename TI, typename TO, int VEC>
 __global__ void __launch_bounds__(256) grad_tiles_kernel(const GradArgs a) {
+  constexpr int kBatch = kBatchOf<TI, TO>;
   pdl_trigger();
   pdl_wait();
   const int tile = blockIdx.x * blockDim.y + threadIdx.y;
@@ -574,19 +578,28 @@ struct GradCall {
   }
 };
 
-// Sorted positions per tile: long tiles leave fewer partial sums, short ones
-// give few tokens enough blocks.
-int tile_len(long long n) { return n >= 8192 ? 32 : n >= 2048 ? 16 : 8; }
+// Sorted positions per tile: long tiles leave fewer partial sums and fewer
+// blocks that look for runs, so the longest that gives the SMs 24 warps each
+// (8192 x 4096 bf16: 32, 200 us with the clearing; 16 and 64 204 us), and no more
+// than 2048 tiles where longer ones can be had (65536 x 256: 32, 82 us; 16 90 us).
+int tile_len(long long n, long long h, int vec) {
+  const long long warps = (h + 32 * vec - 1) / (32 * vec);  // per tile
+  int len = 64;
+  while (len > 8 && (n + len - 1) / len * warps < 148 * 24 && (n + len / 2 - 1) / (len / 2) <= 2048) len /= 2;
+  return len;
+}
 
 struct EmbedGradLayout {
   size_t buf0, buf1, part, total;
   long long ldp;
-  int tiles, len;
+  int tiles, len, vec;
 };
-EmbedGradLayout grad_layout(long long n, long long h) {
+EmbedGradLayout grad_layout(const EmbedGradArgs& a) {
   EmbedGradLayout L;
+  const long long n = a.n, h = a.h;
   auto up = [](size_t x) { return (x + 255) / 256 * 256; };
-  L.len = tile_len(n);
+  L.vec = pick_vec(h, a.g, a.ldg, a.in_bf16 ? 2 : 4, a.out, a.ldo, a.out_bf16 ? 2 : 4);
+  L.len = tile_len(n, h, L.vec);
   L.tiles = static_cast<int>((n + L.len - 1) / L.len);
   L.ldp = (h + 7) / 8 * 8;
   L.buf0 = 0;
@@ -627,12 +640,12 @@ cudaError_t launch_sort(const SortArgs& s, bool beside_clear, cudaStream_t st) {
   return cudaGetLastError();
 }
 
-size_t embed_grad_workspace(long long n, long long h) { return grad_layout(n, h).total; }
+size_t embed_grad_workspace(const EmbedGradArgs& a) { return grad_layout(a).total; }
 
 cudaError_t launch_embed_grad(const EmbedGradArgs& a, void* ws, int num_sms, cudaStream_t st, int* launches) {
   if (a.n == 0 && a.accumulate) return cudaSuccess;
   const int es_out = a.out_bf16 ? 2 : 4;
-  const EmbedGradLayout L = grad_layout(a.n, a.h);
+  const EmbedGradLayout L = grad_layout(a);
   uint8_t* w = static_cast<uint8_t*>(ws);
   SortArgs s{};
   s.ids = a.ids;
@@ -674,8 +687,7 @@ cudaError_t launch_embed_grad(const EmbedGradArgs& a, void* ws, int num_sms, cud
   g.accumulate = a.accumulate;
   g.part = reinterpret_cast<float*>(w + L.part);
   g.ldp = L.ldp;
-  const int vec = pick_vec(a.h, a.g, a.ldg, a.in_bf16 ? 2 : 4, a.out, a.ldo, es_out);
-  by_types(a.in_bf16, a.out_bf16, vec, GradCall{g, st, &e});
+  by_types(a.in_bf16, a.out_bf16, L.vec, GradCall{g, st, &e});
   *launches += L.tiles > 1 ? 2 : 1;
   return e;
 }

@@ -1899,7 +1899,7 @@ int orda_embedding_grad_device(OrdaContext* ctx, const OrdaDeviceMat* grad_out, 
   a.bad = ctx->d_words + 3;
   ctx->vocab_ready = false;  // the workspace no longer holds a vocabulary forward phase
   bool capturing = false;
-  if (int rc = call_ws(ctx, embed_grad_workspace(a.n, a.h), st, &capturing, err, err_len)) return rc;
+  if (int rc = call_ws(ctx, embed_grad_workspace(a), st, &capturing, err, err_len)) return rc;
   int nl = 0;
   const cudaError_t e = launch_embed_grad(a, ctx->ws, ctx->num_sms, st, &nl);
   ctx->launches += static_cast<uint64_t>(nl);

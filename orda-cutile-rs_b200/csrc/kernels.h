@@ -199,7 +199,7 @@ struct EmbedGradArgs {
   int accumulate = 0;
   int* bad = nullptr;
 };
-size_t embed_grad_workspace(long long n, long long h);
+size_t embed_grad_workspace(const EmbedGradArgs& a);
 cudaError_t launch_embed_grad(const EmbedGradArgs& a, void* ws, int num_sms, cudaStream_t st, int* launches);
 
 // ------------------------------------------------------------ row kernels
