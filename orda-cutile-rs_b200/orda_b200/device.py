@@ -432,58 +432,65 @@ def linear_cross_entropy_device(
     lse, grad_hidden and grad_weight to write into (their own types decide).
     piece_bytes bounds the 16-bit logits kept at once (0: 4 GiB); columns of
     the vocabulary beyond it are computed twice. nll and lse are those of
-    each token, for log-probabilities (-nll) and for a z-loss of the caller's.
+    each token, for log-probabilities (-nll without smoothing).
     Labels out of range are reported by ctx.check()."""
     if hidden.dim() != 2 or weight.dim() != 2 or labels.dim() != 1:
         raise ValueError("hidden and weight must be 2-D and labels 1-D")
     if labels.dtype != torch.int64 or not labels.is_contiguous():
         raise ValueError("labels must be contiguous int64")
-    if out and not out.keys() <= {"loss", "nll", "lse", "grad_hidden", "grad_weight"}:
+    if out is not None:
         unknown = set(out) - {"loss", "nll", "lse", "grad_hidden", "grad_weight"}
-        raise ValueError(f"unknown outputs {sorted(unknown)}")
-    out = out or {}
-    _on_context(ctx, hidden=hidden, weight=weight, labels=labels, **out)
-    bt, h = hidden.shape
-    v, dev = weight.shape[0], hidden.device
-    loss, nll, lse = out.get("loss"), out.get("nll"), out.get("lse")
-    for name, t, n in (("loss", loss, 1), ("nll", nll, bt), ("lse", lse, bt)):
-        if t is not None and (t.dtype != torch.float32 or t.numel() != n or not t.is_contiguous()):
-            raise ValueError(f"{name} must be contiguous float32 of {n} element(s)")
-    if loss is None and nll is None and lse is None:
+        if unknown:
+            raise ValueError(f"unknown outputs {sorted(unknown)}")
+    dev = ctx.device
+    if hidden.get_device() != dev or weight.get_device() != dev or labels.get_device() != dev:
+        _on_context(ctx, hidden=hidden, weight=weight, labels=labels)
+    h_mat, w_mat = _mat(_abi.OrdaDeviceMat, hidden, "hidden"), _mat(_abi.OrdaDeviceMat, weight, "weight")
+    bt, h, v = h_mat.rows, h_mat.cols, w_mat.rows
+    if out is None:
         # one allocation for the three
-        store = torch.empty(2 * bt + 1, device=dev, dtype=torch.float32)
-        nll, lse, loss = store[:bt], store[bt:2 * bt], store[2 * bt:]
-    if loss is None:
-        loss = torch.empty(1, device=dev, dtype=torch.float32)
-    if nll is None:
-        nll = torch.empty(bt, device=dev, dtype=torch.float32)
-    if lse is None:
-        lse = torch.empty(bt, device=dev, dtype=torch.float32)
-    grads = []
-    for name, rows, need in (("grad_hidden", bt, need_grad_hidden), ("grad_weight", v, need_grad_weight)):
-        t = out.get(name)
-        if not need:
-            if t is not None:
+        store = torch.empty(2 * bt + 1, device=hidden.device, dtype=torch.float32)
+        nll, lse, loss = store.split((bt, bt, 1))
+        at = store.data_ptr()
+        o = _abi.OrdaLinearCeOutputs(at + 8 * bt, at, at + 4 * bt)
+    else:
+        for name, need in (("grad_hidden", need_grad_hidden), ("grad_weight", need_grad_weight)):
+            if not need and out.get(name) is not None:
                 raise ValueError(f"out holds {name}, which need_{name}=False leaves out")
-            grads.append((None, None, 0, 0))
-            continue
+        _on_context(ctx, **out)
+        given = []
+        for name, n in (("loss", 1), ("nll", bt), ("lse", bt)):
+            t = out.get(name)
+            if t is None:
+                t = torch.empty(n, device=hidden.device, dtype=torch.float32)
+            elif t.dtype != torch.float32 or t.numel() != n or not t.is_contiguous():
+                raise ValueError(f"{name} must be contiguous float32 of {n} element(s)")
+            given.append(t)
+        loss, nll, lse = given
+        o = _abi.OrdaLinearCeOutputs(loss.data_ptr(), nll.data_ptr(), lse.data_ptr())
+
+    def gradient(name, rows):
+        t = None if out is None else out.get(name)
         if t is None:
-            t = _row_major(rows, h, grad_dtype, dev)
+            t = _row_major(rows, h, grad_dtype, hidden.device)
         elif tuple(t.shape) != (rows, h) or (h > 1 and t.stride(1) != 1):
             raise ValueError(f"{name} must be ({rows}, {h}) with unit column stride")
         # a row stride means nothing for a single row
-        grads.append((t, t.data_ptr(), t.stride(0) if rows > 1 else max(t.stride(0), h), _grad_dtype(t, name)))
-    (gh, gh_ptr, gh_ld, gh_type), (gw, gw_ptr, gw_ld, gw_type) = grads
-    o = _abi.OrdaLinearCeOutputs(loss.data_ptr(), nll.data_ptr(), lse.data_ptr(), gh_ptr, gh_ld, gw_ptr, gw_ld,
-                                 gh_type, gw_type)
+        return t, t.data_ptr(), t.stride(0) if rows > 1 else max(t.stride(0), h), _grad_dtype(t, name)
+
+    gh = gw = None
+    if need_grad_hidden:
+        gh, o.grad_hidden, o.ld_grad_hidden, o.grad_hidden_dtype = gradient("grad_hidden", bt)
+    if need_grad_weight:
+        gw, o.grad_weight, o.ld_grad_weight, o.grad_weight_dtype = gradient("grad_weight", v)
     opts = _abi.OrdaLinearCeOptions(ignore_index, label_smoothing, reduction, global_non_ignore, piece_bytes)
     buf = _err()
-    rc = _lib().orda_linear_cross_entropy_device(
-        ctx.handle, C.byref(_mat(_abi.OrdaDeviceMat, hidden, "hidden")),
-        C.byref(_mat(_abi.OrdaDeviceMat, weight, "weight")), labels.data_ptr(), labels.numel(), C.byref(opts),
-        C.byref(o), _context_stream(ctx, stream), buf, len(buf))
-    _check(rc, buf)
-    return LinearCrossEntropyResult(loss.view(-1)[0], nll, lse, gh, gw)
+    rc = _lib().orda_linear_cross_entropy_device(ctx.handle, C.byref(h_mat), C.byref(w_mat), labels.data_ptr(),
+                                                 labels.numel(), C.byref(opts), C.byref(o),
+                                                 _context_stream(ctx, stream), buf, len(buf))
+    if rc:
+        _check(rc, buf)
+    return LinearCrossEntropyResult(loss.view(()), nll, lse, gh, gw)
 
 
 def _ids(ids: torch.Tensor) -> torch.Tensor:
@@ -530,10 +537,11 @@ def embedding_device(
         raise ValueError("table must be 2-D")
     _ids(ids)
     src = _mat(_abi.OrdaDeviceMat, table, "table")
-    _on_context(ctx, table=table, ids=ids, out=out)
-    n, h = ids.numel(), table.shape[1]
+    if table.get_device() != ctx.device or ids.get_device() != ctx.device or out is not None:
+        _on_context(ctx, table=table, ids=ids, out=out)
+    n, h = ids.numel(), src.cols
     if out is None:
-        out = torch.empty((*ids.shape, h), device=table.device, dtype=dtype or table.dtype)
+        out = table.new_empty((*ids.shape, h), dtype=dtype)
         dst = _abi.OrdaDeviceMatMut(out.data_ptr(), n, h, h, _grad_dtype(out, "out"))
     elif dtype is not None and out.dtype != dtype:
         raise ValueError(f"out is {out.dtype}, not {dtype}")
@@ -542,7 +550,8 @@ def embedding_device(
     buf = _err()
     rc = _lib().orda_embedding_device(ctx.handle, C.byref(src), ids.data_ptr(), n, scale, C.byref(dst),
                                       _context_stream(ctx, stream), buf, len(buf))
-    _check(rc, buf)
+    if rc:
+        _check(rc, buf)
     return out
 
 
