@@ -343,37 +343,12 @@ struct GradArgs {
   long long ldp;
 };
 
-// Adds to fp32 elements in L2 without waiting for them. Each element of the
-// gradient gets one addition per call, so the order of the additions cannot
-// matter; a read, add and write here would put a memory latency at each run's
-// end (72 us instead of 58 us for 8192 tokens on top of an fp32 gradient).
-template <int VEC>
-__device__ __forceinline__ void red_add(float* p, const float (&f)[VEC]) {
-  if constexpr (VEC % 4 == 0) {
-#pragma unroll
-    for (int j = 0; j < VEC; j += 4)
-      asm volatile("red.global.add.v4.f32 [%0], {%1, %2, %3, %4};" ::"l"(p + j), "f"(f[j]), "f"(f[j + 1]), "f"(f[j + 2]),
-                   "f"(f[j + 3])
-                   : "memory");
-  } else if constexpr (VEC == 2) {
-    asm volatile("red.global.add.v2.f32 [%0], {%1, %2};" ::"l"(p), "f"(f[0]), "f"(f[1]) : "memory");
-  } else {
-    asm volatile("red.global.add.f32 [%0], %1;" ::"l"(p), "f"(f[0]) : "memory");
-  }
-}
-
 template <typename TO, int VEC>
 __device__ __forceinline__ void put_row(const GradArgs& a, int key, long long c, const float (&s)[VEC]) {
   TO* dst = static_cast<TO*>(a.out) + key * a.ldo + c;
   float f[VEC];
 #pragma unroll
   for (int j = 0; j < VEC; ++j) f[j] = s[j] * a.scale;
-  if constexpr (sizeof(TO) == 4) {
-    if (a.accumulate) {
-      red_add<VEC>(dst, f);
-      return;
-    }
-  }
   Vec<TO, VEC> y;
   if (a.accumulate) {
     Vec<TO, VEC> old;
@@ -386,15 +361,14 @@ __device__ __forceinline__ void put_row(const GradArgs& a, int key, long long c,
 }
 
 // One tile per threadIdx.y: its sorted positions in order, four rows of grad_out
-// in flight per thread; eight leave fewer warps (32768 x 2048 bf16: 98 us, 110 us
-// with eight) except for fp32 sums of bf16 rows, where the adds to L2 are the
-// slower part (8192 x 4096: 65 us with four, 60 us).
-template <typename TI, typename TO>
-constexpr int kBatchOf = sizeof(TI) == 2 && sizeof(TO) == 4 ? 8 : 4;
+// in flight per thread (eight leave fewer warps: 32768 x 2048 bf16 took 110 us,
+// 98 us with four). On top of a gradient, the rows that will be read and added
+// to are asked for with the rows of grad_out: 8192 tokens on top of 4096 fp32
+// columns take 55 us, 72 us without, and 60 us with fp32 adds in L2 instead.
+constexpr int kBatch = 4;
 
 template <typename TI, typename TO, int VEC>
 __global__ void __launch_bounds__(256) grad_tiles_kernel(const GradArgs a) {
-  constexpr int kBatch = kBatchOf<TI, TO>;
   pdl_trigger();
   pdl_wait();
   const int tile = blockIdx.x * blockDim.y + threadIdx.y;
@@ -422,14 +396,11 @@ __global__ void __launch_bounds__(256) grad_tiles_kernel(const GradArgs a) {
 #pragma unroll
     for (int k = 0; k < kBatch; ++k)
       if (kv[k].x < a.v) x[k].load(static_cast<const TI*>(a.g) + kv[k].y * a.ldg + c);
-    if constexpr (sizeof(TO) == 2) {
-      // rows that will be read and added to
-      if (a.accumulate) {
+    if (a.accumulate) {
 #pragma unroll
-        for (int k = 0; k < kBatch; ++k)
-          if (kv[k].x < a.v)
-            asm volatile("prefetch.global.L2 [%0];" ::"l"(static_cast<const TO*>(a.out) + kv[k].x * a.ldo + c));
-      }
+      for (int k = 0; k < kBatch; ++k)
+        if (kv[k].x < a.v)
+          asm volatile("prefetch.global.L2 [%0];" ::"l"(static_cast<const TO*>(a.out) + kv[k].x * a.ldo + c));
     }
 #pragma unroll
     for (int k = 0; k < kBatch; ++k) {
