@@ -51,7 +51,7 @@ struct OrdaContext {
   // kept until they are reported), [4] live tokens and [5] finished blocks of a
   // linear cross entropy call (0 between calls)
   int* d_words = nullptr;
-  float* d_mean_scale = nullptr;
+  float* d_mean_scale = nullptr;  // [0] distillation loss, [1] linear cross entropy
   void* ws = nullptr;
   size_t ws_bytes = 0;
   // A graph captured with this workspace replays with its address: once that
@@ -1078,6 +1078,7 @@ int run_linear_ce(OrdaContext* ctx, const OrdaDeviceMat& hm, const OrdaDeviceMat
   a.nll = out.nll ? out.nll : reinterpret_cast<float*>(ws + L.nll);
   a.lse = out.lse;
   a.loss = out.loss;
+  a.scale = ctx->d_mean_scale + 1;
   a.status = ctx->d_words;
   a.bad_label = ctx->d_words + 2;
   a.count = ctx->d_words + 4;
@@ -1154,6 +1155,7 @@ int run_linear_ce(OrdaContext* ctx, const OrdaDeviceMat& hm, const OrdaDeviceMat
       if (L.dgrad_direct) {
         gd.args.out0 = static_cast<float*>(out.grad_hidden);
         gd.args.ld0 = static_cast<long long>(out.ld_grad_hidden);
+        gd.args.alpha_ptr = a.scale;
       } else {
         gd.args.out0 = reinterpret_cast<float*>(ws + L.dgrad);
         gd.args.ld0 = static_cast<long long>(L.ld_dgrad);
@@ -1182,6 +1184,7 @@ int run_linear_ce(OrdaContext* ctx, const OrdaDeviceMat& hm, const OrdaDeviceMat
       gd.N = a.hd;
       gd.raster_n_fastest = true;
       gd.status = ctx->d_words;
+      gd.args.alpha_ptr = a.scale;
       if (out.grad_weight_dtype == ORDA_DTYPE_BF16) {
         gd.epi = Epi::StoreBf16;
         gd.args.out16 = static_cast<uint16_t*>(out.grad_weight) + v0 * out.ld_grad_weight;
@@ -1204,7 +1207,7 @@ int run_linear_ce(OrdaContext* ctx, const OrdaDeviceMat& hm, const OrdaDeviceMat
     ph.launched();
     if ((e = launch_slab_sum(reinterpret_cast<const float*>(ws + L.dgrad), L.slabs,
                              static_cast<long long>(L.slab_rows), static_cast<long long>(L.ld_dgrad), a.bt, a.hd,
-                             out.grad_hidden, static_cast<long long>(out.ld_grad_hidden),
+                             a.scale, out.grad_hidden, static_cast<long long>(out.ld_grad_hidden),
                              out.grad_hidden_dtype == ORDA_DTYPE_BF16, st)) != cudaSuccess)
       return cuda_fail(e, "dgrad sum", err, len);
   }

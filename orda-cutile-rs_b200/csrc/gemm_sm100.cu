@@ -746,18 +746,20 @@ __global__ void __launch_bounds__(epi_threads(EPI), 1)
         ce_epilogue<EPI>(p, &mapC, buf, lane, t_row, colh, row0, grow, row_ok, colh / kCePartCols, row_c, pol_c,
                          release_tmem);
       } else if constexpr (EPI == kEpiStoreBf16) {
+        const float alpha = p.e.alpha_ptr ? *p.e.alpha_ptr : p.e.alpha;
         auto store = [&](int c, const uint32_t(&r)[32]) {
           const int col0 = colh + c * 32;
           if (p.tma_store) {
             uint32_t q[16];
 #pragma unroll
-            for (int j = 0; j < 16; ++j) q[j] = pack_bf16x2(__uint_as_float(r[2 * j]), __uint_as_float(r[2 * j + 1]));
+            for (int j = 0; j < 16; ++j)
+              q[j] = pack_bf16x2(alpha * __uint_as_float(r[2 * j]), alpha * __uint_as_float(r[2 * j + 1]));
             stage16(buf, lane, q, &mapC, col0, row0, row0 < p.M && col0 < p.N, pol_c);
           } else if (row_ok) {
             __nv_bfloat16* dst = static_cast<__nv_bfloat16*>(p.e.out16) + grow * p.e.ld16 + col0;
 #pragma unroll
             for (int j = 0; j < 32; ++j)
-              if (col0 + j < p.N) dst[j] = __float2bfloat16_rn(__uint_as_float(r[j]));
+              if (col0 + j < p.N) dst[j] = __float2bfloat16_rn(alpha * __uint_as_float(r[j]));
           }
         };
         uint32_t r[32];

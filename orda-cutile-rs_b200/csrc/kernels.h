@@ -41,7 +41,7 @@ enum class Epi : int { Store = 0, Logits = 1, StoreBf16 = 2, CeStats = 3, CeGrad
 // split_row go to out0, the rest to out1 (row - split_row).
 // Logits: fp32 logits written to `logits` (ldl) plus per-(row, 128-column
 // part) online-softmax records (see rows.cu for the record layout).
-// StoreBf16: out16 = acc rounded to bf16.
+// StoreBf16: out16 = alpha * acc rounded to bf16.
 // CeStats / CeGrad: the two passes of the linear cross entropy over a piece
 // of the vocabulary (see linear_ce.cu).
 constexpr int kPdlWaitFirst = 1, kPdlWaitLast = 2;
@@ -157,6 +157,7 @@ struct CeArgs {
   float* nll = nullptr;         // [bt]
   float* lse = nullptr;         // [bt], optional
   float* loss = nullptr;        // [1]
+  float* scale = nullptr;       // [1] what the gradients are multiplied by after the products
   int* status = nullptr;        // cleared by the first kernel
   int* bad_label = nullptr;     // set to DEV_LABEL_RANGE
   int* count = nullptr;         // live tokens; 0 between calls
@@ -167,9 +168,9 @@ cudaError_t launch_ce_prep(const CeArgs& a, cudaStream_t stream);
 // Records -> nll, lse, the gradient's row constants and the loss; and with a
 // piece the kept 16-bit logits of its n first columns -> bf16 logit gradients.
 cudaError_t launch_ce_rows(const CeArgs& a, uint16_t* piece, long long ld, long long n, cudaStream_t stream);
-// out = the sum over slabs of buf (fp32 [slabs][slab_rows][ldb]) for rows x cols, as bf16 or fp32.
+// out = *scale times the sum over slabs of buf (fp32 [slabs][slab_rows][ldb]) for rows x cols, as bf16 or fp32.
 cudaError_t launch_slab_sum(const float* buf, int slabs, long long slab_rows, long long ldb, long long rows, long long cols,
-                     void* out, long long ldo, int out_bf16, cudaStream_t stream);
+                            const float* scale, void* out, long long ldo, int out_bf16, cudaStream_t stream);
 
 // ---------------------------------------------------- embedding (embedding.cu)
 struct EmbedArgs {

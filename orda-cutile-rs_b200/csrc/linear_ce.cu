@@ -4,7 +4,9 @@
 // With z = h W^T, y the label, a the label smoothing and g the loss scale:
 //   lse = log sum_v e^{z_v}
 //   nll = (1 - a) (lse - z_y) + a (lse - mean_v z_v)
-//   dz_v = g (e^{z_v - lse} - (1 - a) [v = y] - a / V),  dh = dz W,  dW = dz^T h
+//   dz_v = e^{z_v - lse} - (1 - a) [v = y] - a / V,  dh = g dz W,  dW = g dz^T h
+// (g after the products: in dz it would round one factor of every row, 1 / the
+// count of tokens, to bf16)
 // The label's logit is the reference of its row: the logits product sums
 // Z_o = sum_{v != y} e^{z_v - z_y} per 64-column part, so that
 //   lse - z_y = log(1 + Z_o),  1 - p_y = Z_o / (1 + Z_o)
@@ -129,15 +131,12 @@ __device__ __forceinline__ void acc_add(Acc& a, double d, float r) {
 // the row does the same. Results are fp32, and so is the arithmetic where no
 // two large numbers cancel.
 struct RowResult {
-  float4 c;  // -lse log2 e + log2 g, label, a / V g, the label's gradient
+  float4 c;  // -lse log2 e, label, a / V, the label's gradient
   float nll, lse;
 };
 
 __device__ __forceinline__ RowResult row_result(const CeArgs& a, float2 ref, const Acc& m, float sx) {
   RowResult r;
-  const long long n = a.denom_override > 0 ? a.denom_override : max(*static_cast<volatile int*>(a.count), 1);
-  const float nf = a.reduction_sum ? 1.f : static_cast<float>(n);
-  const float g = 1.f / nf;
   float gap, miss, l;  // lse - z_y, 1 - p_y and lse
   if (m.r == ref.x) {
     const float z = static_cast<float>(m.d);
@@ -155,17 +154,23 @@ __device__ __forceinline__ RowResult row_result(const CeArgs& a, float2 ref, con
   const float uni = a.alpha / static_cast<float>(a.v);
   r.nll = a.alpha > 0.f ? (1.f - a.alpha) * gap + a.alpha * (l - sx / static_cast<float>(a.v)) : gap;
   r.lse = l;
-  r.c.x = fmaf(-l, kLog2E, -log2f(nf));
+  r.c.x = -l * kLog2E;
   r.c.y = ref.y;
-  r.c.z = g * uni;
-  r.c.w = g * (a.alpha - uni - miss);
+  r.c.z = uni;
+  r.c.w = a.alpha - uni - miss;
   return r;
+}
+
+// The count of tokens that the mean divides by (1 for a sum).
+__device__ __forceinline__ double loss_denominator(const CeArgs& a) {
+  if (a.reduction_sum) return 1.0;
+  return static_cast<double>(a.denom_override > 0 ? a.denom_override : max(*static_cast<volatile int*>(a.count), 1));
 }
 
 // One block per row, or several along the columns where the rows are few:
 //   * the row's records (coalesced, 8 bytes per 64 columns) -> constants;
-//   * 16-bit logits -> bf16 logit gradients, in place: 2^(t + off) - a g / V with
-//     off = (the part's reference - lse) log2 e + log2 g. Bound by bandwidth, 4 bytes
+//   * 16-bit logits -> bf16 logit gradients, in place: 2^(t + off) - a / V with
+//     off = (the part's reference - lse) log2 e. Bound by bandwidth, 4 bytes
 //     per element; a thread holds 8 neighbouring columns, and the first loads
 //     are under way while the constants are formed.
 // The block that ends last sums the losses in row order.
@@ -260,6 +265,7 @@ __global__ void __launch_bounds__(kRowThreads) ce_rows_kernel(const CeArgs a, ui
       a.row_const[row] = r.c;
       a.nll[row] = r.nll;
       if (a.lse) a.lse[row] = r.lse;
+      if (row == 0) *a.scale = static_cast<float>(1.0 / loss_denominator(a));
       __threadfence();
     }
   }
@@ -316,20 +322,20 @@ __global__ void __launch_bounds__(kRowThreads) ce_rows_kernel(const CeArgs a, ui
   if (threadIdx.x == 0) {
     s = 0.0;
     for (int w = 0; w < kRowThreads / 32; ++w) s += d_s[w];
-    const long long live_n = a.denom_override > 0 ? a.denom_override : max(*static_cast<volatile int*>(a.count), 1);
-    *a.loss = static_cast<float>(a.reduction_sum ? s : s / static_cast<double>(live_n));
+    *a.loss = static_cast<float>(s / loss_denominator(a));
     *a.count = 0;
     *a.done = 0;
   }
 }
 
-// Sum over K slabs, in slab order, and the output's type.
+// scale times the sum over K slabs, in slab order, and the output's type.
 template <bool BF16>
 __global__ void __launch_bounds__(256)
     slab_sum_kernel(const float* __restrict__ buf, int slabs, long long slab_rows, long long ldb, long long rows,
-                    long long cols, void* out, long long ldo, int vec_ok) {
+                    long long cols, const float* scale, void* out, long long ldo, int vec_ok) {
   pdl_trigger();
   pdl_wait();
+  const float g = *scale;
   const long long groups = (cols + 3) / 4;
   for (long long i = blockIdx.x * 256ll + threadIdx.x; i < rows * groups; i += gridDim.x * 256ll) {
     const long long r = i / groups, c = (i - r * groups) * 4;
@@ -342,6 +348,7 @@ __global__ void __launch_bounds__(256)
       s.z += x.z;
       s.w += x.w;
     }
+    s = make_float4(g * s.x, g * s.y, g * s.z, g * s.w);
     const float f[4] = {s.x, s.y, s.z, s.w};
     if (BF16) {
       __nv_bfloat16* o = static_cast<__nv_bfloat16*>(out) + r * ldo + c;
@@ -377,13 +384,14 @@ cudaError_t launch_ce_rows(const CeArgs& a, uint16_t* piece, long long ld, long 
 }
 
 cudaError_t launch_slab_sum(const float* buf, int slabs, long long slab_rows, long long ldb, long long rows,
-                            long long cols, void* out, long long ldo, int out_bf16, cudaStream_t stream) {
+                            long long cols, const float* scale, void* out, long long ldo, int out_bf16,
+                            cudaStream_t stream) {
   const long long n = rows * ((cols + 3) / 4);
   const unsigned blocks = static_cast<unsigned>(std::min<long long>((n + 255) / 256, 148 * 16));
   const int esz = out_bf16 ? 2 : 4;
   const int vec_ok = reinterpret_cast<uintptr_t>(out) % (4 * esz) == 0 && ldo % 4 == 0;
   return launch_pdl(out_bf16 ? slab_sum_kernel<true> : slab_sum_kernel<false>, dim3(blocks), dim3(256), 0, stream, buf,
-                    slabs, slab_rows, ldb, rows, cols, out, ldo, vec_ok);
+                    slabs, slab_rows, ldb, rows, cols, scale, out, ldo, vec_ok);
 }
 
 }  // namespace orda
