@@ -474,6 +474,85 @@ __global__ void __launch_bounds__(kRunX* kRunY) grad_runs_kernel(const GradArgs 
   put_row<TO, VEC>(a, key, c, s);
 }
 
+// ------------------------------------------------- the gradient, few tokens
+// Up to kFewTokens tokens need no sort: the block of a token looks through all
+// ids, leaves if an earlier token has the same one, and otherwise adds up the rows
+// of all that do, in order (split over threadIdx.y in contiguous parts that are
+// added in order). One launch after the clearing one, which it overlaps until it
+// writes, instead of three.
+// (500 x 1024 on top of fp32: 6.2 us, 14.5 us sorted; 1000 x 1024: 10.6 and 16.4 us,
+// but a run then may be 1024 rows long in one block.)
+constexpr int kFewTokens = 512;
+constexpr int kFewBatch = 8;
+
+template <typename TI, typename TO, int VEC>
+__global__ void __launch_bounds__(256) grad_few_kernel(const EmbedGradArgs a) {
+  __shared__ int list[kFewTokens];
+  __shared__ int warp_n[8];
+  __shared__ float sum_s[256 * VEC];
+  const int i = blockIdx.x, n = static_cast<int>(a.n);
+  const int tid = threadIdx.y * blockDim.x + threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int64_t id = a.ids[i];
+  if (a.has_padding && id == a.padding_id) return;
+  if (id < 0 || id >= a.v) {
+    if (tid == 0) atomicExch(a.bad, DEV_ID_RANGE);
+    return;
+  }
+  int count = 0;
+  for (int j0 = 0; j0 < n; j0 += 256) {
+    const int j = j0 + tid;
+    const bool same = j < n && a.ids[j] == id;
+    const uint32_t votes = __ballot_sync(0xffffffffu, same);
+    if (lane == 0) warp_n[warp] = __popc(votes);
+    __syncthreads();
+    int at = count;
+#pragma unroll
+    for (int w = 0; w < 8; ++w) {
+      if (w < warp) at += warp_n[w];
+      count += warp_n[w];
+    }
+    if (same) list[at + __popc(votes & ((1u << lane) - 1))] = j;
+    __syncthreads();
+    if (count > 0 && list[0] < i) return;  // an earlier token's block does it
+  }
+  const int each = (count + blockDim.y - 1) / blockDim.y;
+  const int k0 = threadIdx.y * each, k1 = min(count, k0 + each);
+  const long long c = (static_cast<long long>(blockIdx.y) * blockDim.x + threadIdx.x) * VEC;
+  float s[VEC];
+#pragma unroll
+  for (int j = 0; j < VEC; ++j) s[j] = 0.f;
+  if (c < a.h) {
+    for (int k = k0; k < k1; k += kFewBatch) {
+      Vec<TI, VEC> x[kFewBatch];
+#pragma unroll
+      for (int b = 0; b < kFewBatch; ++b)
+        if (k + b < k1) x[b].load(static_cast<const TI*>(a.g) + list[k + b] * a.ldg + c);
+#pragma unroll
+      for (int b = 0; b < kFewBatch; ++b)
+        if (k + b < k1)
+#pragma unroll
+          for (int j = 0; j < VEC; ++j) s[j] += x[b].get(j);
+    }
+  }
+  if (blockDim.y > 1) {
+#pragma unroll
+    for (int j = 0; j < VEC; ++j) sum_s[tid * VEC + j] = s[j];
+    __syncthreads();
+    if (threadIdx.y != 0) return;
+    for (int y = 1; y < static_cast<int>(blockDim.y); ++y)
+#pragma unroll
+      for (int j = 0; j < VEC; ++j) s[j] += sum_s[(y * blockDim.x + threadIdx.x) * VEC + j];
+  }
+  if (c >= a.h) return;
+  pdl_wait();  // the rows are cleared
+  GradArgs o{};
+  o.scale = a.scale;
+  o.out = a.out;
+  o.ldo = a.ldo;
+  o.accumulate = a.accumulate;
+  put_row<TO, VEC>(o, static_cast<int>(id), c, s);
+}
+
 // Largest VEC (8, 4, 2, 1 elements, 16 bytes of the first matrix) such that
 // rows and their pieces are aligned for both matrices: VEC divides h, and VEC
 // elements (at most 16 bytes of them at a time) divide the address and the
@@ -513,6 +592,16 @@ cudaError_t grad_t(const GradArgs& a, cudaStream_t st) {
                              dim3((a.tiles + y - 1) / y, groups(static_cast<long long>(x) * VEC)), dim3(x, y), 0, st, a);
   if (e != cudaSuccess || a.tiles < 2) return e;
   return launch_pdl(grad_runs_kernel<TO, VEC>, dim3(a.tiles - 1, groups(kRunX * VEC)), dim3(kRunX, kRunY), 0, st, a);
+}
+
+template <typename TI, typename TO, int VEC>
+cudaError_t few_t(const EmbedGradArgs& a, bool after_clear, cudaStream_t st) {
+  const int x = row_threads(a.h, VEC, 1);
+  const long long cols = static_cast<long long>(x) * VEC;
+  const dim3 grid(static_cast<unsigned>(a.n), static_cast<unsigned>((a.h + cols - 1) / cols)), block(x, 256 / x);
+  if (after_clear) return launch_pdl(grad_few_kernel<TI, TO, VEC>, grid, block, 0, st, a);
+  grad_few_kernel<TI, TO, VEC><<<grid, block, 0, st>>>(a);
+  return cudaGetLastError();
 }
 
 template <typename F>
@@ -588,6 +677,17 @@ void launch_embed(const EmbedArgs& a, cudaStream_t st) {
   by_types(a.in_bf16, a.out_bf16, vec, EmbedCall{a, st});
 }
 
+struct FewCall {
+  const EmbedGradArgs& a;
+  bool after_clear;
+  cudaStream_t st;
+  cudaError_t* e;
+  template <typename TI, typename TO, int VEC>
+  void operator()() const {
+    *e = few_t<TI, TO, VEC>(a, after_clear, st);
+  }
+};
+
 // beside_clear: next to the clearing kernel, which reads and writes none of the sort's data.
 template <int THREADS>
 cudaError_t launch_sort(const SortArgs& s, bool beside_clear, cudaStream_t st) {
@@ -611,11 +711,27 @@ cudaError_t launch_sort(const SortArgs& s, bool beside_clear, cudaStream_t st) {
   return cudaGetLastError();
 }
 
-size_t embed_grad_workspace(const EmbedGradArgs& a) { return grad_layout(a).total; }
+size_t embed_grad_workspace(const EmbedGradArgs& a) { return a.n <= kFewTokens ? 0 : grad_layout(a).total; }
 
 cudaError_t launch_embed_grad(const EmbedGradArgs& a, void* ws, int num_sms, cudaStream_t st, int* launches) {
   if (a.n == 0 && a.accumulate) return cudaSuccess;
   const int es_out = a.out_bf16 ? 2 : 4;
+  if (!a.accumulate) {
+    const long long bytes = a.v * a.h * es_out;
+    const long long blocks = std::max<long long>(1, std::min<long long>((bytes + 8191) / 8192, num_sms * kClearBlocks));
+    clear_kernel<<<static_cast<unsigned>(blocks), 256, 0, st>>>(static_cast<uint8_t*>(a.out), a.v, a.h * es_out,
+                                                                a.ldo * es_out);
+    *launches += 1;
+    const cudaError_t e = cudaGetLastError();
+    if (e != cudaSuccess || a.n == 0) return e;
+  }
+  if (a.n <= kFewTokens) {
+    cudaError_t e = cudaSuccess;
+    const int vec = pick_vec(a.h, a.g, a.ldg, a.in_bf16 ? 2 : 4, a.out, a.ldo, es_out);
+    by_types(a.in_bf16, a.out_bf16, vec, FewCall{a, !a.accumulate, st, &e});
+    *launches += 1;
+    return e;
+  }
   const EmbedGradLayout L = grad_layout(a);
   uint8_t* w = static_cast<uint8_t*>(ws);
   SortArgs s{};
@@ -631,15 +747,6 @@ cudaError_t launch_embed_grad(const EmbedGradArgs& a, void* ws, int num_sms, cud
   s.buf0 = reinterpret_cast<int2*>(w + L.buf0);
   s.buf1 = reinterpret_cast<int2*>(w + L.buf1);
   s.bad = a.bad;
-  if (!a.accumulate) {
-    const long long bytes = a.v * a.h * es_out;
-    const long long blocks = std::max<long long>(1, std::min<long long>((bytes + 8191) / 8192, num_sms * kClearBlocks));
-    clear_kernel<<<static_cast<unsigned>(blocks), 256, 0, st>>>(static_cast<uint8_t*>(a.out), a.v, a.h * es_out,
-                                                                a.ldo * es_out);
-    *launches += 1;
-    const cudaError_t e = cudaGetLastError();
-    if (e != cudaSuccess || a.n == 0) return e;
-  }
   cudaError_t e = a.n <= kFewIds ? launch_sort<512>(s, !a.accumulate, st) : launch_sort<1024>(s, !a.accumulate, st);
   if (e != cudaSuccess) return e;
   *launches += 1;

@@ -962,6 +962,7 @@ struct CeLayout {
   size_t cols = 0;      // vocabulary columns of one piece
   size_t n_parts = 0, rec_ld = 0, clean_rows = 0, ld_clean = 0, ld_piece = 0, ld_dgrad = 0, slab_rows = 0;
   int slabs = 1;
+  bool few = false;           // logits by few_kernel
   bool dgrad_direct = false;  // the dgrad product writes the fp32 output itself
 };
 
@@ -983,7 +984,8 @@ CeLayout ce_layout(size_t bt, size_t h, size_t v, size_t cols, bool smooth, cons
   CeLayout L;
   const bool grads = o.grad_hidden || o.grad_weight;
   L.cols = cols;
-  L.n_parts = ceil_div(v, kCePartCols);
+  L.few = bt <= kCeFewRows;
+  L.n_parts = ceil_div(v, L.few ? kCeFewPartCols : kCePartCols);
   L.rec_ld = round_up(L.n_parts, 4);  // rows of records start on 32-byte sectors
   // rows on 128-byte lines: a TMA box row (128 bytes) then is one line, not two
   // (1999 x 1000 x 100003 with gradients: 1.42 ms, 1.67 ms with 16-byte rows)
@@ -995,10 +997,10 @@ CeLayout ce_layout(size_t bt, size_t h, size_t v, size_t cols, bool smooth, cons
     off = round_up(off + bytes, 256);
     return at;
   };
-  // at least 32 rows (zeros behind the last token): rows of a TMA box beyond the
-  // matrix are still fetched, all from one place, and 148 SMs asking for the same
-  // lines took the logits of one token from 190 us to 250 us (H = 4096, V = 131072)
-  L.clean_rows = std::max<size_t>(bt, 32);
+  // few tokens: as many rows as the kernel reads (zeros behind the last token). Rows
+  // of a TMA box beyond the matrix are fetched too, all from one place, and 148 SMs
+  // asking for the same lines cost a quarter of the time
+  L.clean_rows = L.few ? static_cast<size_t>(few_rows(static_cast<long long>(bt))) : bt;
   L.h_clean = take(L.clean_rows * L.ld_clean * 2);
   L.ref = take(bt * sizeof(float2));
   L.rec = take(bt * L.rec_ld * sizeof(float2));
@@ -1074,6 +1076,9 @@ int run_linear_ce(OrdaContext* ctx, const OrdaDeviceMat& hm, const OrdaDeviceMat
   a.sx = smooth ? reinterpret_cast<float*>(ws + L.sx) : nullptr;
   a.rec_ld = static_cast<long long>(L.rec_ld);
   a.n_parts = static_cast<int>(L.n_parts);
+  a.part_shift = L.few ? 5 : 6;
+  static_assert(kCeFewPartCols == 1 << 5 && kCePartCols == 1 << 6, "part_shift");
+  a.cut = cut_factor(a.hd);
   a.row_const = reinterpret_cast<float4*>(ws + L.row_const);
   a.nll = out.nll ? out.nll : reinterpret_cast<float*>(ws + L.nll);
   a.lse = out.lse;
@@ -1109,16 +1114,17 @@ int run_linear_ce(OrdaContext* ctx, const OrdaDeviceMat& hm, const OrdaDeviceMat
     gd.args.out16 = keep;
     gd.args.ld16 = static_cast<long long>(L.ld_piece);
     gd.args.ce_v0 = static_cast<long long>(v0);
+    gd.args.ce_log2e = static_cast<float>(1.4426950408889634 * (1.0 + static_cast<double>(h) * 0x1p-30));
     gd.args.ce_ref = a.ref;
-    gd.args.ce_rec = a.rec + v0 / kCePartCols;
-    gd.args.ce_sx = smooth ? a.sx + v0 / kCePartCols : nullptr;
+    gd.args.ce_rec = a.rec + (v0 >> a.part_shift);
+    gd.args.ce_sx = smooth ? a.sx + (v0 >> a.part_shift) : nullptr;
     gd.args.ce_rec_ld = a.rec_ld;
     gd.args.ce_const = a.row_const;
     gd.args.pdl = kPdlWaitFirst;
     gd.demote_kept = ctx->l2_set;
     gd.launches = &nl;
-    if ((e = gemm_launch(gd, ctx->num_sms, st, &why)) != cudaSuccess)
-      return cuda_fail(e, why ? why : "logits GEMM", err, len);
+    e = L.few && epi == Epi::CeStats ? few_launch(gd, ctx->num_sms, st, &why) : gemm_launch(gd, ctx->num_sms, st, &why);
+    if (e != cudaSuccess) return cuda_fail(e, why ? why : "logits GEMM", err, len);
     ph.launched(nl);
     return ORDA_OK;
   };

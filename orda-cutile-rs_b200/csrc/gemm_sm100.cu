@@ -384,13 +384,13 @@ __device__ __forceinline__ void stage16(uint8_t* buf, int lane, const uint32_t (
 // mantissa of t * 512 + (2^23 + 2^15): one FMA and half a byte permute per
 // element, where a conversion instruction would share the SFU's pipe with ex2.
 template <bool MASK, bool STORE, bool SX>
-__device__ __forceinline__ void ce_stats_chunk(const uint32_t (&r)[32], float ref2, int lab, int nvalid, float& d,
+__device__ __forceinline__ void ce_stats_chunk(const uint32_t (&r)[32], float log2e, float ref2, int lab, int nvalid, float& d,
                                                float& sx, uint32_t (&q)[16]) {
   float a[4] = {0.f, 0.f, 0.f, 0.f}, ax[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
   for (int j = 0; j < 32; ++j) {
     const float x = __uint_as_float(r[j]);
-    const float t = fmaf(x, LOG2E, -ref2);
+    const float t = fmaf(x, log2e, -ref2);
     float e = fast_exp2(t);
     if (MASK) e = (j < nvalid && j != lab) ? e : 0.0f;
     a[j & 3] += e;
@@ -435,8 +435,8 @@ __device__ __forceinline__ void ce_epilogue(const KParams& p, const CUtensorMap*
     if constexpr (GRAD) {
 #pragma unroll
       for (int j = 0; j < 16; ++j) {
-        float v0 = fast_exp2(fmaf(__uint_as_float(r[2 * j]), LOG2E, row_c.x)) - row_c.z;
-        float v1 = fast_exp2(fmaf(__uint_as_float(r[2 * j + 1]), LOG2E, row_c.x)) - row_c.z;
+        float v0 = fast_exp2(fmaf(__uint_as_float(r[2 * j]), p.e.ce_log2e, row_c.x)) - row_c.z;
+        float v1 = fast_exp2(fmaf(__uint_as_float(r[2 * j + 1]), p.e.ce_log2e, row_c.x)) - row_c.z;
         if (has_label) {
           if (lc == 2 * j) v0 = row_c.w;
           if (lc == 2 * j + 1) v1 = row_c.w;
@@ -444,9 +444,9 @@ __device__ __forceinline__ void ce_epilogue(const KParams& p, const CUtensorMap*
         q[j] = pack_bf16x2(v0, v1);
       }
     } else if (has_label || nvalid < 32) {
-      ce_stats_chunk<true, STORE, SX>(r, ref2, lc, nvalid, d, sx, q);
+      ce_stats_chunk<true, STORE, SX>(r, p.e.ce_log2e, ref2, lc, nvalid, d, sx, q);
     } else {
-      ce_stats_chunk<false, STORE, SX>(r, ref2, lc, 32, d, sx, q);
+      ce_stats_chunk<false, STORE, SX>(r, p.e.ce_log2e, ref2, lc, 32, d, sx, q);
     }
     if constexpr (STORE) {
       const int x = colh + c * 32;
@@ -479,7 +479,7 @@ __device__ __forceinline__ void ce_epilogue(const KParams& p, const CUtensorMap*
       }
       __syncwarp();
       // a part of nothing, or of logits near the type's lowest value, keeps the row's reference
-      if (out_of_range && m * LOG2E > -INFINITY) ref2 = m * LOG2E;
+      if (out_of_range && m * p.e.ce_log2e > -INFINITY) ref2 = m * p.e.ce_log2e;
       d = 0.f;
       sx = 0.f;
       // the first stores of this part are complete before it is written again
@@ -1214,7 +1214,312 @@ bool use_wide(const GemmDesc& d, long long k_blocks, long long m_blocks, int num
   return tiles >= num_sms && k_blocks >= (d.args.scatter ? 1024 : 128);
 }
 
+// ---------------------------------------------------------- few-row logits
+// The linear cross entropy's logits and statistics for at most 128 tokens, where
+// reading W once is the time. W is the MMA's A operand (M = 128 vocabulary
+// entries) and the tokens are its N, so the tensor cores' time follows the
+// tokens: with the tokens as a 256-row tile they keep it to 9 TB/s at best, and
+// half of the ring holds rows that are zero. Here a CTA has 96 to 160 KB of W in
+// flight: one token at H = 4096, V = 131072 takes 172 us (6.2 TB/s; 186 us as a
+// 256 x 256 tile), 77 tokens at H = 2048, V = 128256 98 us (102 us). W comes in
+// boxes of 128 rows: boxes of 32 rows, which would let the CTAs' shares differ by
+// less, took 233 us for the one token.
+//   * Tiles go round the CTAs, so at any time neighbouring tiles are read.
+//   * Epilogue: one warp per 32 entries (its TMEM quadrant), a lane per entry,
+//     tokens along the registers; a transposing butterfly of 31 shuffles adds 32
+//     tokens' exponentials over the lanes and leaves token j to lane j.
+constexpr int FEW_THREADS = 256;  // warp 0 TMA, 1 MMA, 2 TMEM, 3 idle, 4..7 epilogue
+constexpr int FEW_TILE = 128;  // vocabulary entries
+
+template <int N>
+struct FewCfg {
+  static constexpr int W_STAGE = FEW_TILE * BK * 2;
+  static constexpr int STAGE = W_STAGE + N * BK * 2;
+  static constexpr int STAGES = 208 * 1024 / STAGE;  // 10, 8, 6 for N = 32, 64, 128
+  static constexpr int REF_BYTES = N * 8;
+  static constexpr int SMEM = STAGES * STAGE + REF_BYTES + 256 + 1024;
+  static constexpr int TMEM = 2 * N < 32 ? 32 : 2 * N;
+  static_assert(SMEM <= 232448 && (2 * STAGES + 5) * 8 + 4 <= 256, "shared memory");
+};
+
+struct FewParams {
+  int M, n, kblocks, tiles;
+  int* status;
+  int pol_w, pol_h;
+  EpiArgs e;
+};
+
+template <int N, bool STORE, bool SX>
+__global__ void __launch_bounds__(FEW_THREADS, 1)
+    few_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_h,
+               const __grid_constant__ FewParams p) {
+  using T = FewCfg<N>;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  float2* refs = reinterpret_cast<float2*>(smem + T::STAGES * T::STAGE);
+  uint64_t* full = reinterpret_cast<uint64_t*>(smem + T::STAGES * T::STAGE + T::REF_BYTES);
+  uint64_t* empty = full + T::STAGES;
+  uint64_t* tfull = empty + T::STAGES;
+  uint64_t* tempty = tfull + 2;
+  uint64_t* drain = tempty + 2;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drain + 1);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < T::STAGES; ++s) {
+      mbar_init(&full[s], 1);
+      mbar_init(&empty[s], 1);
+    }
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&tfull[i], 1);
+      mbar_init(&tempty[i], 4);
+    }
+    mbar_init(drain, 1);
+    fence_mbarrier_init();
+    tma_prefetch_desc(&map_w);
+    tma_prefetch_desc(&map_h);
+  }
+  if (warp == 2) {
+    tmem_alloc(tmem_slot, T::TMEM);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem_base = *tmem_slot;
+  pdl_trigger();
+
+  // this CTA's tiles: blockIdx.x, blockIdx.x + gridDim.x, ...
+  const int first = static_cast<int>(blockIdx.x), step = static_cast<int>(gridDim.x);
+  const int tiles = (p.tiles - first + step - 1) / step;
+  const int total = tiles * p.kblocks;  // stages over the CTA's life
+
+  if (warp == 0) {
+    // ---------------------------------------------------------- producer
+    const uint64_t pol_w = l2_policy(p.pol_w), pol_h = l2_policy(p.pol_h);
+    auto load_w = [&](int it) {  // stage it of the CTA: W's part
+      const int tile = it / p.kblocks, kb = it - tile * p.kblocks, st = it % T::STAGES;
+      mbar_arrive_expect_tx(&full[st], T::STAGE);
+      tma_load_2d_hint<1>(smem + st * T::STAGE, &map_w, smem_u32(&full[st]), kb * BK, (first + tile * step) * FEW_TILE,
+                          pol_w);
+    };
+    auto load_h = [&](int it) {
+      const int st = it % T::STAGES;
+      tma_load_2d_hint<1>(smem + st * T::STAGE + T::W_STAGE, &map_h, smem_u32(&full[st]), (it % p.kblocks) * BK, 0,
+                          pol_h);
+    };
+    // W is no product of the kernels before this one: the ring fills with it
+    // while they end
+    const int ahead = min(total, T::STAGES);
+    if (lane == 0)
+      for (int it = 0; it < ahead; ++it) load_w(it);
+    __syncwarp();
+    pdl_wait();
+    if (lane == 0)
+      for (int it = 0; it < ahead; ++it) load_h(it);
+    __syncwarp();
+    for (int it = ahead; it < total; ++it) {
+      if (!mbar_wait(&empty[it % T::STAGES], (it / T::STAGES - 1) & 1, p.status, DEV_TIMEOUT_PRODUCER)) break;
+      if (lane == 0) {
+        load_w(it);
+        load_h(it);
+      }
+      __syncwarp();
+    }
+  } else if (warp == 1) {
+    // --------------------------------------------------------------- MMA
+    constexpr uint32_t idesc = make_idesc_bf16_f32(128, N, false, false);
+    bool ok = true;
+    for (int tile = 0, it = 0; tile < tiles && ok; ++tile) {
+      const int acc = tile & 1;
+      if (!mbar_wait(&tempty[acc], ((tile >> 1) & 1) ^ 1, p.status, DEV_TIMEOUT_MMA)) break;
+      tc_fence_after();
+      for (int kb = 0; kb < p.kblocks; ++kb, ++it) {
+        const int st = it % T::STAGES;
+        if (!mbar_wait(&full[st], (it / T::STAGES) & 1, p.status, DEV_TIMEOUT_MMA)) {
+          ok = false;
+          break;
+        }
+        tc_fence_after();
+        if (lane == 0) {
+          const uint32_t a = smem_u32(smem + st * T::STAGE), b = a + T::W_STAGE;
+#pragma unroll
+          for (int k = 0; k < BK / 16; ++k)
+            umma_bf16(tmem_base + acc * N, make_smem_desc_sw128(a + k * 32, 16, 1024),
+                      make_smem_desc_sw128(b + k * 32, 16, 1024), idesc, kb > 0 || k > 0 ? 1u : 0u);
+          umma_commit(&empty[st]);
+        }
+        __syncwarp();
+      }
+      if (!ok) break;
+      if (lane == 0) umma_commit(&tfull[acc]);
+      __syncwarp();
+    }
+    if (lane == 0) umma_commit(drain);
+    __syncwarp();
+    mbar_wait(drain, 0, p.status, DEV_TIMEOUT_DRAIN);
+  } else if (warp >= 4) {
+    // ---------------------------------------------------------- epilogue
+    const int quad = warp & 3;
+    pdl_wait();
+    for (int j = threadIdx.x - 128; j < N; j += 128)
+      refs[j] = j < p.M ? p.e.ce_ref[j] : make_float2(0.f, __int_as_float(-1));
+    asm volatile("bar.sync 1, 128;" ::: "memory");
+    const float log2e = p.e.ce_log2e;
+    for (int tile = 0; tile < tiles; ++tile) {
+      const int acc = tile & 1;
+      if (!mbar_wait(&tfull[acc], (tile >> 1) & 1, p.status, DEV_TIMEOUT_EPILOGUE)) break;
+      tc_fence_after();
+      const int col0 = (first + tile * step) * FEW_TILE + quad * kCeFewPartCols;  // of this launch's columns
+      if (col0 < p.n) {
+        const int col = col0 + lane;
+        const bool in = col < p.n;
+        const int v = static_cast<int>(p.e.ce_v0) + col;
+#pragma unroll 1
+        for (int c = 0; c < N; c += 32) {
+          if (c >= p.M) break;
+          uint32_t r[32];
+          tmem_ld_32x32b_x32(tmem_base + (static_cast<uint32_t>(quad * 32) << 16) + acc * N + c, r);
+          tmem_ld_wait();
+          float e[32];
+#pragma unroll
+          for (int j = 0; j < 32; ++j) {
+            const float2 ref = refs[c + j];
+            const float x = fast_exp2(fmaf(__uint_as_float(r[j]), log2e, -ref.x));
+            e[j] = in && v != __float_as_int(ref.y) ? x : 0.f;
+          }
+#pragma unroll
+          for (int o = 16; o > 0; o >>= 1) {
+#pragma unroll
+            for (int k = 0; k < o; ++k) {
+              const float give = lane & o ? e[k] : e[k + o], keep = lane & o ? e[k + o] : e[k];
+              e[k] = keep + __shfl_xor_sync(0xffffffffu, give, o);
+            }
+          }
+          // lane j: token c + j
+          float d = e[0], ref2 = refs[c + lane].x;
+          const uint32_t far = __ballot_sync(0xffffffffu, c + lane < p.M && !(d >= kCeSumLow && d < kCeSumHigh));
+          if (far != 0) {
+            // against the part's own maximum, as in ce_epilogue
+#pragma unroll
+            for (int j = 0; j < 32; ++j) {
+              if (!(far >> j & 1)) continue;
+              const float x = __uint_as_float(r[j]);
+              const bool use = in && v != __float_as_int(refs[c + j].y);
+              float m = use ? x : -INFINITY;
+#pragma unroll
+              for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+              const float own = m * log2e > -INFINITY ? m * log2e : refs[c + j].x;
+              float s = use ? fast_exp2(fmaf(x, log2e, -own)) : 0.f;
+#pragma unroll
+              for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+              if (lane == j) {
+                d = s;
+                ref2 = own;
+              }
+            }
+          }
+          const long long ri = static_cast<long long>(c + lane) * p.e.ce_rec_ld + col0 / kCeFewPartCols;
+          if (c + lane < p.M) p.e.ce_rec[ri] = make_float2(d, ref2);
+          if constexpr (STORE) {
+            uint16_t* dst = static_cast<uint16_t*>(p.e.out16) + static_cast<long long>(c) * p.e.ld16 + col;
+#pragma unroll
+            for (int j = 0; j < 32; ++j) {
+              const float t = fmaf(__uint_as_float(r[j]), log2e, -__shfl_sync(0xffffffffu, ref2, j));
+              const float u = fmaf(fmaxf(t, kCeQLow), kCeQScale, 8388608.0f + kCeQBias);
+              if (c + j < p.M && in) dst[j * p.e.ld16] = static_cast<uint16_t>(__float_as_uint(u));
+            }
+          }
+          if constexpr (SX) {
+#pragma unroll
+            for (int j = 0; j < 32; ++j) e[j] = in ? __uint_as_float(r[j]) : 0.f;
+#pragma unroll
+            for (int o = 16; o > 0; o >>= 1) {
+#pragma unroll
+              for (int k = 0; k < o; ++k) {
+                const float give = lane & o ? e[k] : e[k + o], keep = lane & o ? e[k + o] : e[k];
+                e[k] = keep + __shfl_xor_sync(0xffffffffu, give, o);
+              }
+            }
+            if (c + lane < p.M) p.e.ce_sx[ri] = e[0];
+          }
+        }
+      }
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&tempty[acc]);
+    }
+  }
+  // warps without a wait of their own: this grid ends after the ones before it
+  pdl_wait();
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 2) {
+    tc_fence_after();
+    tmem_dealloc(tmem_base, T::TMEM);
+  }
+}
+
+template <int N, bool STORE, bool SX>
+cudaError_t few_t(const CUtensorMap& map_w, const CUtensorMap& map_h, const FewParams& fp, int num_sms,
+                  cudaStream_t stream) {
+  using T = FewCfg<N>;
+  auto kern = few_kernel<N, STORE, SX>;
+  static LaunchCache cache;
+  int dev = 0;
+  cudaGetDevice(&dev);
+  dev &= 63;
+  {
+    std::lock_guard<std::mutex> lock(cache.mu);
+    if (!(cache.attr_done & (1ull << dev))) {
+      cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, T::SMEM);
+      if (e != cudaSuccess) return e;
+      cache.attr_done |= 1ull << dev;
+    }
+  }
+  return launch_pdl(kern, dim3(static_cast<unsigned>(std::min(num_sms, fp.tiles))), dim3(FEW_THREADS), T::SMEM,
+                    stream, map_w, map_h, fp);
+}
+
+template <int N>
+cudaError_t few_n(const CUtensorMap& map_w, const CUtensorMap& map_h, const FewParams& fp, int num_sms,
+                  cudaStream_t stream) {
+  if (fp.e.out16) {
+    if (fp.e.ce_sx) return few_t<N, true, true>(map_w, map_h, fp, num_sms, stream);
+    return few_t<N, true, false>(map_w, map_h, fp, num_sms, stream);
+  }
+  if (fp.e.ce_sx) return few_t<N, false, true>(map_w, map_h, fp, num_sms, stream);
+  return few_t<N, false, false>(map_w, map_h, fp, num_sms, stream);
+}
+
 }  // namespace
+
+cudaError_t few_launch(const GemmDesc& d, int num_sms, cudaStream_t stream, const char** why) {
+  if (why) *why = nullptr;
+  if (!get_encode()) {
+    if (why) *why = "cuTensorMapEncodeTiled entry point unavailable";
+    return cudaErrorNotSupported;
+  }
+  const int n = static_cast<int>(few_rows(d.M));
+  CUtensorMap map_w, map_h;
+  if (d.M > kCeFewRows || !encode_map(&map_w, d.b[0], BK, FEW_TILE) || !encode_map(&map_h, d.a[0], BK, n)) {
+    if (why) *why = "few-row logits: more rows than the kernel takes, or operands that TMA cannot address";
+    return cudaErrorInvalidValue;
+  }
+  FewParams fp{};
+  fp.M = static_cast<int>(d.M);
+  fp.n = static_cast<int>(d.N);
+  fp.kblocks = static_cast<int>((d.k_seg[0] + BK - 1) / BK);
+  fp.tiles = static_cast<int>((d.N + FEW_TILE - 1) / FEW_TILE);
+  fp.status = d.status;
+  fp.pol_w = 0;
+  fp.pol_h = 2;
+  fp.e = d.args;
+  if (d.launches) *d.launches += 1;
+  if (n == 32) return few_n<32>(map_w, map_h, fp, num_sms, stream);
+  if (n == 64) return few_n<64>(map_w, map_h, fp, num_sms, stream);
+  return few_n<128>(map_w, map_h, fp, num_sms, stream);
+}
 
 cudaError_t gemm_launch(const GemmDesc& d, int num_sms, cudaStream_t stream, const char** why) {
   if (why) *why = nullptr;

@@ -88,7 +88,9 @@ struct EpiArgs {
   // StoreBf16, and the 16-bit piece that CeStats (optionally) and CeGrad write
   void* out16 = nullptr;
   long long ld16 = 0;
-  // CeStats, CeGrad: column c is vocabulary index ce_v0 + c
+  // CeStats, CeGrad: column c is vocabulary index ce_v0 + c; logits times
+  // ce_log2e are base-2 exponents
+  float ce_log2e = 0.0f;
   long long ce_v0 = 0;
   const float2* ce_ref = nullptr;    // CeStats: per row (reference logit * log2 e, label as int bits)
   float2* ce_rec = nullptr;          // CeStats: [rows][ce_rec_ld] records of the parts, from column 0 of this launch
@@ -119,6 +121,11 @@ struct GemmDesc {
   int spare_sms = 0;
 };
 
+// CeStats for at most kCeFewRows rows of d.a[0] (few_kernel; K-major operands).
+cudaError_t few_launch(const GemmDesc& d, int num_sms, cudaStream_t stream, const char** why);
+// The rows of d.a[0] that few_kernel reads for m tokens (a multiple of 32).
+constexpr long long few_rows(long long m) { return m <= 32 ? 32 : m <= 64 ? 64 : 128; }
+
 // Encodes the tensor maps and launches the persistent tcgen05 GEMM.
 // Returns cudaSuccess or the first error.
 cudaError_t gemm_launch(const GemmDesc& d, int num_sms, cudaStream_t stream, const char** why);
@@ -134,6 +141,17 @@ constexpr float kCeQLow = -64.0f;
 constexpr float kCeSumLow = 9.094947017729282e-13f;
 constexpr float kCeSumHigh = 4611686018427387904.0f;
 constexpr int kCePartCols = 64;  // columns of one epilogue warp
+// Up to this many tokens the logits come from few_kernel, whose parts have 32 columns.
+constexpr int kCeFewRows = 128;
+constexpr int kCeFewPartCols = 32;
+
+// The tensor cores' fp32 accumulator cuts where it adds, so a sum of k products
+// comes out smaller in magnitude, by k 2^-30 of itself on average (measured on
+// random operands: 3.8e-7, 8.2e-7, 1.77e-6 and 3.74e-6 for k = 512, 1024, 2048 and
+// 4096, nearly all of the error, where rounded fp32 sums have a mean error of
+// 1e-10). Unlike a rounding it does not average out over the vocabulary or the
+// tokens, so the cross entropy undoes it with the exponents' factor.
+inline float cut_factor(long long k) { return 1.0f + static_cast<float>(k) * 9.313225746154785e-10f; }
 
 struct CeArgs {
   const void* h = nullptr;  // bf16 [bt, hd]
@@ -152,7 +170,8 @@ struct CeArgs {
   float2* rec = nullptr;       // [bt][rec_ld]
   float* sx = nullptr;         // [bt][rec_ld], with label smoothing
   long long rec_ld = 0;
-  int n_parts = 0;
+  int n_parts = 0, part_shift = 0;  // parts of 1 << part_shift columns
+  float cut = 1.0f;             // what a logit of the tensor cores is multiplied by (see cut_factor)
   float4* row_const = nullptr;  // [bt]
   float* nll = nullptr;         // [bt]
   float* lse = nullptr;         // [bt], optional

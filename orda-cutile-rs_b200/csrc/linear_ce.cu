@@ -152,7 +152,7 @@ __device__ __forceinline__ RowResult row_result(const CeArgs& a, float2 ref, con
     l = static_cast<float>(static_cast<double>(m.r) * kLn2 + lg);
   }
   const float uni = a.alpha / static_cast<float>(a.v);
-  r.nll = a.alpha > 0.f ? (1.f - a.alpha) * gap + a.alpha * (l - sx / static_cast<float>(a.v)) : gap;
+  r.nll = a.alpha > 0.f ? (1.f - a.alpha) * gap + a.alpha * (l - sx * a.cut / static_cast<float>(a.v)) : gap;
   r.lse = l;
   r.c.x = -l * kLog2E;
   r.c.y = ref.y;
@@ -284,7 +284,7 @@ __global__ void __launch_bounds__(kRowThreads) ce_rows_kernel(const CeArgs a, ui
         // 2^(t + off) = 2^(t - 62.5) 2^(off + 62.5): the first factor is an exact
         // argument from u's bits (2^23 + u as a float, over 512, less the bias), and
         // flushes to zero for code 0, so the code needs no test of its own
-        const float up = ex2(rec[col / kCePartCols].y + (c.x + 62.5f));
+        const float up = ex2(rec[col >> a.part_shift].y + (c.x + 62.5f));
         uint32_t w[4] = {v[i].x, v[i].y, v[i].z, v[i].w};
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
