@@ -1751,7 +1751,7 @@ static bool grad_out_ok(const void* p, size_t ld, OrdaDType dt, size_t cols) {
 int orda_linear_cross_entropy_device(OrdaContext* ctx, const OrdaDeviceMat* hidden, const OrdaDeviceMat* weight,
                                      const int64_t* labels, size_t bt, const OrdaLinearCeOptions* opts,
                                      const OrdaLinearCeOutputs* out, void* stream, char* err, size_t err_len) {
-  if (!ctx || !hidden || !weight || !labels || !opts || !out) {
+  if (!ctx || !hidden || !weight || (bt > 0 && !labels) || !opts || !out) {
     set_error(err, err_len, "null argument");
     return ORDA_ERR_INVALID;
   }
@@ -1814,9 +1814,10 @@ static bool elem_mat_ok(const void* data, size_t rows, size_t cols, size_t ld, O
 
 // Sizes and scale of the two embedding entries.
 static int embedding_args_ok(size_t v, size_t h, size_t n, const int64_t* ids, float scale, char* err, size_t err_len) {
-  constexpr size_t kMax = size_t{1} << 30;  // positions and keys are 32-bit
-  if (v == 0 || h == 0 || v > kMax || h > kMax || n > kMax) {
-    set_error(err, err_len, "V and H must be in [1, 2^30] and n at most 2^30, got %zu, %zu and %zu", v, h, n);
+  constexpr size_t kMax = size_t{1} << 30;   // positions and keys are 32-bit
+  constexpr size_t kMaxH = size_t{1} << 20;  // column blocks are the grid's y
+  if (v == 0 || h == 0 || v > kMax || h > kMaxH || n > kMax) {
+    set_error(err, err_len, "V must be in [1, 2^30], H in [1, 2^20] and n at most 2^30, got %zu, %zu and %zu", v, h, n);
     return ORDA_ERR_INVALID;
   }
   if (n > 0 && !ids) {

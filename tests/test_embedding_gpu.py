@@ -243,6 +243,10 @@ def test_refusals(ctx):
         embedding_device(ctx, table, ids, scale=float("inf"))
     with pytest.raises(ValueError, match="rows of"):
         embedding_device(ctx, table, ids, out=torch.zeros(3, 8, device="cuda"))
+    with pytest.raises(ob.OrdaError, match="2\\^20"):
+        embedding_device(ctx, torch.zeros(1, 2**20 + 8, device="cuda", dtype=BF16), ids)
+    with pytest.raises(ob.OrdaError, match="ld >= H"):
+        embedding_grad_device(ctx, g, ids, 10, out=torch.zeros(1, 8, device="cuda").expand(10, 8))
     with pytest.raises(ValueError, match="accumulate"):
         embedding_grad_device(ctx, g, ids, 10, accumulate=True)
     with pytest.raises(ValueError, match="rows of"):
@@ -317,5 +321,62 @@ def test_shared_table_step(ctx):
     loss = torch.nn.functional.cross_entropy(z, labels)
     loss.backward()
     # x is rounded to bf16 (2^-8 of it, once) and so are the logit gradients: three such roundings, rms 1.6e-3 each
-    assert abs(float(loss) - float(r.loss)) <= 2.0**-8 * float(z.detach().abs().max())
+    assert abs(loss.item() - float(r.loss)) <= 2.0**-8 * float(z.detach().abs().max())
     assert ((r.grad_weight.double() - t.grad).norm() / t.grad.norm()) < 3 * 2.0**-8
+
+
+@pytest.mark.parametrize("n", [1, 2, 255, 256, 257, 511, 512, 513, 600])
+def test_few_tokens_and_the_sorted_path(ctx, n):
+    """Around the token count where the sort takes over; runs over several lookups of 256 ids."""
+    from orda_b200.device import embedding_grad_device
+
+    gen = rng(n)
+    for h, v in ((40, 3), (2056, 900)):
+        g = rand((n, h), BF16, gen)
+        for ids in (skewed(n, v, gen), torch.full((n,), v - 1, device="cuda"), torch.arange(n, device="cuda") % v):
+            got = embedding_grad_device(ctx, g, ids, v, scale=0.5, dtype=F32)
+            finish(ctx)
+            check_grad(got, *grad_formula(g, ids, v, 0.5))
+
+
+def test_offsets_beyond_32_bits(ctx):
+    """A table of 2.4e9 elements."""
+    from orda_b200.device import embedding_device, embedding_grad_device
+
+    gen = rng(9)
+    v, h = 590000, 4096
+    table = torch.zeros(v, h, device="cuda", dtype=BF16)
+    for n in (40, 700):
+        ids = torch.randint(v - 5000, v, (n,), generator=gen, device="cuda")
+        ids[::3] = torch.randint(0, 50, (len(ids[::3]),), generator=gen, device="cuda")
+        rows = rand((n, h), BF16, gen)
+        table[ids] = rows
+        assert torch.equal(embedding_device(ctx, table, ids), table[ids])
+        got = embedding_grad_device(ctx, rows, ids, v)
+        finish(ctx)
+        named, back = torch.unique(ids, return_inverse=True)
+        check_grad(got[named], *grad_formula(rows, back, len(named), 1.0))
+        got[named] = 0
+        assert not got.any()
+        del got
+
+
+def test_two_contexts_at_once(ctx):
+    from orda_b200.device import DeviceContext, embedding_grad_device
+
+    gen = rng(10)
+    with DeviceContext(0) as a, DeviceContext(0) as b:
+        work = []
+        for c, n, v in ((a, 9000, 4000), (b, 5000, 70000)):
+            g, ids = rand((n, 512), BF16, gen), skewed(n, v, gen)
+            work.append((c, g, ids, v, embedding_grad_device(c, g, ids, v)))
+        torch.cuda.synchronize()
+        streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+        outs = [[], []]
+        for _ in range(5):
+            for k, (c, g, ids, v, _) in enumerate(work):
+                with torch.cuda.stream(streams[k]):
+                    outs[k].append(embedding_grad_device(c, g, ids, v))
+        torch.cuda.synchronize()
+        for k in range(2):
+            assert all(torch.equal(o, work[k][4]) for o in outs[k])

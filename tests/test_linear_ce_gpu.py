@@ -357,3 +357,111 @@ def test_larger_products(ctx, bt, h, v, pull):
         for got, want in ((r.grad_hidden, f["dh"]), (r.grad_weight, f["dw"])):
             flushed = math.sqrt(want.numel()) * 2.0**-126
             assert (got.double() - want).norm() < 1.6e-3 * math.sqrt(3) * want.norm() + flushed
+
+
+@pytest.mark.parametrize("bt", [1, 31, 32, 33, 64, 65, 127, 128, 129])
+@pytest.mark.parametrize("a", [0.0, 0.1])
+def test_few_rows(ctx, bt, a):
+    """Around the row counts at which the logits' kernel changes, whole and in pieces."""
+    x, w, labels = make(bt, 200, 2531, seed=bt, ignored=0.2 if bt > 4 else 0.0)
+    f = formula(x, w, labels, a)
+    for piece in (0, bt * 1024 * 2):
+        check(call(ctx, x, w, labels, a, grad_dtype=torch.bfloat16, piece_bytes=piece), f)
+    check(call(ctx, x, w, labels, a, need_grad_hidden=False, need_grad_weight=False), f)
+
+
+def test_refusals(ctx):
+    import orda_b200 as ob
+    from orda_b200.device import linear_cross_entropy_device as f
+
+    x, w, labels = make(20, 64, 100)
+    for args, kw, what in [
+        ((x, w, labels), {"label_smoothing": 1.5}, "label_smoothing"),
+        ((x, w, labels), {"label_smoothing": float("nan")}, "label_smoothing"),
+        ((x, w, labels), {"reduction": 7}, "reduction"),
+        ((x, w, labels), {"global_non_ignore": -1}, "global_non_ignore"),
+        ((x, w, labels[:19].clone()), {}, "BT=20"),
+        ((x, w[:, :56], labels), {}, "weight must be"),
+        ((x[:0], w, labels[:0]), {}, "BT must be > 0"),
+        ((x.float(), w, labels), {}, "bf16"),
+        ((x, w[:, 1:57], labels), {}, "weight must be"),
+        ((x[:, 1:57], w[:, 1:57], labels), {}, "16-byte aligned"),
+        ((x[:1].expand(20, 64), w, labels), {}, "16-byte aligned"),
+        ((x, w, labels), {"out": {"grad_weight": torch.zeros(1, 64, device="cuda").expand(100, 64)}}, "ld >= H"),
+    ]:
+        with pytest.raises(ob.OrdaError, match=what):
+            f(ctx, *args, **kw)
+    for kw, what in [({"out": {"loss": torch.zeros(2, device="cuda")}}, "loss"),
+                     ({"out": {"nll": torch.zeros(20, device="cuda", dtype=torch.float64)}}, "nll"),
+                     ({"out": {"grad_hidden": torch.zeros(20, 65, device="cuda")}}, "grad_hidden"),
+                     ({"out": {"grad_hidden": torch.zeros(20, 64, device="cuda")}, "need_grad_hidden": False}, "need_"),
+                     ({"grad_dtype": torch.float16}, "dtype")]:
+        with pytest.raises(ValueError, match=what):
+            f(ctx, x, w, labels, **kw)
+    check(call(ctx, x, w, labels), formula(x, w, labels))
+
+
+def test_two_graphs_share_a_context(ctx):
+    from orda_b200.device import DeviceContext, linear_cross_entropy_device
+
+    cases = [make(100, 128, 2000, seed=31), make(300, 64, 5000, seed=32, ignored=0.3)]
+    with DeviceContext(0) as own:
+        want = [call(own, *c) for c in cases]
+        graphs, outs = [], []
+        for c in cases:
+            g = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(g):
+                outs.append(linear_cross_entropy_device(own, *c))
+            graphs.append(g)
+        for _ in range(3):
+            for g in graphs:
+                g.replay()
+        torch.cuda.synchronize()
+        for r, f in zip(outs, want):
+            for n in ("loss", "nll", "lse", "grad_hidden", "grad_weight"):
+                assert torch.equal(getattr(r, n), getattr(f, n)), n
+        del graphs
+
+
+def test_two_contexts_at_once(ctx):
+    from orda_b200.device import DeviceContext, linear_cross_entropy_device
+
+    cases = [make(200, 128, 9000, seed=41), make(40, 512, 20000, seed=42)]
+    with DeviceContext(0) as a, DeviceContext(0) as b:
+        want = [call(c, *case) for c, case in zip((a, b), cases)]
+        streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+        got = [[], []]
+        for _ in range(5):
+            for k, c in enumerate((a, b)):
+                with torch.cuda.stream(streams[k]):
+                    got[k].append(linear_cross_entropy_device(c, *cases[k]))
+        torch.cuda.synchronize()
+        for k in range(2):
+            for r in got[k]:
+                assert torch.equal(r.grad_weight, want[k].grad_weight) and float(r.loss) == float(want[k].loss)
+
+
+def test_offsets_beyond_32_bits(ctx):
+    """2.2e9 kept logits (4.5 GB), checked against 64 bits a thousand rows at a time."""
+    bt, h, v = 17000, 64, 131072
+    x, w, labels = make(bt, h, v, seed=51, ignored=0.1)
+    r = call(ctx, x, w, labels, grad_dtype=torch.bfloat16, piece_bytes=8 << 30)
+    live = labels != -100
+    n = int(live.sum())
+    wd = w.double()
+    dw = torch.zeros(v, h, dtype=torch.float64, device="cuda")
+    for rows in torch.arange(bt, device="cuda").split(1000):
+        xd = torch.where(live[rows, None], x[rows].double(), 0.0)
+        z = xd @ wd.T
+        lse = torch.logsumexp(z, 1)
+        y = torch.where(live[rows], labels[rows], 0)
+        nll = torch.where(live[rows], lse - z.gather(1, y[:, None])[:, 0], 0.0)
+        # logits of 64 products below 8 in magnitude: 2 H 2^-24 sum |h w| < 1e-4
+        assert (r.nll[rows].double() - nll).abs().max() < 1e-4
+        d = torch.exp(z - lse[:, None])
+        d[torch.arange(len(rows), device="cuda"), y] -= 1
+        d *= live[rows, None] / n
+        dw += d.T @ xd
+        dh = d @ wd
+        assert (r.grad_hidden[rows].double() - dh).norm() < 1.6e-3 * math.sqrt(3) * dh.norm()
+    assert (r.grad_weight.double() - dw).norm() < 1.6e-3 * math.sqrt(3) * dw.norm()
