@@ -493,10 +493,10 @@ __global__ void __launch_bounds__(256) grad_few_kernel(const EmbedGradArgs a) {
   const int i = blockIdx.x, n = static_cast<int>(a.n);
   const int tid = threadIdx.y * blockDim.x + threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int64_t id = a.ids[i];
-  if (a.has_padding && id == a.padding_id) return;
+  if (a.has_padding && id == a.padding_id) return pdl_wait();  // every exit: the grid ends after the clearing
   if (id < 0 || id >= a.v) {
     if (tid == 0) atomicExch(a.bad, DEV_ID_RANGE);
-    return;
+    return pdl_wait();
   }
   int count = 0;
   for (int j0 = 0; j0 < n; j0 += 256) {
@@ -513,7 +513,7 @@ __global__ void __launch_bounds__(256) grad_few_kernel(const EmbedGradArgs a) {
     }
     if (same) list[at + __popc(votes & ((1u << lane) - 1))] = j;
     __syncthreads();
-    if (count > 0 && list[0] < i) return;  // an earlier token's block does it
+    if (count > 0 && list[0] < i) return pdl_wait();  // an earlier token's block does it
   }
   const int each = (count + blockDim.y - 1) / blockDim.y;
   const int k0 = threadIdx.y * each, k1 = min(count, k0 + each);
@@ -538,13 +538,13 @@ __global__ void __launch_bounds__(256) grad_few_kernel(const EmbedGradArgs a) {
 #pragma unroll
     for (int j = 0; j < VEC; ++j) sum_s[tid * VEC + j] = s[j];
     __syncthreads();
-    if (threadIdx.y != 0) return;
+    if (threadIdx.y != 0) return pdl_wait();
     for (int y = 1; y < static_cast<int>(blockDim.y); ++y)
 #pragma unroll
       for (int j = 0; j < VEC; ++j) s[j] += sum_s[(y * blockDim.x + threadIdx.x) * VEC + j];
   }
-  if (c >= a.h) return;
   pdl_wait();  // the rows are cleared
+  if (c >= a.h) return;
   GradArgs o{};
   o.scale = a.scale;
   o.out = a.out;

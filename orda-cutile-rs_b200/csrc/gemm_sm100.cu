@@ -1330,6 +1330,7 @@ __global__ void __launch_bounds__(FEW_THREADS, 1)
     // --------------------------------------------------------------- MMA
     constexpr uint32_t idesc = make_idesc_bf16_f32(128, N, false, false);
     bool ok = true;
+    pdl_wait();  // the kernel before clears the status word that a wait gives up for
     for (int tile = 0, it = 0; tile < tiles && ok; ++tile) {
       const int acc = tile & 1;
       if (!mbar_wait(&tempty[acc], ((tile >> 1) & 1) ^ 1, p.status, DEV_TIMEOUT_MMA)) break;
