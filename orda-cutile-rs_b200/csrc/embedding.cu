@@ -262,6 +262,10 @@ __global__ void __cluster_dims__(kSortCtas, 1, 1) __launch_bounds__(THREADS, 1) 
         all += c;
       }
     }
+    // no CTA ends before its totals have been read; the last pass needs no more of
+    // the cluster, so that barrier runs while the pairs are placed
+    const bool last = pass + 1 == a.passes;
+    if (last) cluster_arrive();
     // inclusive scan over the digits: within warps, then the warps' sums
     auto warp_scan = [lane](uint32_t x) {
 #pragma unroll
@@ -295,7 +299,8 @@ __global__ void __cluster_dims__(kSortCtas, 1, 1) __launch_bounds__(THREADS, 1) 
       }
     }
     // the pairs are placed, and no CTA reads another's totals any more
-    cluster_sync();
+    if (last) cluster_wait();
+    else cluster_sync();
   }
   // the clearing kernel that runs beside this one is part of what comes before the next
   pdl_wait();
