@@ -460,7 +460,9 @@ ORDA_API int orda_vocab_backward_device(OrdaContext* ctx, const OrdaDeviceMat* s
  * The logits are never kept in fp32. A call with gradients holds 16-bit logits
  * (then logit gradients, in place) of a piece of the vocabulary, at most
  * piece_bytes for all rows; columns beyond the first piece are computed a
- * second time. A call without gradients keeps none.
+ * second time. A call without gradients keeps none. The rest of the workspace
+ * is 1/8 byte of statistics per logit (3/16 with smoothing; twice that up to
+ * 128 rows), a bf16 copy of hidden, and fp32 sums of grad_hidden.
  *
  * hidden [BT, H] and weight [V, H] as in orda_distillation_loss_device. The
  * products take bf16 operands: gradients carry the rounding of the logit
