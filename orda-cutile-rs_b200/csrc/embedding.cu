@@ -480,14 +480,15 @@ __global__ void __launch_bounds__(kRunX* kRunY) grad_runs_kernel(const GradArgs 
 }
 
 // ------------------------------------------------- the gradient, few tokens
-// Up to kFewTokens tokens need no sort: the block of a token looks through all
-// ids, leaves if an earlier token has the same one, and otherwise adds up the rows
-// of all that do, in order (split over threadIdx.y in contiguous parts that are
-// added in order). One launch after the clearing one, which it overlaps until it
-// writes, instead of three.
-// (500 x 1024 on top of fp32: 6.2 us, 14.5 us sorted; 1000 x 1024: 10.6 and 16.4 us,
-// but a run then may be 1024 rows long in one block.)
-constexpr int kFewTokens = 512;
+// Few tokens need no sort: the block of a token looks through all ids, leaves if
+// an earlier token has the same one, and otherwise adds up the rows of all that
+// do, in order (split over threadIdx.y in contiguous parts that are added in
+// order). One launch after the clearing one, which it overlaps until it writes,
+// instead of three. 500 x 1024 on top of fp32 take 6.2 us, 14.5 us sorted; 1000 x
+// 512 8.2 and 15.5 us; 2000 x 1000 16.4 and 18.3 us. But a run may be as long as
+// the call in one block, so wide rows, which leave no second threadIdx.y to
+// share it, stop at half as many tokens.
+constexpr int kFewTokens = 1024;
 constexpr int kFewBatch = 8;
 
 template <typename TI, typename TO, int VEC>
@@ -674,6 +675,11 @@ EmbedGradLayout grad_layout(const EmbedGradArgs& a) {
   return L;
 }
 
+// Which of the two gradients takes the call.
+bool few_tokens(const EmbedGradArgs& a, int vec) {
+  return a.n <= kFewTokens / 2 || (a.n <= kFewTokens && row_threads(a.h, vec, 1) <= 128);
+}
+
 }  // namespace
 
 void launch_embed(const EmbedArgs& a, cudaStream_t st) {
@@ -716,7 +722,10 @@ cudaError_t launch_sort(const SortArgs& s, bool beside_clear, cudaStream_t st) {
   return cudaGetLastError();
 }
 
-size_t embed_grad_workspace(const EmbedGradArgs& a) { return a.n <= kFewTokens ? 0 : grad_layout(a).total; }
+size_t embed_grad_workspace(const EmbedGradArgs& a) {
+  const EmbedGradLayout L = grad_layout(a);
+  return few_tokens(a, L.vec) ? 0 : L.total;
+}
 
 cudaError_t launch_embed_grad(const EmbedGradArgs& a, void* ws, int num_sms, cudaStream_t st, int* launches) {
   if (a.n == 0 && a.accumulate) return cudaSuccess;
@@ -730,14 +739,13 @@ cudaError_t launch_embed_grad(const EmbedGradArgs& a, void* ws, int num_sms, cud
     const cudaError_t e = cudaGetLastError();
     if (e != cudaSuccess || a.n == 0) return e;
   }
-  if (a.n <= kFewTokens) {
+  const EmbedGradLayout L = grad_layout(a);
+  if (few_tokens(a, L.vec)) {
     cudaError_t e = cudaSuccess;
-    const int vec = pick_vec(a.h, a.g, a.ldg, a.in_bf16 ? 2 : 4, a.out, a.ldo, es_out);
-    by_types(a.in_bf16, a.out_bf16, vec, FewCall{a, !a.accumulate, st, &e});
+    by_types(a.in_bf16, a.out_bf16, L.vec, FewCall{a, !a.accumulate, st, &e});
     *launches += 1;
     return e;
   }
-  const EmbedGradLayout L = grad_layout(a);
   uint8_t* w = static_cast<uint8_t*>(ws);
   SortArgs s{};
   s.ids = a.ids;

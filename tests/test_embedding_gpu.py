@@ -325,7 +325,7 @@ def test_shared_table_step(ctx):
     assert ((r.grad_weight.double() - t.grad).norm() / t.grad.norm()) < 3 * 2.0**-8
 
 
-@pytest.mark.parametrize("n", [1, 2, 255, 256, 257, 511, 512, 513, 600])
+@pytest.mark.parametrize("n", [1, 2, 255, 256, 257, 511, 512, 513, 600, 1023, 1024, 1025])
 def test_few_tokens_and_the_sorted_path(ctx, n):
     """Around the token count where the sort takes over; runs over several lookups of 256 ids."""
     from orda_b200.device import embedding_grad_device
