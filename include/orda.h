@@ -453,7 +453,9 @@ ORDA_API int orda_vocab_backward_device(OrdaContext* ctx, const OrdaDeviceMat* s
  *   loss = sum nll (SUM), or divided by the count of live tokens, at least 1 (MEAN)
  * and the gradients of the loss with respect to hidden and weight. A token
  * whose label is ignore_index is not live: its nll, lse and grad_hidden row
- * are 0 and what its hidden row holds is not used. The student term of
+ * are 0 and what its hidden row holds is not used. A live row whose logits all
+ * lie below -2.36e38 gives NaN; single ones there (masked entries, the label
+ * among them) do not. The student term of
  * `distillation_loss` (src/reference/cross_entropy.rs:20-74) on its own; the
  * reference has no entry without a teacher.
  *

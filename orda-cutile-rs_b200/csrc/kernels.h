@@ -173,7 +173,7 @@ struct CeArgs {
   int n_parts = 0, part_shift = 0;  // parts of 1 << part_shift columns
   float cut = 1.0f;             // what a logit of the tensor cores is multiplied by (see cut_factor)
   float4* row_const = nullptr;  // [bt]
-  float* nll = nullptr;         // [bt]
+  float* nll = nullptr;         // [bt]; the label's logit between the first kernel and the loss
   float* lse = nullptr;         // [bt], optional
   float* loss = nullptr;        // [1]
   float* scale = nullptr;       // [1] what the gradients are multiplied by after the products

@@ -10,7 +10,10 @@
 // The label's logit is the reference of its row: the logits product sums
 // Z_o = sum_{v != y} e^{z_v - z_y} per 64-column part, so that
 //   lse - z_y = log(1 + Z_o),  1 - p_y = Z_o / (1 + Z_o)
-// lose nothing to cancellation when the label's probability nears 1.
+// lose nothing to cancellation when the label's probability nears 1. A label's
+// logit below -2.36e38 (a masked entry), whose base-2 exponent fp32 does not hold,
+// is held as -FLT_MAX: an infinite reference would turn the parts that keep it
+// into NaN. The loss of such a row comes from the logit itself.
 //
 // Between the logits product and the two gradient products the logits of a
 // piece are kept as 16-bit fixed point, t = log2 e^{z - z_y} in steps of
@@ -24,6 +27,7 @@
 #include <cuda_runtime.h>
 
 #include <algorithm>
+#include <cfloat>
 #include <cstdint>
 
 #include "kernels.h"
@@ -103,7 +107,9 @@ __global__ void __launch_bounds__(kPrepThreads) ce_prep_kernel(const CeArgs a) {
     float x = 0.f;
 #pragma unroll
     for (int k = 0; k < kPrepThreads / 32; ++k) x += part[k];
-    a.ref[row] = make_float2(live ? x * kLog2E : 0.f, __int_as_float(live ? static_cast<int>(y) : -1));
+    const float x2 = x * kLog2E;
+    a.ref[row] = make_float2(!live ? 0.f : x2 < -FLT_MAX ? -FLT_MAX : x2, __int_as_float(live ? static_cast<int>(y) : -1));
+    a.nll[row] = x;
     if (live) atomicAdd(a.count, 1);
   }
 }
@@ -135,10 +141,13 @@ struct RowResult {
   float nll, lse;
 };
 
-__device__ __forceinline__ RowResult row_result(const CeArgs& a, float2 ref, const Acc& m, float sx) {
+__device__ __forceinline__ RowResult row_result(const CeArgs& a, float2 ref, float zy, const Acc& m, float sx) {
   RowResult r;
   float gap, miss, l;  // lse - z_y, 1 - p_y and lse
-  if (m.r == ref.x) {
+  if (m.r == ref.x && ref.x <= -FLT_MAX) {
+    // every logit lies below -2.36e38: the exponents do not hold their differences
+    gap = miss = l = NAN;
+  } else if (m.r == ref.x) {
     const float z = static_cast<float>(m.d);
     gap = log1pf(z);
     miss = z < INFINITY ? z / (1.f + z) : 1.f;
@@ -147,9 +156,10 @@ __device__ __forceinline__ RowResult row_result(const CeArgs& a, float2 ref, con
     const double up = static_cast<double>(m.r) - static_cast<double>(ref.x);
     const double own = exp2(-up);  // the label's term next to m.d
     const double lg = log(m.d + own);
-    gap = static_cast<float>(up * kLn2 + lg);
+    const double lse = static_cast<double>(m.r) * kLn2 + lg;
+    gap = static_cast<float>(ref.x > -FLT_MAX ? up * kLn2 + lg : lse - static_cast<double>(zy));
     miss = static_cast<float>(m.d / (m.d + own));
-    l = static_cast<float>(static_cast<double>(m.r) * kLn2 + lg);
+    l = static_cast<float>(lse);
   }
   const float uni = a.alpha / static_cast<float>(a.v);
   r.nll = a.alpha > 0.f ? (1.f - a.alpha) * gap + a.alpha * (l - sx * a.cut / static_cast<float>(a.v)) : gap;
@@ -258,7 +268,8 @@ __global__ void __launch_bounds__(kRowThreads) ce_rows_kernel(const CeArgs a, ui
         x += x_s[w];
       }
       if (mixed) m = acc_s[0];
-      r = row_result(a, ref, m, static_cast<float>(x));
+      // a.nll holds the label's logit until seg 0 replaces it; only that block's loss is used
+      r = row_result(a, ref, seg == 0 ? a.nll[row] : 0.f, m, static_cast<float>(x));
     }
     const_s = r.c;
     if (seg == 0) {

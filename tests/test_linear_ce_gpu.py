@@ -465,3 +465,53 @@ def test_offsets_beyond_32_bits(ctx):
         dh = d @ wd
         assert (r.grad_hidden[rows].double() - dh).norm() < 1.6e-3 * math.sqrt(3) * dh.norm()
     assert (r.grad_weight.double() - dw).norm() < 1.6e-3 * math.sqrt(3) * dw.norm()
+
+
+@pytest.mark.parametrize("bt", [64, 300])
+@pytest.mark.parametrize("piece_bytes", [0, 1])
+def test_label_at_the_lowest_value(ctx, bt, piece_bytes):
+    """Labels on vocabulary entries that a large negative logit masks: z log2 e leaves fp32, the other entries'
+    softmax does not."""
+    x, w, labels = make(bt, 64, 640, seed=6)
+    x[:, 0] = 1.0
+    w[:, 0] = 0.0
+    w[128:384, 0] = -3.0e38
+    labels = torch.where((labels >= 128) & (labels < 384), 5, labels)
+    labels[::3] = 200
+    r = call(ctx, x, w, labels, mean=False, piece_bytes=piece_bytes)
+    keep = torch.cat([torch.arange(128), torch.arange(384, 640)]).cuda()
+    z = x.double() @ w[keep].double().T
+    lse = torch.logsumexp(z, 1)
+    f = formula(x, w[keep].contiguous(), torch.zeros(bt, dtype=torch.int64, device="cuda"))
+    assert torch.all((r.lse.double() - lse).abs() <= f["row_tol"])
+    masked = torch.zeros(bt, dtype=torch.bool, device="cuda")
+    masked[::3] = True
+    zy = (x.double() * w.double()[labels]).sum(1)
+    # 2^-22 of a loss of 3e38: the products' sum and the difference to lse
+    tol = f["row_tol"] + 2.0**-22 * zy.abs()
+    assert torch.all((r.nll.double() - (lse - zy)).abs() <= tol)
+    # the gradients: p over the entries that are left, -1 at the label
+    p = torch.zeros(bt, 640, dtype=torch.float64, device="cuda")
+    p[:, keep] = torch.exp(z - lse[:, None])
+    p[torch.arange(bt, device="cuda"), labels] -= 1
+    dw = p.T @ x.double()
+    assert torch.isfinite(r.grad_hidden).all() and torch.isfinite(r.grad_weight).all()
+    assert (r.grad_weight.double() - dw).norm() < 5e-3 * dw.norm()
+    others = ~masked
+    dh = p[others][:, keep] @ w[keep].double()
+    assert (r.grad_hidden[others].double() - dh).norm() < 5e-3 * dh.norm()
+
+
+@pytest.mark.parametrize("bt", [64, 300])
+def test_a_row_of_lowest_values_only_shows(ctx, bt):
+    x, w, labels = make(bt, 64, 640, seed=6)
+    x[:, 0] = 0.0
+    x[5, 0] = 1.0
+    f = formula(x, w, labels)
+    w[:, 0] = -3.0e38
+    r = call(ctx, x, w, labels, need_grad_hidden=False, need_grad_weight=False)
+    rest = torch.arange(bt, device="cuda") != 5
+    assert torch.isnan(r.nll[5]) and torch.isnan(r.lse[5])
+    g = formula(x[rest], w, labels[rest])
+    tol = f["row_tol"][rest] + 2.0**-23 * g["nll"].abs()
+    assert torch.all((r.nll[rest].double() - g["nll"]).abs() <= tol)
