@@ -1078,7 +1078,6 @@ int run_linear_ce(OrdaContext* ctx, const OrdaDeviceMat& hm, const OrdaDeviceMat
   a.n_parts = static_cast<int>(L.n_parts);
   a.part_shift = L.few ? 5 : 6;
   static_assert(kCeFewPartCols == 1 << 5 && kCePartCols == 1 << 6, "part_shift");
-  a.cut = cut_factor(a.hd);
   a.row_const = reinterpret_cast<float4*>(ws + L.row_const);
   a.nll = out.nll ? out.nll : reinterpret_cast<float*>(ws + L.nll);
   a.lse = out.lse;
@@ -1114,7 +1113,6 @@ int run_linear_ce(OrdaContext* ctx, const OrdaDeviceMat& hm, const OrdaDeviceMat
     gd.args.out16 = keep;
     gd.args.ld16 = static_cast<long long>(L.ld_piece);
     gd.args.ce_v0 = static_cast<long long>(v0);
-    gd.args.ce_log2e = static_cast<float>(1.4426950408889634 * (1.0 + static_cast<double>(h) * 0x1p-30));
     gd.args.ce_ref = a.ref;
     gd.args.ce_rec = a.rec + (v0 >> a.part_shift);
     gd.args.ce_sx = smooth ? a.sx + (v0 >> a.part_shift) : nullptr;

@@ -343,12 +343,30 @@ constexpr int kEpiStoreBf16 = 32;
 constexpr int kEpiStoreSlab = 33;
 constexpr int kEpiCeStats = 64;  // + 1: keep the 16-bit logits, + 2: sums of the logits
 constexpr int kEpiCeGrad = 68;
+constexpr int kEpiCeParts = 72;  // CeStats (+ 1, + 2 as there) of K loops longer than kCeKBlocks
+
+// The tensor cores' accumulator cuts what does not fit fp32 at every addition,
+// so a sum of k products comes out too small by k 2^-30 of itself on random
+// operands (measured: 3.8e-7, 8.2e-7, 1.77e-6 and 3.74e-6 for k = 512, 1024, 2048 and
+// 4096; rounded fp32 sums have a mean error of 1e-10), and that does not average
+// out over the vocabulary. The cross entropy's logits therefore sum K in even
+// parts of at most 2048, each from zero, and the epilogue adds the parts in fp32.
+// Losses at H = 4096 against 64 bits: 5e-7 (1e-6 in one part, 2.5e-7 in parts of
+// 1024; fp32 torch 6e-7). Each further part costs the products' time: 2048 x 4096
+// x 32000 without gradients 362 us in one part, 377 in two, 388 in four.
+constexpr int kCeKBlocks = 2048 / BK;
+__host__ __device__ constexpr int ce_k_parts(int kblocks) { return (kblocks + kCeKBlocks - 1) / kCeKBlocks; }
+// First K block of part i.
+__host__ __device__ constexpr int ce_k_begin(int kblocks, int parts, int i) {
+  return static_cast<int>(static_cast<long long>(kblocks) * i / parts);
+}
 
 // Epilogue warps. The 16-bit epilogues of the linear cross entropy take 16
 // (four per scheduler): one warp's chain of TMEM load, exponentials, staging
 // and proxy fence leaves its scheduler idle most of the time (two warps each
 // issued in 31 % of the cycles at H = 64), and with a short K loop the epilogue
 // is the tile's time.
+constexpr bool epi_parts(int epi) { return epi >= kEpiCeParts; }
 constexpr int epi_warps(int epi) { return epi == kEpiStoreBf16 || epi >= kEpiCeStats ? 16 : 8; }
 constexpr int epi_threads(int epi) { return NUM_THREADS - 256 + 32 * epi_warps(epi); }
 
@@ -358,23 +376,34 @@ __device__ __forceinline__ uint32_t pack_bf16x2(float a, float b) {
   return *reinterpret_cast<const uint32_t*>(&h);
 }
 
-// Stages this row's 32 16-bit values (16 packed words) and sends the warp's
-// 32 x 32 block (64-byte rows, 64-byte swizzle) out in one TMA store, clipped
-// at the tensor bounds.
-__device__ __forceinline__ void stage16(uint8_t* buf, int lane, const uint32_t (&w)[16], const CUtensorMap* map, int x,
-                                        int y, bool store, uint64_t policy) {
+// The steps of stage16: the staging block is free, 8 values (k of 4) of this row, the store.
+__device__ __forceinline__ void stage16_begin(int lane) {
   if (lane == 0) bulk_wait_read_all();
   __syncwarp();
-#pragma unroll
-  for (int k = 0; k < 4; ++k)
-    *reinterpret_cast<uint4*>(buf + lane * 64 + ((k ^ ((lane >> 1) & 3)) << 4)) =
-        make_uint4(w[4 * k], w[4 * k + 1], w[4 * k + 2], w[4 * k + 3]);
+}
+__device__ __forceinline__ void stage16_put(uint8_t* buf, int lane, int k, uint4 w) {
+  *reinterpret_cast<uint4*>(buf + lane * 64 + ((k ^ ((lane >> 1) & 3)) << 4)) = w;
+}
+__device__ __forceinline__ void stage16_send(uint8_t* buf, int lane, const CUtensorMap* map, int x, int y, bool store,
+                                             uint64_t policy) {
   fence_proxy_async_smem();
   __syncwarp();
   if (lane == 0 && store) {
     tma_store_2d_hint(map, buf, x, y, policy);
     bulk_commit();
   }
+}
+
+// Stages this row's 32 16-bit values (16 packed words) and sends the warp's
+// 32 x 32 block (64-byte rows, 64-byte swizzle) out in one TMA store, clipped
+// at the tensor bounds.
+__device__ __forceinline__ void stage16(uint8_t* buf, int lane, const uint32_t (&w)[16], const CUtensorMap* map, int x,
+                                        int y, bool store, uint64_t policy) {
+  stage16_begin(lane);
+#pragma unroll
+  for (int k = 0; k < 4; ++k)
+    stage16_put(buf, lane, k, make_uint4(w[4 * k], w[4 * k + 1], w[4 * k + 2], w[4 * k + 3]));
+  stage16_send(buf, lane, map, x, y, store, policy);
 }
 
 // One 32-column chunk of one row of the linear cross entropy's first pass:
@@ -384,23 +413,27 @@ __device__ __forceinline__ void stage16(uint8_t* buf, int lane, const uint32_t (
 // mantissa of t * 512 + (2^23 + 2^15): one FMA and half a byte permute per
 // element, where a conversion instruction would share the SFU's pipe with ex2.
 template <bool MASK, bool STORE, bool SX>
-__device__ __forceinline__ void ce_stats_chunk(const uint32_t (&r)[32], float log2e, float ref2, int lab, int nvalid, float& d,
-                                               float& sx, uint32_t (&q)[16]) {
+__device__ __forceinline__ void ce_stats_column(float x, int j, float ref2, int lab, int nvalid, float& a, float& ax,
+                                                uint32_t& q) {
+  const float t = fmaf(x, LOG2E, -ref2);
+  float e = fast_exp2(t);
+  if (MASK) e = (j < nvalid && j != lab) ? e : 0.0f;
+  a += e;
+  if (SX) ax += (!MASK || j < nvalid) ? x : 0.0f;
+  if (STORE) {
+    const uint32_t u = __float_as_uint(fmaf(fmaxf(t, kCeQLow), kCeQScale, 8388608.0f + kCeQBias));
+    if (j & 1) q = __byte_perm(q, u, 0x5410);
+    else q = u;
+  }
+}
+
+template <bool MASK, bool STORE, bool SX>
+__device__ __forceinline__ void ce_stats_chunk(const uint32_t (&r)[32], float ref2, int lab, int nvalid, float& d, float& sx,
+                                               uint32_t (&q)[16]) {
   float a[4] = {0.f, 0.f, 0.f, 0.f}, ax[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-  for (int j = 0; j < 32; ++j) {
-    const float x = __uint_as_float(r[j]);
-    const float t = fmaf(x, log2e, -ref2);
-    float e = fast_exp2(t);
-    if (MASK) e = (j < nvalid && j != lab) ? e : 0.0f;
-    a[j & 3] += e;
-    if (SX) ax[j & 3] += (!MASK || j < nvalid) ? x : 0.0f;
-    if (STORE) {
-      const uint32_t u = __float_as_uint(fmaf(fmaxf(t, kCeQLow), kCeQScale, 8388608.0f + kCeQBias));
-      if (j & 1) q[j >> 1] = __byte_perm(q[j >> 1], u, 0x5410);
-      else q[j >> 1] = u;
-    }
-  }
+  for (int j = 0; j < 32; ++j)
+    ce_stats_column<MASK, STORE, SX>(__uint_as_float(r[j]), j, ref2, lab, nvalid, a[j & 3], ax[j & 3], q[j >> 1]);
   d += (a[0] + a[1]) + (a[2] + a[3]);
   if (SX) sx += (ax[0] + ax[1]) + (ax[2] + ax[3]);
 }
@@ -435,8 +468,8 @@ __device__ __forceinline__ void ce_epilogue(const KParams& p, const CUtensorMap*
     if constexpr (GRAD) {
 #pragma unroll
       for (int j = 0; j < 16; ++j) {
-        float v0 = fast_exp2(fmaf(__uint_as_float(r[2 * j]), p.e.ce_log2e, row_c.x)) - row_c.z;
-        float v1 = fast_exp2(fmaf(__uint_as_float(r[2 * j + 1]), p.e.ce_log2e, row_c.x)) - row_c.z;
+        float v0 = fast_exp2(fmaf(__uint_as_float(r[2 * j]), LOG2E, row_c.x)) - row_c.z;
+        float v1 = fast_exp2(fmaf(__uint_as_float(r[2 * j + 1]), LOG2E, row_c.x)) - row_c.z;
         if (has_label) {
           if (lc == 2 * j) v0 = row_c.w;
           if (lc == 2 * j + 1) v1 = row_c.w;
@@ -444,9 +477,9 @@ __device__ __forceinline__ void ce_epilogue(const KParams& p, const CUtensorMap*
         q[j] = pack_bf16x2(v0, v1);
       }
     } else if (has_label || nvalid < 32) {
-      ce_stats_chunk<true, STORE, SX>(r, p.e.ce_log2e, ref2, lc, nvalid, d, sx, q);
+      ce_stats_chunk<true, STORE, SX>(r, ref2, lc, nvalid, d, sx, q);
     } else {
-      ce_stats_chunk<false, STORE, SX>(r, p.e.ce_log2e, ref2, lc, 32, d, sx, q);
+      ce_stats_chunk<false, STORE, SX>(r, ref2, lc, 32, d, sx, q);
     }
     if constexpr (STORE) {
       const int x = colh + c * 32;
@@ -479,7 +512,7 @@ __device__ __forceinline__ void ce_epilogue(const KParams& p, const CUtensorMap*
       }
       __syncwarp();
       // a part of nothing, or of logits near the type's lowest value, keeps the row's reference
-      if (out_of_range && m * p.e.ce_log2e > -INFINITY) ref2 = m * p.e.ce_log2e;
+      if (out_of_range && m * LOG2E > -INFINITY) ref2 = m * LOG2E;
       d = 0.f;
       sx = 0.f;
       // the first stores of this part are complete before it is written again
@@ -501,6 +534,76 @@ __device__ __forceinline__ void ce_epilogue(const KParams& p, const CUtensorMap*
   }
 }
 
+// CeStats where the logits are in registers (x, complete sums of the K parts):
+// the same records and stores, without another look at TMEM.
+template <int EPI>
+__device__ __forceinline__ void ce_parts_epilogue(const KParams& p, const CUtensorMap* map, uint8_t* buf, int lane,
+                                                  const uint32_t (&x)[2][32], int colh, int row0, long long grow,
+                                                  bool row_ok, int part, const float4& row_c, uint64_t pol_c) {
+  constexpr bool STORE = (EPI & 1) != 0, SX = (EPI & 2) != 0;
+  if (colh >= p.N) return;
+  const long long lab_rel = static_cast<long long>(__float_as_int(row_c.y)) - p.e.ce_v0 - colh;
+  const int lab = lab_rel >= 0 && lab_rel < kCePartCols ? static_cast<int>(lab_rel) : -1;
+  float d = 0.f, sx = 0.f;
+  float ref2 = row_c.x;
+#pragma unroll 1
+  for (int again = 0; again < 2; ++again) {
+#pragma unroll
+    for (int c = 0; c < 2; ++c) {
+      const int nvalid = p.N - (colh + c * 32);
+      const int lc = lab - c * 32;
+      float a[4] = {0.f, 0.f, 0.f, 0.f}, ax[4] = {0.f, 0.f, 0.f, 0.f};
+      if constexpr (STORE) stage16_begin(lane);
+      // eight columns' codes at a time: x leaves few registers
+      const bool mask = __any_sync(0xffffffffu, lc >= 0 && lc < 32) || nvalid < 32;
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        uint32_t q[4];
+        if (mask) {
+#pragma unroll
+          for (int j = 8 * k; j < 8 * k + 8; ++j)
+            ce_stats_column<true, STORE, SX>(__uint_as_float(x[c][j]), j, ref2, lc, nvalid, a[j & 3], ax[j & 3],
+                                             q[(j >> 1) & 3]);
+        } else {
+#pragma unroll
+          for (int j = 8 * k; j < 8 * k + 8; ++j)
+            ce_stats_column<false, STORE, SX>(__uint_as_float(x[c][j]), j, ref2, lc, 32, a[j & 3], ax[j & 3],
+                                              q[(j >> 1) & 3]);
+        }
+        if constexpr (STORE) stage16_put(buf, lane, k, make_uint4(q[0], q[1], q[2], q[3]));
+      }
+      d += (a[0] + a[1]) + (a[2] + a[3]);
+      if (SX) sx += (ax[0] + ax[1]) + (ax[2] + ax[3]);
+      if constexpr (STORE) {
+        const int col = colh + c * 32;
+        stage16_send(buf, lane, map, col, row0, row0 < p.M && col < p.N, pol_c);
+      }
+    }
+    const bool out_of_range = !(d >= kCeSumLow && d < kCeSumHigh);
+    if (again == 1 || !__any_sync(0xffffffffu, out_of_range)) break;
+    // against the part's own maximum, as in ce_epilogue
+    float m = -INFINITY;
+#pragma unroll
+    for (int c = 0; c < 2; ++c) {
+      const int nvalid = p.N - (colh + c * 32);
+#pragma unroll
+      for (int j = 0; j < 32; ++j)
+        if (j < nvalid && j != lab - c * 32) m = fmaxf(m, __uint_as_float(x[c][j]));
+    }
+    __syncwarp();
+    if (out_of_range && m * LOG2E > -INFINITY) ref2 = m * LOG2E;
+    d = 0.f;
+    sx = 0.f;
+    if (STORE && lane == 0) bulk_wait_all();
+    __syncwarp();
+  }
+  if (row_ok) {
+    const long long ri = grow * p.e.ce_rec_ld + part;
+    p.e.ce_rec[ri] = make_float2(d, ref2);
+    if (SX) p.e.ce_sx[ri] = sx;
+  }
+}
+
 // ------------------------------------------------------------------ kernel
 
 template <int CG, bool A_MN, bool B_MN, int EPI, bool WIDE>
@@ -514,6 +617,9 @@ __global__ void __launch_bounds__(epi_threads(EPI), 1)
   constexpr bool PAIR = CG == 2;
   constexpr int EW = epi_warps(EPI);
   constexpr int SLICE = T::TILE_N / (EW / 4);  // tile columns of one epilogue warp
+  // K parts: a tile takes an accumulator for each part in turn
+  constexpr bool PARTS = epi_parts(EPI);
+  const int k_parts = PARTS ? ce_k_parts(p.seg_kblocks[0]) : 1;
   extern __shared__ uint8_t smem_raw[];
   // Same static layout in both CTAs of a pair: the MMA reads the peer's
   // operands at the leader's offsets.
@@ -636,59 +742,61 @@ __global__ void __launch_bounds__(epi_threads(EPI), 1)
     for (int w = unit; w < p.num_items && ok; w += nunits) {
       int kb0, kb1;
       work_item(p, w, kb0, kb1);
-      if (!mbar_wait<PAIR>(&tempty[acc], acc_phase ^ 1, p.status, DEV_TIMEOUT_MMA)) {
-        ok = false;
-        break;
-      }
-      tc_fence_after();
-      const uint32_t d_tmem = tmem_base + static_cast<uint32_t>(acc * BN);
-      bool first = true;
-      for (int seg = 0; seg < p.nseg && ok; ++seg) {
-        const int k_end = kb1 < 0 ? p.seg_kblocks[seg] : kb1;
-        for (int kb = kb1 < 0 ? 0 : kb0; kb < k_end; ++kb) {
-          if (!mbar_wait<PAIR>(&full[stage], phase, p.status, DEV_TIMEOUT_MMA)) {
-            ok = false;
-            break;
-          }
-          tc_fence_after();
-          if (lane == 0) {
-            const uint32_t a_base = smem_u32(sA + stage * T::A_STAGE);
-            const uint32_t b_base = smem_u32(sB + stage * T::B_STAGE);
-#pragma unroll
-            for (int k = 0; k < BK / 16; ++k) {
-              uint64_t ad;
-              if (!A_MN) ad = make_smem_desc_sw128(a_base + k * 32, 16, 1024);
-              else ad = make_smem_desc_sw128(a_base + k * 2048, BK * 128, 1024);
-#pragma unroll
-              for (int q = 0; q < T::NW; ++q) {
-                const uint32_t bq = b_base + q * T::B_PART_BYTES;
-                uint64_t bd;
-                if (!B_MN) bd = make_smem_desc_sw128(bq + k * 32, 16, 1024);
-                else bd = make_smem_desc_sw128(bq + k * 2048, BK * 128, 1024);
-                umma_bf16_cg<CG>(d_tmem + q * BN, ad, bd, idesc, (first && k == 0) ? 0u : 1u);
-              }
+      for (int kp = 0; kp < k_parts && ok; ++kp) {
+        if (!mbar_wait<PAIR>(&tempty[acc], acc_phase ^ 1, p.status, DEV_TIMEOUT_MMA)) {
+          ok = false;
+          break;
+        }
+        tc_fence_after();
+        const uint32_t d_tmem = tmem_base + static_cast<uint32_t>(acc * BN);
+        bool first = true;
+        for (int seg = 0; seg < p.nseg && ok; ++seg) {
+          const int k_end = PARTS ? ce_k_begin(p.seg_kblocks[0], k_parts, kp + 1) : kb1 < 0 ? p.seg_kblocks[seg] : kb1;
+          for (int kb = PARTS ? ce_k_begin(p.seg_kblocks[0], k_parts, kp) : kb1 < 0 ? 0 : kb0; kb < k_end; ++kb) {
+            if (!mbar_wait<PAIR>(&full[stage], phase, p.status, DEV_TIMEOUT_MMA)) {
+              ok = false;
+              break;
             }
-            // frees this stage in both CTAs once the MMAs have read it
-            if constexpr (PAIR) umma_commit_pair(&empty[stage], 0x3);
-            else umma_commit(&empty[stage]);
-          }
-          __syncwarp();
-          first = false;
-          if (++stage == T::STAGES) {
-            stage = 0;
-            phase ^= 1;
+            tc_fence_after();
+            if (lane == 0) {
+              const uint32_t a_base = smem_u32(sA + stage * T::A_STAGE);
+              const uint32_t b_base = smem_u32(sB + stage * T::B_STAGE);
+#pragma unroll
+              for (int k = 0; k < BK / 16; ++k) {
+                uint64_t ad;
+                if (!A_MN) ad = make_smem_desc_sw128(a_base + k * 32, 16, 1024);
+                else ad = make_smem_desc_sw128(a_base + k * 2048, BK * 128, 1024);
+#pragma unroll
+                for (int q = 0; q < T::NW; ++q) {
+                  const uint32_t bq = b_base + q * T::B_PART_BYTES;
+                  uint64_t bd;
+                  if (!B_MN) bd = make_smem_desc_sw128(bq + k * 32, 16, 1024);
+                  else bd = make_smem_desc_sw128(bq + k * 2048, BK * 128, 1024);
+                  umma_bf16_cg<CG>(d_tmem + q * BN, ad, bd, idesc, (first && k == 0) ? 0u : 1u);
+                }
+              }
+              // frees this stage in both CTAs once the MMAs have read it
+              if constexpr (PAIR) umma_commit_pair(&empty[stage], 0x3);
+              else umma_commit(&empty[stage]);
+            }
+            __syncwarp();
+            first = false;
+            if (++stage == T::STAGES) {
+              stage = 0;
+              phase ^= 1;
+            }
           }
         }
-      }
-      if (!ok) break;
-      if (lane == 0) {
-        if constexpr (PAIR) umma_commit_pair(&tfull[acc], 0x3);
-        else umma_commit(&tfull[acc]);
-      }
-      __syncwarp();
-      if (++acc == T::NACC) {
-        acc = 0;
-        acc_phase ^= 1;
+        if (!ok) break;
+        if (lane == 0) {
+          if constexpr (PAIR) umma_commit_pair(&tfull[acc], 0x3);
+          else umma_commit(&tfull[acc]);
+        }
+        __syncwarp();
+        if (++acc == T::NACC) {
+          acc = 0;
+          acc_phase ^= 1;
+        }
       }
     }
     // Drain: every MMA this thread issued has completed before teardown.
@@ -742,7 +850,41 @@ __global__ void __launch_bounds__(epi_threads(EPI), 1)
           else mbar_arrive(&tempty[acc]);
         }
       };
-      if constexpr (EPI >= kEpiCeStats) {
+      if constexpr (PARTS) {
+        uint32_t x[2][32];
+        bool ok = true;
+#pragma unroll
+        for (int c = 0; c < 2; ++c) tmem_ld_32x32b_x32(t_row + c * 32, x[c]);
+        tmem_ld_wait();
+        release_tmem();
+        for (int kp = 1; kp < k_parts; ++kp) {
+          if (++acc == T::NACC) {
+            acc = 0;
+            acc_phase ^= 1;
+          }
+          if (!mbar_wait<PAIR>(&tfull[acc], acc_phase, p.status, DEV_TIMEOUT_EPILOGUE)) {
+            ok = false;
+            break;
+          }
+          tc_fence_after();
+          const uint32_t t_part = tmem_base + (static_cast<uint32_t>(quad * 32) << 16) +
+                                  static_cast<uint32_t>(acc * BN + part * SLICE);
+          uint32_t r[8];
+#pragma unroll
+          for (int c = 0; c < 8; ++c) {
+            tmem_ld_32x32b_x8(t_part + c * 8, r);
+            tmem_ld_wait();
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+              uint32_t& sum = x[c >> 2][(c & 3) * 8 + j];
+              sum = __float_as_uint(__uint_as_float(sum) + __uint_as_float(r[j]));
+            }
+          }
+          release_tmem();
+        }
+        if (!ok) break;
+        ce_parts_epilogue<EPI>(p, &mapC, buf, lane, x, colh, row0, grow, row_ok, colh / kCePartCols, row_c, pol_c);
+      } else if constexpr (EPI >= kEpiCeStats) {
         ce_epilogue<EPI>(p, &mapC, buf, lane, t_row, colh, row0, grow, row_ok, colh / kCePartCols, row_c, pol_c,
                          release_tmem);
       } else if constexpr (EPI == kEpiStoreBf16) {
@@ -1154,6 +1296,14 @@ cudaError_t dispatch(const GemmDesc& d, const CUtensorMap* maps, const KParams& 
       return cudaErrorInvalidValue;
     }
     if (d.epi == Epi::CeGrad) return launch_t<CG, false, false, kEpiCeGrad>(maps, kp, num_sms, stream);
+    if (ce_k_parts(kp.seg_kblocks[0]) > 1) {
+      if (d.args.out16) {
+        if (d.args.ce_sx) return launch_t<CG, false, false, kEpiCeParts + 3>(maps, kp, num_sms, stream);
+        return launch_t<CG, false, false, kEpiCeParts + 1>(maps, kp, num_sms, stream);
+      }
+      if (d.args.ce_sx) return launch_t<CG, false, false, kEpiCeParts + 2>(maps, kp, num_sms, stream);
+      return launch_t<CG, false, false, kEpiCeParts>(maps, kp, num_sms, stream);
+    }
     if (d.args.out16) {
       if (d.args.ce_sx) return launch_t<CG, false, false, kEpiCeStats + 3>(maps, kp, num_sms, stream);
       return launch_t<CG, false, false, kEpiCeStats + 1>(maps, kp, num_sms, stream);
@@ -1238,12 +1388,12 @@ struct FewCfg {
   static constexpr int STAGES = 208 * 1024 / STAGE;  // 10, 8, 6 for N = 32, 64, 128
   static constexpr int REF_BYTES = N * 8;
   static constexpr int SMEM = STAGES * STAGE + REF_BYTES + 256 + 1024;
-  static constexpr int TMEM = 2 * N < 32 ? 32 : 2 * N;
   static_assert(SMEM <= 232448 && (2 * STAGES + 5) * 8 + 4 <= 256, "shared memory");
 };
 
 struct FewParams {
   int M, n, kblocks, tiles;
+  int k_parts;  // accumulators of a tile; two tiles' fit TMEM
   int* status;
   int pol_w, pol_h;
   EpiArgs e;
@@ -1280,7 +1430,7 @@ __global__ void __launch_bounds__(FEW_THREADS, 1)
     tma_prefetch_desc(&map_h);
   }
   if (warp == 2) {
-    tmem_alloc(tmem_slot, T::TMEM);
+    tmem_alloc(tmem_slot, TMEM_COLS);
     tmem_relinquish();
   }
   tc_fence_before();
@@ -1335,7 +1485,14 @@ __global__ void __launch_bounds__(FEW_THREADS, 1)
       const int acc = tile & 1;
       if (!mbar_wait(&tempty[acc], ((tile >> 1) & 1) ^ 1, p.status, DEV_TIMEOUT_MMA)) break;
       tc_fence_after();
+      int part = 0, next = 0;  // the K part under way, where the next one begins
+      uint32_t d_tmem = 0;
       for (int kb = 0; kb < p.kblocks; ++kb, ++it) {
+        const bool begins = kb == next;
+        if (begins) {
+          d_tmem = tmem_base + static_cast<uint32_t>((acc * p.k_parts + part) * N);
+          next = ce_k_begin(p.kblocks, p.k_parts, ++part);
+        }
         const int st = it % T::STAGES;
         if (!mbar_wait(&full[st], (it / T::STAGES) & 1, p.status, DEV_TIMEOUT_MMA)) {
           ok = false;
@@ -1346,8 +1503,8 @@ __global__ void __launch_bounds__(FEW_THREADS, 1)
           const uint32_t a = smem_u32(smem + st * T::STAGE), b = a + T::W_STAGE;
 #pragma unroll
           for (int k = 0; k < BK / 16; ++k)
-            umma_bf16(tmem_base + acc * N, make_smem_desc_sw128(a + k * 32, 16, 1024),
-                      make_smem_desc_sw128(b + k * 32, 16, 1024), idesc, kb > 0 || k > 0 ? 1u : 0u);
+            umma_bf16(d_tmem, make_smem_desc_sw128(a + k * 32, 16, 1024),
+                      make_smem_desc_sw128(b + k * 32, 16, 1024), idesc, begins && k == 0 ? 0u : 1u);
           umma_commit(&empty[st]);
         }
         __syncwarp();
@@ -1366,7 +1523,6 @@ __global__ void __launch_bounds__(FEW_THREADS, 1)
     for (int j = threadIdx.x - 128; j < N; j += 128)
       refs[j] = j < p.M ? p.e.ce_ref[j] : make_float2(0.f, __int_as_float(-1));
     asm volatile("bar.sync 1, 128;" ::: "memory");
-    const float log2e = p.e.ce_log2e;
     for (int tile = 0; tile < tiles; ++tile) {
       const int acc = tile & 1;
       if (!mbar_wait(&tfull[acc], (tile >> 1) & 1, p.status, DEV_TIMEOUT_EPILOGUE)) break;
@@ -1379,14 +1535,23 @@ __global__ void __launch_bounds__(FEW_THREADS, 1)
 #pragma unroll 1
         for (int c = 0; c < N; c += 32) {
           if (c >= p.M) break;
+          const uint32_t t_row = tmem_base + (static_cast<uint32_t>(quad * 32) << 16) + acc * p.k_parts * N + c;
           uint32_t r[32];
-          tmem_ld_32x32b_x32(tmem_base + (static_cast<uint32_t>(quad * 32) << 16) + acc * N + c, r);
+          tmem_ld_32x32b_x32(t_row, r);
           tmem_ld_wait();
+          for (int part = 1; part < p.k_parts; ++part) {
+            uint32_t more[32];
+            tmem_ld_32x32b_x32(t_row + part * N, more);
+            tmem_ld_wait();
+#pragma unroll
+            for (int j = 0; j < 32; ++j)
+              r[j] = __float_as_uint(__uint_as_float(r[j]) + __uint_as_float(more[j]));
+          }
           float e[32];
 #pragma unroll
           for (int j = 0; j < 32; ++j) {
             const float2 ref = refs[c + j];
-            const float x = fast_exp2(fmaf(__uint_as_float(r[j]), log2e, -ref.x));
+            const float x = fast_exp2(fmaf(__uint_as_float(r[j]), LOG2E, -ref.x));
             e[j] = in && v != __float_as_int(ref.y) ? x : 0.f;
           }
 #pragma unroll
@@ -1410,8 +1575,8 @@ __global__ void __launch_bounds__(FEW_THREADS, 1)
               float m = use ? x : -INFINITY;
 #pragma unroll
               for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
-              const float own = m * log2e > -INFINITY ? m * log2e : refs[c + j].x;
-              float s = use ? fast_exp2(fmaf(x, log2e, -own)) : 0.f;
+              const float own = m * LOG2E > -INFINITY ? m * LOG2E : refs[c + j].x;
+              float s = use ? fast_exp2(fmaf(x, LOG2E, -own)) : 0.f;
 #pragma unroll
               for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
               if (lane == j) {
@@ -1426,7 +1591,7 @@ __global__ void __launch_bounds__(FEW_THREADS, 1)
             uint16_t* dst = static_cast<uint16_t*>(p.e.out16) + static_cast<long long>(c) * p.e.ld16 + col;
 #pragma unroll
             for (int j = 0; j < 32; ++j) {
-              const float t = fmaf(__uint_as_float(r[j]), log2e, -__shfl_sync(0xffffffffu, ref2, j));
+              const float t = fmaf(__uint_as_float(r[j]), LOG2E, -__shfl_sync(0xffffffffu, ref2, j));
               const float u = fmaf(fmaxf(t, kCeQLow), kCeQScale, 8388608.0f + kCeQBias);
               if (c + j < p.M && in) dst[j * p.e.ld16] = static_cast<uint16_t>(__float_as_uint(u));
             }
@@ -1457,7 +1622,7 @@ __global__ void __launch_bounds__(FEW_THREADS, 1)
   __syncthreads();
   if (warp == 2) {
     tc_fence_after();
-    tmem_dealloc(tmem_base, T::TMEM);
+    tmem_dealloc(tmem_base, TMEM_COLS);
   }
 }
 
@@ -1512,6 +1677,12 @@ cudaError_t few_launch(const GemmDesc& d, int num_sms, cudaStream_t stream, cons
   fp.n = static_cast<int>(d.N);
   fp.kblocks = static_cast<int>((d.k_seg[0] + BK - 1) / BK);
   fp.tiles = static_cast<int>((d.N + FEW_TILE - 1) / FEW_TILE);
+  // K parts as in the GEMM, or of half that length where it costs nothing (one
+  // token at H = 4096 175 us in one part and in four, 50 tokens 184 and 185), as
+  // many as TMEM holds for two tiles: 8, 4 and 2 for 32, 64 and 128 rows. 128 rows
+  // in four, with one tile's accumulators: 209 us, in one part 191.
+  const int longest = n <= 64 ? kCeKBlocks / 2 : kCeKBlocks;
+  fp.k_parts = std::min((fp.kblocks + longest - 1) / longest, TMEM_COLS / (2 * n));
   fp.status = d.status;
   fp.pol_w = 0;
   fp.pol_h = 2;

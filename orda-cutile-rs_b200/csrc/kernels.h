@@ -88,9 +88,7 @@ struct EpiArgs {
   // StoreBf16, and the 16-bit piece that CeStats (optionally) and CeGrad write
   void* out16 = nullptr;
   long long ld16 = 0;
-  // CeStats, CeGrad: column c is vocabulary index ce_v0 + c; logits times
-  // ce_log2e are base-2 exponents
-  float ce_log2e = 0.0f;
+  // CeStats, CeGrad: column c is vocabulary index ce_v0 + c
   long long ce_v0 = 0;
   const float2* ce_ref = nullptr;    // CeStats: per row (reference logit * log2 e, label as int bits)
   float2* ce_rec = nullptr;          // CeStats: [rows][ce_rec_ld] records of the parts, from column 0 of this launch
@@ -145,14 +143,6 @@ constexpr int kCePartCols = 64;  // columns of one epilogue warp
 constexpr int kCeFewRows = 128;
 constexpr int kCeFewPartCols = 32;
 
-// The tensor cores' fp32 accumulator cuts where it adds, so a sum of k products
-// comes out smaller in magnitude, by k 2^-30 of itself on average (measured on
-// random operands: 3.8e-7, 8.2e-7, 1.77e-6 and 3.74e-6 for k = 512, 1024, 2048 and
-// 4096, nearly all of the error, where rounded fp32 sums have a mean error of
-// 1e-10). Unlike a rounding it does not average out over the vocabulary or the
-// tokens, so the cross entropy undoes it with the exponents' factor.
-inline float cut_factor(long long k) { return 1.0f + static_cast<float>(k) * 9.313225746154785e-10f; }
-
 struct CeArgs {
   const void* h = nullptr;  // bf16 [bt, hd]
   long long ldh = 0;
@@ -171,7 +161,6 @@ struct CeArgs {
   float* sx = nullptr;         // [bt][rec_ld], with label smoothing
   long long rec_ld = 0;
   int n_parts = 0, part_shift = 0;  // parts of 1 << part_shift columns
-  float cut = 1.0f;             // what a logit of the tensor cores is multiplied by (see cut_factor)
   float4* row_const = nullptr;  // [bt]
   float* nll = nullptr;         // [bt]; the label's logit between the first kernel and the loss
   float* lse = nullptr;         // [bt], optional

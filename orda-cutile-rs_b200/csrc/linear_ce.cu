@@ -15,6 +15,13 @@
 // is held as -FLT_MAX: an infinite reference would turn the parts that keep it
 // into NaN. The loss of such a row comes from the logit itself.
 //
+// The label's logit is a rounded fp32 sum; the other logits are the tensor cores'
+// fp32 sums over at most 2048 of K at a time, added in fp32: exact where fp32 holds
+// the sums, else too small by up to 2e-6 of themselves on average (see kCeKBlocks in
+// gemm_sm100.cu). No factor undoes that average: it would be an error of its own
+// size wherever nothing was cut. The recomputed pieces' gradients, which are
+// rounded to bf16, sum K in one.
+//
 // Between the logits product and the two gradient products the logits of a
 // piece are kept as 16-bit fixed point, t = log2 e^{z - z_y} in steps of
 // 2^-9 over (-64, 64), and 0 below (a part whose own sum is under 2^-40 is
@@ -162,7 +169,7 @@ __device__ __forceinline__ RowResult row_result(const CeArgs& a, float2 ref, flo
     l = static_cast<float>(lse);
   }
   const float uni = a.alpha / static_cast<float>(a.v);
-  r.nll = a.alpha > 0.f ? (1.f - a.alpha) * gap + a.alpha * (l - sx * a.cut / static_cast<float>(a.v)) : gap;
+  r.nll = a.alpha > 0.f ? (1.f - a.alpha) * gap + a.alpha * (l - sx / static_cast<float>(a.v)) : gap;
   r.lse = l;
   r.c.x = -l * kLog2E;
   r.c.y = ref.y;

@@ -515,3 +515,48 @@ def test_a_row_of_lowest_values_only_shows(ctx, bt):
     g = formula(x[rest], w, labels[rest])
     tol = f["row_tol"][rest] + 2.0**-23 * g["nll"].abs()
     assert torch.all((r.nll[rest].double() - g["nll"]).abs() <= tol)
+
+
+@pytest.mark.parametrize("bt", [20, 300])
+@pytest.mark.parametrize("dense", [False, True])
+def test_logits_whose_sums_are_exact(ctx, bt, dense):
+    """Equal rows of weight and products that fp32 adds up without rounding: every logit is the same z, so lse - z =
+    log V. fp32 rounds z log2 e and z (2^-24 of each, and twice more in lse), an exponential is off by 2^-22 and a sum
+    of V of them by 2^-21 at most; the results round once more."""
+    h, v = 4096, 5000
+    x = torch.zeros(bt, h, device="cuda", dtype=torch.bfloat16)
+    w = torch.zeros(v, h, device="cuda", dtype=torch.bfloat16)
+    z = torch.tensor([100.0, -75.0, 50.0, 3.0, 0.0], device="cuda").repeat(bt)[:bt]
+    if dense:
+        w[:] = 2.0**-6
+        x[:] = (z / 64).to(torch.bfloat16)[:, None]
+        z = x[:, 0].double() * 64
+    else:
+        w[:, 0] = 1.0
+        x[:, 0] = z.to(torch.bfloat16)
+        z = z.double()
+    labels = torch.arange(bt, device="cuda") * 7 % v
+    for grads in (False, True):
+        r = call(ctx, x, w, labels, need_grad_hidden=grads, need_grad_weight=grads, grad_dtype=torch.bfloat16)
+        tol = 2 * 2.0**-24 * z.abs() + 2.0**-20 + 2.0**-22 * math.log(v)
+        assert torch.all((r.nll.double() - math.log(v)).abs() <= tol), float((r.nll.double() - math.log(v)).abs().max())
+        assert torch.all((r.lse.double() - math.log(v) - z).abs() <= 2 * tol)
+
+
+
+@pytest.mark.parametrize("bt,h", [(64, 4096), (100, 4096), (300, 4096), (300, 2000), (300, 6200), (20, 9000)])
+def test_logits_of_long_products_are_not_cut(ctx, bt, h):
+    """Random operands: the tensor cores' sums over k come out too small by k 2^-30 of themselves on average, and the
+    logits sum at most 2048 at once. lse is at most its largest logits and log V, so its mean relative error stays
+    within 2048 2^-30 (twice to four times that where K is summed in one; the mean logit under the softmax is 0.93 of lse here) and
+    that of the rounded results, 2^-24 / sqrt(bt)."""
+    gen = torch.Generator(device="cuda").manual_seed(bt + h)
+    v = 5003
+    w = (torch.randn(v, h, generator=gen, device="cuda") * (6.0 / math.sqrt(h))).bfloat16()
+    x = torch.randn(bt, h, generator=gen, device="cuda").bfloat16()
+    labels = torch.randint(0, v, (bt,), generator=gen, device="cuda")
+    lse = torch.logsumexp(x.double() @ w.double().T, 1)
+    for grads in (False, True):
+        r = call(ctx, x, w, labels, need_grad_hidden=grads, need_grad_weight=grads)
+        off = float(((r.lse.double() - lse) / lse).mean())
+        assert abs(off) <= 2048 * 2.0**-30 + 3 * 2.0**-24 / math.sqrt(bt), off
