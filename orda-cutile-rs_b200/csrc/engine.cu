@@ -190,12 +190,12 @@ cudaError_t ensure_ws(OrdaContext* ctx, size_t bytes) {
     return cudaErrorMemoryAllocation;
   }
   if (ctx->ws_bytes >= bytes) return cudaSuccess;
-  if (ctx->ws) {
-    if (ctx->ws_in_graph) ctx->ws_retired.push_back(ctx->ws);
-    else cudaFree(ctx->ws);
+  // a workspace that a graph holds frees no memory for the larger one: it stays
+  // the context's until that one has been had
+  if (ctx->ws && !ctx->ws_in_graph) {
+    cudaFree(ctx->ws);
     ctx->ws = nullptr;
     ctx->ws_bytes = 0;
-    ctx->ws_in_graph = false;
   }
   void* p = nullptr;
   cudaError_t e = cudaMalloc(&p, bytes);
@@ -203,8 +203,10 @@ cudaError_t ensure_ws(OrdaContext* ctx, size_t bytes) {
     cudaGetLastError();  // clear the sticky-free allocation error
     return e;
   }
+  if (ctx->ws) ctx->ws_retired.push_back(ctx->ws);
   ctx->ws = p;
   ctx->ws_bytes = bytes;
+  ctx->ws_in_graph = false;
   return cudaSuccess;
 }
 

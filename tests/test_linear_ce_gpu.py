@@ -560,3 +560,31 @@ def test_logits_of_long_products_are_not_cut(ctx, bt, h):
         r = call(ctx, x, w, labels, need_grad_hidden=grads, need_grad_weight=grads)
         off = float(((r.lse.double() - lse) / lse).mean())
         assert abs(off) <= 2048 * 2.0**-30 + 3 * 2.0**-24 / math.sqrt(bt), off
+
+
+def test_a_refused_workspace_leaves_a_captured_one(ctx):
+    """A workspace that a graph holds stays the context's when a larger one cannot be had (275 GB of statistics)."""
+    from orda_b200.device import DeviceContext, linear_cross_entropy_device
+
+    x, w, labels = make(100, 128, 2000, seed=11)
+    with DeviceContext(0) as own:
+        want = call(own, x, w, labels)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            r = linear_cross_entropy_device(own, x, w, labels)
+        held = own.workspace_bytes()
+        bt, v = 1 << 19, 1 << 22
+        huge = [torch.zeros(bt, 8, device="cuda", dtype=torch.bfloat16),
+                torch.zeros(v, 8, device="cuda", dtype=torch.bfloat16), torch.zeros(bt, device="cuda", dtype=torch.int64)]
+        with pytest.raises(RuntimeError, match="workspace"):
+            linear_cross_entropy_device(own, *huge, need_grad_hidden=False, need_grad_weight=False)
+        assert own.workspace_bytes() == held
+        second = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(second):
+            r2 = linear_cross_entropy_device(own, x, w, labels)
+        graph.replay()
+        second.replay()
+        torch.cuda.synchronize()
+        own.check()
+        assert torch.equal(r.grad_weight, want.grad_weight) and torch.equal(r2.grad_weight, want.grad_weight)
+        del graph, second
