@@ -184,12 +184,14 @@ WsLayout make_layout(const DevInputs& in, const Flags& f, size_t cs, size_t fwd_
   return L;
 }
 
-cudaError_t ensure_ws(OrdaContext* ctx, size_t bytes) {
+// With `keeps`, for what outlives the call: not a workspace that a graph holds,
+// whose replay would write over it.
+cudaError_t ensure_ws(OrdaContext* ctx, size_t bytes, bool keeps = false) {
   if (ctx->inject_fail > 0) {
     --ctx->inject_fail;
     return cudaErrorMemoryAllocation;
   }
-  if (ctx->ws_bytes >= bytes) return cudaSuccess;
+  if (ctx->ws_bytes >= bytes && !(keeps && ctx->ws_in_graph)) return cudaSuccess;
   // a workspace that a graph holds frees no memory for the larger one: it stays
   // the context's until that one has been had
   if (ctx->ws && !ctx->ws_in_graph) {
@@ -487,7 +489,7 @@ int run_device(OrdaContext* ctx, const DevInputs& in, const OrdaLossOptions& o, 
     // backward phase: one forward and one backward group
     ctx->vocab_ready = false;
     at.layout = make_layout(in, f, plan.chunk_size, bt, bt);
-    if (ensure_ws(ctx, at.layout.total) != cudaSuccess) {
+    if (ensure_ws(ctx, at.layout.total, true) != cudaSuccess) {
       set_error(err, len, "vocabulary-sharded calls keep the whole batch's slice logits between the two phases: "
                           "%zu bytes of workspace are not available", at.layout.total);
       return ORDA_ERR_OOM;

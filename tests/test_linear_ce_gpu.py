@@ -588,3 +588,35 @@ def test_a_refused_workspace_leaves_a_captured_one(ctx):
         own.check()
         assert torch.equal(r.grad_weight, want.grad_weight) and torch.equal(r2.grad_weight, want.grad_weight)
         del graph, second
+
+
+def test_a_replay_leaves_a_vocabulary_forward_phase(ctx):
+    """A captured call replayed between the two phases of a vocabulary-sharded step on the same context."""
+    import orda_b200 as ob
+    from orda_b200.device import (DeviceContext, linear_cross_entropy_device, vocab_backward_device,
+                                  vocab_forward_device)
+
+    x, w, labels = make(256, 128, 4096, seed=19)
+    teacher = (x.float() * 0.9).bfloat16()
+    opts = ob.LossOptions(kd_weight=0.4, temperature=1.5)
+    big = make(400, 256, 9000, seed=20)
+    with DeviceContext(0) as own:
+        call(own, *big)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            r = linear_cross_entropy_device(own, *big)
+        got = []
+        for replay in (False, True):
+            part = vocab_forward_device(own, x, w, labels, ob.TeacherMode.Tied, 4096, 0, opts=opts,
+                                        teacher_hidden=teacher)
+            if replay:
+                graph.replay()
+            got.append(vocab_backward_device(own, x, w, labels, ob.TeacherMode.Tied, 4096, 0, part[None], True,
+                                             opts=opts, teacher_hidden=teacher))
+        torch.cuda.synchronize()
+        own.check()
+        assert torch.equal(got[0].scalars, got[1].scalars)
+        assert torch.equal(got[0].grad_weight, got[1].grad_weight)
+        assert torch.equal(got[0].grad_student_hidden, got[1].grad_student_hidden)
+        check(r, formula(*big))
+        del graph
