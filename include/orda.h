@@ -263,7 +263,12 @@ typedef struct OrdaContext OrdaContext;
 ORDA_API int orda_context_create(int device, OrdaContext** out, char* err, size_t err_len);
 ORDA_API void orda_context_destroy(OrdaContext* ctx);
 /* Synchronizes the context's last stream and reports asynchronous device
- * failures (label out of range, bounded-wait timeout). */
+ * failures (label or token id out of range, bounded-wait timeout), one kind a
+ * call: what else there is comes with the next ones. What a linear cross entropy
+ * or embedding call finds out of range is kept until it is reported, and so is
+ * what any call left unreported before a linear cross entropy. A distillation
+ * call forgets an expired wait, and a bad label of the distillation call before
+ * it. */
 ORDA_API int orda_context_check(OrdaContext* ctx, char* err, size_t err_len);
 /* Bytes of device workspace currently held by the context. */
 ORDA_API size_t orda_context_workspace_bytes(const OrdaContext* ctx);

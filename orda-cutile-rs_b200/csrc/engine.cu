@@ -47,9 +47,10 @@
 struct OrdaContext {
   int device = 0;
   int num_sms = 148;
-  // [0] status, [1] n_non_ignore, [2] a label, [3] a token id out of range (both
-  // kept until they are reported), [4] live tokens and [5] finished blocks of a
-  // linear cross entropy call (0 between calls)
+  // [0] status of the last call that clears it, [1] n_non_ignore, [2] a label and
+  // [3] a token id out of range, [6] an expired wait of a call before a linear
+  // cross entropy (each kept until it is reported), [4] live tokens and [5]
+  // finished blocks of a linear cross entropy call (0 between calls)
   int* d_words = nullptr;
   float* d_mean_scale = nullptr;  // [0] distillation loss, [1] linear cross entropy
   void* ws = nullptr;
@@ -1089,6 +1090,7 @@ int run_linear_ce(OrdaContext* ctx, const OrdaDeviceMat& hm, const OrdaDeviceMat
   a.scale = ctx->d_mean_scale + 1;
   a.status = ctx->d_words;
   a.bad_label = ctx->d_words + 2;
+  a.earlier = ctx->d_words + 6;
   a.count = ctx->d_words + 4;
   a.done = ctx->d_words + 5;
   uint16_t* piece = grads ? reinterpret_cast<uint16_t*>(ws + L.piece) : nullptr;
@@ -1231,25 +1233,38 @@ bool device_is_sm100(int dev) {
 }
 
 int check_status(OrdaContext* ctx, char* err, size_t len) {
-  int words[4] = {0, 0, 0, 0};
+  int words[7] = {};
   cudaError_t e = cudaStreamSynchronize(ctx->last_stream);
   if (e != cudaSuccess) return cuda_fail(e, "stream synchronize", err, len);
   e = cudaMemcpy(words, ctx->d_words, sizeof words, cudaMemcpyDeviceToHost);
   if (e != cudaSuccess) return cuda_fail(e, "status read", err, len);
-  if (words[2] != DEV_OK || words[3] != DEV_OK) {
-    // kept across calls until they are reported here
-    if ((e = cudaMemset(ctx->d_words + 2, 0, 2 * sizeof(int))) != cudaSuccess) return cuda_fail(e, "memset", err, len);
-  }
+  // one report a call; a word is cleared with its own report, so that what else
+  // happened is reported by the next calls. Word 0 stays until the next loss call
+  // clears it, marked as reported.
+  auto put = [&](int word, int value) {
+    return cudaMemcpy(ctx->d_words + word, &value, sizeof value, cudaMemcpyHostToDevice);
+  };
+  int status = words[0] & ~kStatusReported;
   if (words[3] != DEV_OK) {
+    if ((e = put(3, DEV_OK)) != cudaSuccess) return cuda_fail(e, "status write", err, len);
     set_error(err, len, "a token id is out of range [0, V) (device id check)");
     return ORDA_ERR_LABEL;
   }
-  if (words[0] == DEV_LABEL_RANGE || words[2] != DEV_OK) {
+  if (words[2] != DEV_OK) {
+    if ((e = put(2, DEV_OK)) != cudaSuccess) return cuda_fail(e, "status write", err, len);
+    status = DEV_LABEL_RANGE;
+  } else if (words[6] != DEV_OK) {
+    if ((e = put(6, DEV_OK)) != cudaSuccess) return cuda_fail(e, "status write", err, len);
+    status = words[6];
+  } else if (status != DEV_OK) {
+    if ((e = put(0, status | kStatusReported)) != cudaSuccess) return cuda_fail(e, "status write", err, len);
+  }
+  if (status == DEV_LABEL_RANGE) {
     set_error(err, len, "a label is out of range [0, V) and != ignore_index (device label check)");
     return ORDA_ERR_LABEL;
   }
-  if (words[0] != DEV_OK) {
-    set_error(err, len, "a bounded device wait expired (status 0x%x); results are invalid", words[0]);
+  if (status != DEV_OK) {
+    set_error(err, len, "a bounded device wait expired (status 0x%x); results are invalid", status);
     return ORDA_ERR_TIMEOUT;
   }
   return ORDA_OK;

@@ -166,7 +166,8 @@ struct CeArgs {
   float* lse = nullptr;         // [bt], optional
   float* loss = nullptr;        // [1]
   float* scale = nullptr;       // [1] what the gradients are multiplied by after the products
-  int* status = nullptr;        // cleared by the first kernel
+  int* status = nullptr;        // cleared by the first kernel; what was not reported yet goes to the next two
+  int* earlier = nullptr;       // an expired wait of an earlier call
   int* bad_label = nullptr;     // set to DEV_LABEL_RANGE
   int* count = nullptr;         // live tokens; 0 between calls
   int* done = nullptr;          // ended blocks of ce_rows_kernel; 0 between calls

@@ -74,7 +74,11 @@ __global__ void __launch_bounds__(kPrepThreads) ce_prep_kernel(const CeArgs a) {
   const bool token = row < a.bt;
   const int64_t y = token ? a.labels[row] : a.ignore_index;
   bool live = token && y != a.ignore_index;
-  if (row == 0 && threadIdx.x == 0) *a.status = DEV_OK;
+  if (row == 0 && threadIdx.x == 0) {
+    const int old = *a.status;
+    if (old != DEV_OK && !(old & kStatusReported)) *(old == DEV_LABEL_RANGE ? a.bad_label : a.earlier) = old;
+    *a.status = DEV_OK;
+  }
   if (live && (y < 0 || y >= a.v)) {
     if (threadIdx.x == 0) *a.bad_label = DEV_LABEL_RANGE;
     live = false;

@@ -27,6 +27,8 @@ enum DeviceStatus : int {
   DEV_ID_RANGE = 0x202,
   DEV_TIMEOUT_SELFTEST = 0x301,
 };
+// Set in the status word by the host once it has reported what the word holds.
+constexpr int kStatusReported = 0x10000;
 
 __device__ __forceinline__ uint32_t smem_u32(const void* p) {
   return static_cast<uint32_t>(__cvta_generic_to_shared(p));

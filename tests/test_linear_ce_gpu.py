@@ -620,3 +620,57 @@ def test_a_replay_leaves_a_vocabulary_forward_phase(ctx):
         assert torch.equal(got[0].grad_student_hidden, got[1].grad_student_hidden)
         check(r, formula(*big))
         del graph
+
+
+def test_faults_of_earlier_calls_are_reported(ctx):
+    """A bad id and a bad label are reported one after the other; a distillation call's bad label and an expired
+    wait outlive a cross entropy call, and what has been reported is not reported again after it."""
+    import orda_b200 as ob
+    from orda_b200 import _abi
+    from orda_b200.device import DeviceContext, distillation_loss_device, embedding_device, linear_cross_entropy_device
+
+    x, w, labels = make(40, 64, 300)
+    bad = labels.clone()
+    bad[7] = 300
+    with DeviceContext(0) as own:
+        embedding_device(own, w, bad)
+        linear_cross_entropy_device(own, x, w, bad)
+        linear_cross_entropy_device(own, x, w, labels)
+        with pytest.raises(ob.OrdaError, match="token id"):
+            own.check()
+        with pytest.raises(ob.OrdaError, match="label is out of range"):
+            own.check()
+        own.check()
+        # in the other order, and two of each: one report for each kind
+        for _ in range(2):
+            linear_cross_entropy_device(own, x, w, bad)
+            embedding_device(own, w, bad)
+        for _ in range(2):
+            with pytest.raises(ob.OrdaError) as e:
+                own.check()
+            assert e.value.code == _abi.ORDA_ERR_LABEL
+        own.check()
+        # a distillation call keeps its state in a word of its own kind
+        opts = ob.LossOptions(kd_weight=0.0, teacher_ce_weight=0.0)
+        distillation_loss_device(own, x, w, bad, ob.TeacherMode.Tied, teacher_hidden=x, opts=opts)
+        r = linear_cross_entropy_device(own, x, w, labels)
+        with pytest.raises(ob.OrdaError, match="label is out of range"):
+            own.check()
+        own.check()
+        check(r, formula(x, w, labels))
+        # reported before the cross entropy call: not again after it
+        distillation_loss_device(own, x, w, bad, ob.TeacherMode.Tied, teacher_hidden=x, opts=opts)
+        with pytest.raises(ob.OrdaError, match="label is out of range"):
+            own.check()
+        check(call(own, x, w, labels), formula(x, w, labels))
+        # an expired wait, likewise
+        own.selftest_bounded_wait(1000)
+        linear_cross_entropy_device(own, x, w, labels)
+        with pytest.raises(ob.OrdaError) as e:
+            own.check()
+        assert e.value.code == _abi.ORDA_ERR_TIMEOUT
+        own.check()
+        own.selftest_bounded_wait(1000)
+        with pytest.raises(ob.OrdaError):
+            own.check()
+        check(call(own, x, w, labels), formula(x, w, labels))
