@@ -486,7 +486,8 @@ typedef struct OrdaLinearCeOptions {
   int64_t global_non_ignore; /* > 0: use this token count as the mean denominator */
   size_t piece_bytes;        /* bytes of 16-bit logits kept at once; 0 = 4 GiB. Pieces are multiples of 512
                                 columns, so one holds at least 1 KiB for each row. Smaller pieces are
-                                taken when the device memory is short. */
+                                taken when the device memory is short, and by the context's later calls
+                                until its workspace has grown. */
 } OrdaLinearCeOptions;
 typedef struct OrdaLinearCeOutputs {
   float* loss;        /* required device float[1] */

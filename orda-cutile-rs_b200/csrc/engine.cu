@@ -55,6 +55,7 @@ struct OrdaContext {
   float* d_mean_scale = nullptr;  // [0] distillation loss, [1] linear cross entropy
   void* ws = nullptr;
   size_t ws_bytes = 0;
+  size_t ws_refused = 0;  // the smallest size that could not be had, 0 once that has changed
   // A graph captured with this workspace replays with its address: once that
   // has happened a workspace that is outgrown lives on until the context ends.
   bool ws_in_graph = false;
@@ -188,9 +189,13 @@ WsLayout make_layout(const DevInputs& in, const Flags& f, size_t cs, size_t fwd_
 // With `keeps`, for what outlives the call: not a workspace that a graph holds,
 // whose replay would write over it.
 cudaError_t ensure_ws(OrdaContext* ctx, size_t bytes, bool keeps = false) {
+  auto refused = [&] {
+    ctx->ws_refused = ctx->ws_refused ? std::min(ctx->ws_refused, bytes) : bytes;
+    return cudaErrorMemoryAllocation;
+  };
   if (ctx->inject_fail > 0) {
     --ctx->inject_fail;
-    return cudaErrorMemoryAllocation;
+    return refused();
   }
   if (ctx->ws_bytes >= bytes && !(keeps && ctx->ws_in_graph)) return cudaSuccess;
   // a workspace that a graph holds frees no memory for the larger one: it stays
@@ -204,8 +209,9 @@ cudaError_t ensure_ws(OrdaContext* ctx, size_t bytes, bool keeps = false) {
   cudaError_t e = cudaMalloc(&p, bytes);
   if (e != cudaSuccess) {
     cudaGetLastError();  // clear the sticky-free allocation error
-    return e;
+    return refused();
   }
+  if (bytes >= ctx->ws_refused) ctx->ws_refused = 0;
   if (ctx->ws) ctx->ws_retired.push_back(ctx->ws);
   ctx->ws = p;
   ctx->ws_bytes = bytes;
@@ -934,14 +940,18 @@ struct DeviceScope {
   }
 };
 
-// The workspace for a call on `st`. Under stream capture nothing may be
-// allocated, and the graph keeps the workspace's address.
-int call_ws(OrdaContext* ctx, size_t bytes, cudaStream_t st, bool* capturing, char* err, size_t len) {
+int stream_capturing(cudaStream_t st, bool* capturing, char* err, size_t len) {
   cudaStreamCaptureStatus cap = cudaStreamCaptureStatusNone;
   cudaError_t e = cudaStreamIsCapturing(st, &cap);
   if (e != cudaSuccess) return cuda_fail(e, "cudaStreamIsCapturing", err, len);
   *capturing = cap != cudaStreamCaptureStatusNone;
-  if (*capturing) {
+  return ORDA_OK;
+}
+
+// The workspace for a call. Under stream capture nothing may be allocated, and
+// the graph keeps the workspace's address.
+int call_ws(OrdaContext* ctx, size_t bytes, bool capturing, char* err, size_t len) {
+  if (capturing) {
     if (ctx->ws_bytes < bytes) {
       set_error(err, len, "a captured call cannot allocate its %zu bytes of workspace: make the same call once "
                           "before the capture", bytes);
@@ -1047,17 +1057,28 @@ int run_linear_ce(OrdaContext* ctx, const OrdaDeviceMat& hm, const OrdaDeviceMat
       cols = round_up(ceil_div(v, pieces), kCePieceCols);
     }
   }
-  CeLayout L;
+  auto layout = [&](size_t c) { return ce_layout(bt, h, v, c, smooth, out, ctx->num_sms); };
+  auto narrower = [](size_t c) { return round_up(ceil_div(c, 2), kCePieceCols); };
+  CeLayout L = layout(cols);
   bool capturing = false;
+  if (int rc = stream_capturing(st, &capturing, err, len)) return rc;
+  // Where as much workspace was refused before: the widest of the ladder's pieces
+  // that the present one holds, if any. A call that had to take smaller pieces,
+  // and the same call made again or captured, then take the same ones.
+  if (grads && ctx->inject_fail <= 0 && ctx->ws_refused && L.total >= ctx->ws_refused) {
+    size_t c = cols;
+    while (layout(c).total > ctx->ws_bytes && c > kCePieceCols) c = narrower(c);
+    if (layout(c).total <= ctx->ws_bytes) cols = c;
+  }
   while (true) {
-    pieces = ceil_div(v, cols);
-    L = ce_layout(bt, h, v, cols, smooth, out, ctx->num_sms);
-    const int rc = call_ws(ctx, L.total, st, &capturing, err, len);
+    L = layout(cols);
+    const int rc = call_ws(ctx, L.total, capturing, err, len);
     if (rc == ORDA_OK) break;
     // smaller pieces where the memory is short, as the chunk ladder does
     if (rc != ORDA_ERR_OOM || capturing || !grads || cols <= kCePieceCols) return rc;
-    cols = round_up(ceil_div(cols, 2), kCePieceCols);
+    cols = narrower(cols);
   }
+  pieces = ceil_div(v, cols);
 
   uint8_t* ws = static_cast<uint8_t*>(ctx->ws);
   CeArgs a;
@@ -1926,7 +1947,8 @@ int orda_embedding_grad_device(OrdaContext* ctx, const OrdaDeviceMat* grad_out, 
   a.bad = ctx->d_words + 3;
   ctx->vocab_ready = false;  // the workspace no longer holds a vocabulary forward phase
   bool capturing = false;
-  if (int rc = call_ws(ctx, embed_grad_workspace(a), st, &capturing, err, err_len)) return rc;
+  if (int rc = stream_capturing(st, &capturing, err, err_len)) return rc;
+  if (int rc = call_ws(ctx, embed_grad_workspace(a), capturing, err, err_len)) return rc;
   int nl = 0;
   const cudaError_t e = launch_embed_grad(a, ctx->ws, ctx->num_sms, st, &nl);
   ctx->launches += static_cast<uint64_t>(nl);

@@ -674,3 +674,31 @@ def test_faults_of_earlier_calls_are_reported(ctx):
         with pytest.raises(ob.OrdaError):
             own.check()
         check(call(own, x, w, labels), formula(x, w, labels))
+
+
+def test_smaller_pieces_are_kept_and_captured(ctx):
+    """A call that took smaller pieces because memory was short can be captured, and neither it nor later calls
+    ask for the larger workspace again."""
+    from orda_b200.device import DeviceContext, linear_cross_entropy_device
+
+    x, w, labels = make(64, 64, 3000, seed=14)
+    with DeviceContext(0) as own:
+        own.inject_alloc_failures(2)
+        first = call(own, x, w, labels)
+        held = own.workspace_bytes()
+        again = call(own, x, w, labels)
+        assert own.workspace_bytes() == held
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            r = linear_cross_entropy_device(own, x, w, labels)
+        graph.replay()
+        torch.cuda.synchronize()
+        own.check()
+        assert own.workspace_bytes() == held
+        for n in ("loss", "nll", "lse", "grad_hidden", "grad_weight"):
+            assert torch.equal(getattr(r, n), getattr(first, n)) and torch.equal(getattr(r, n), getattr(again, n)), n
+        # a larger call for which no piece fits that workspace still gets its own
+        big = make(300, 64, 9000, seed=15)
+        check(call(own, *big), formula(*big))
+        assert own.workspace_bytes() > held
+        del graph
