@@ -1688,9 +1688,14 @@ cudaError_t few_launch(const GemmDesc& d, int num_sms, cudaStream_t stream, cons
   fp.pol_h = 2;
   fp.e = d.args;
   if (d.launches) *d.launches += 1;
-  if (n == 32) return few_n<32>(map_w, map_h, fp, num_sms, stream);
-  if (n == 64) return few_n<64>(map_w, map_h, fp, num_sms, stream);
-  return few_n<128>(map_w, map_h, fp, num_sms, stream);
+  cudaError_t e = n == 32   ? few_n<32>(map_w, map_h, fp, num_sms, stream)
+                  : n == 64 ? few_n<64>(map_w, map_h, fp, num_sms, stream)
+                            : few_n<128>(map_w, map_h, fp, num_sms, stream);
+  if (e == cudaSuccess && d.demote_kept) {
+    e = demote_operand(d.a[0], stream);
+    if (d.launches) *d.launches += 1;
+  }
+  return e;
 }
 
 cudaError_t gemm_launch(const GemmDesc& d, int num_sms, cudaStream_t stream, const char** why) {

@@ -702,3 +702,21 @@ def test_smaller_pieces_are_kept_and_captured(ctx):
         check(call(own, *big), formula(*big))
         assert own.workspace_bytes() > held
         del graph
+
+
+def test_few_rows_leave_no_kept_lines(ctx):
+    """With the persisting-L2 carve-out on, a call of few tokens demotes the hidden copy too: one launch more."""
+    from orda_b200.device import DeviceContext
+
+    x, w, labels = make(8, 512, 5000, seed=17)
+    counts, results = [], []
+    for carve in (0, 64 << 20):
+        with DeviceContext(0) as own:
+            if carve:
+                assert own.set_l2_persisting(carve) > 0
+            call(own, x, w, labels, need_grad_hidden=False, need_grad_weight=False)
+            n = own.launch_count()
+            results.append(call(own, x, w, labels, need_grad_hidden=False, need_grad_weight=False))
+            counts.append(own.launch_count() - n)
+    assert counts[1] == counts[0] + 1
+    assert torch.equal(results[0].nll, results[1].nll) and torch.equal(results[0].lse, results[1].lse)
