@@ -478,7 +478,9 @@ ORDA_API int orda_vocab_backward_device(OrdaContext* ctx, const OrdaDeviceMat* s
  * synchronisation; labels out of range are reported by orda_context_check.
  * Under stream capture the context must hold the workspace already (make the
  * same call once before); the graph may be replayed until the context is
- * destroyed. */
+ * destroyed, and counts as a call of the context: replay it in order with the
+ * others. orda_context_check does not wait for replays: synchronize the stream
+ * that they run on first. */
 typedef struct OrdaLinearCeOptions {
   int64_t ignore_index;
   float label_smoothing;     /* in [0, 1] */

@@ -1242,7 +1242,7 @@ int run_linear_ce(OrdaContext* ctx, const OrdaDeviceMat& hm, const OrdaDeviceMat
                              out.grad_hidden_dtype == ORDA_DTYPE_BF16, st)) != cudaSuccess)
       return cuda_fail(e, "dgrad sum", err, len);
   }
-  ctx->last_stream = st;
+  if (!capturing) ctx->last_stream = st;  // what is captured runs elsewhere, and its stream may end before the context
   return ORDA_OK;
 }
 
@@ -1900,9 +1900,12 @@ int orda_embedding_device(OrdaContext* ctx, const OrdaDeviceMat* table, const in
   a.out = out->data;
   a.ldo = static_cast<long long>(out->ld);
   a.bad = ctx->d_words + 3;
-  ctx->last_stream = static_cast<cudaStream_t>(stream);
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  bool capturing = false;
+  if (int rc = stream_capturing(st, &capturing, err, err_len)) return rc;
+  if (!capturing) ctx->last_stream = st;
   if (n == 0) return ORDA_OK;
-  launch_embed(a, static_cast<cudaStream_t>(stream));
+  launch_embed(a, st);
   ctx->launches += 1;
   const cudaError_t e = cudaGetLastError();
   return e == cudaSuccess ? ORDA_OK : cuda_fail(e, "embedding", err, err_len);
@@ -1952,7 +1955,7 @@ int orda_embedding_grad_device(OrdaContext* ctx, const OrdaDeviceMat* grad_out, 
   int nl = 0;
   const cudaError_t e = launch_embed_grad(a, ctx->ws, ctx->num_sms, st, &nl);
   ctx->launches += static_cast<uint64_t>(nl);
-  ctx->last_stream = st;
+  if (!capturing) ctx->last_stream = st;
   return e == cudaSuccess ? ORDA_OK : cuda_fail(e, "embedding gradient", err, err_len);
 }
 

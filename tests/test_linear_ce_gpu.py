@@ -720,3 +720,47 @@ def test_few_rows_leave_no_kept_lines(ctx):
             counts.append(own.launch_count() - n)
     assert counts[1] == counts[0] + 1
     assert torch.equal(results[0].nll, results[1].nll) and torch.equal(results[0].lse, results[1].lse)
+
+
+def test_the_capture_stream_may_end(ctx):
+    """A graph outlives the stream that it was captured on; check() then looks at no stream that is gone."""
+    from cuda.bindings import runtime as rt
+
+    from orda_b200.device import DeviceContext, embedding_device, embedding_grad_device, linear_cross_entropy_device
+
+    def ok(res):
+        assert int(res[0]) == 0, res
+        return res[1] if len(res) > 1 else None
+
+    x, w, labels = make(40, 64, 300, seed=18)
+    out = {"loss": torch.zeros(1, device="cuda"), "nll": torch.zeros(40, device="cuda"),
+           "lse": torch.zeros(40, device="cuda"), "grad_hidden": torch.zeros(40, 64, device="cuda"),
+           "grad_weight": torch.zeros(300, 64, device="cuda")}
+    rows, table = torch.zeros(40, 64, device="cuda"), torch.zeros(300, 64, device="cuda")
+    steps = [lambda c, s: linear_cross_entropy_device(c, x, w, labels, out=out, stream=s),
+             lambda c, s: embedding_device(c, w, labels, out=rows, stream=s),
+             lambda c, s: embedding_grad_device(c, rows, labels, 300, scale=2.0, out=table, stream=s)]
+    for step in steps:
+        with DeviceContext(0) as own:
+            step(own, None)
+            torch.cuda.synchronize()
+            s = ok(rt.cudaStreamCreateWithFlags(rt.cudaStreamNonBlocking))
+            ok(rt.cudaStreamBeginCapture(s, rt.cudaStreamCaptureMode.cudaStreamCaptureModeThreadLocal))
+            step(own, int(s))
+            graph = ok(rt.cudaStreamEndCapture(s))
+            run = ok(rt.cudaGraphInstantiate(graph, 0))
+            ok(rt.cudaStreamDestroy(s))
+            for t in (*out.values(), rows, table):
+                t.fill_(7.0)
+            ok(rt.cudaGraphLaunch(run, torch.cuda.current_stream().cuda_stream))
+            torch.cuda.synchronize()
+            own.check()
+            ok(rt.cudaGraphExecDestroy(run))
+            ok(rt.cudaGraphDestroy(graph))
+            if step is steps[0]:
+                f = formula(x, w, labels)
+                assert torch.all((out["nll"].double() - f["nll"]).abs() <= f["row_tol"] + 2.0**-23 * f["nll"].abs())
+            elif step is steps[1]:
+                assert torch.equal(rows, w[labels].float())
+            else:
+                assert not (table == 7.0).any()
