@@ -279,7 +279,8 @@ ORDA_API size_t orda_context_workspace_bytes(const OrdaContext* ctx);
  *   2 dgrad GEMMs   3 wgrad GEMMs   4 INT8 quantiser   5 label pass + finalize
  * orda_context_phase_times synchronizes, adds the elapsed milliseconds and
  * kernel-launch counts accumulated since the last reset into the outputs
- * (arrays of ORDA_NUM_PHASES entries) and returns ORDA_NUM_PHASES. */
+ * (arrays of ORDA_NUM_PHASES entries) and returns ORDA_NUM_PHASES. A linear cross
+ * entropy call under stream capture is not timed. */
 #define ORDA_NUM_PHASES 6
 ORDA_API void orda_context_enable_timing(OrdaContext* ctx, int enable);
 ORDA_API int orda_context_phase_times(OrdaContext* ctx, double* ms_out, uint64_t* launches_out);

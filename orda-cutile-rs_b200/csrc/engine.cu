@@ -80,6 +80,7 @@ struct OrdaContext {
   std::mutex mu;
   // phase timing (see orda_context_enable_timing)
   bool timing = false;
+  bool capturing = false;  // a call under stream capture is being enqueued: events that are only captured have no times
   struct PhaseEvents {
     int phase;
     cudaEvent_t begin, end;
@@ -275,7 +276,7 @@ struct Phase {
   cudaEvent_t begin = nullptr;
   int n = 0;
   Phase(OrdaContext* c, int p, cudaStream_t s) : ctx(c), phase(p), st(s) {
-    if (ctx->timing) {
+    if (ctx->timing && !ctx->capturing) {
       begin = take_event(ctx);
       cudaEventRecord(begin, st);
     }
@@ -1060,8 +1061,7 @@ int run_linear_ce(OrdaContext* ctx, const OrdaDeviceMat& hm, const OrdaDeviceMat
   auto layout = [&](size_t c) { return ce_layout(bt, h, v, c, smooth, out, ctx->num_sms); };
   auto narrower = [](size_t c) { return round_up(ceil_div(c, 2), kCePieceCols); };
   CeLayout L = layout(cols);
-  bool capturing = false;
-  if (int rc = stream_capturing(st, &capturing, err, len)) return rc;
+  const bool capturing = ctx->capturing;
   // Where as much workspace was refused before: the widest of the ladder's pieces
   // that the present one holds, if any. A call that had to take smaller pieces,
   // and the same call made again or captured, then take the same ones.
@@ -1838,7 +1838,9 @@ int orda_linear_cross_entropy_device(OrdaContext* ctx, const OrdaDeviceMat* hidd
   std::lock_guard<std::mutex> lock(ctx->mu);
   DeviceScope dev(ctx->device);
   cudaStream_t st = static_cast<cudaStream_t>(stream);
+  if (int rc = stream_capturing(st, &ctx->capturing, err, err_len)) return rc;
   const int rc = run_linear_ce(ctx, *hidden, *weight, labels, bt, *opts, *out, st, err, err_len);
+  ctx->capturing = false;
   // a call that broke off leaves its counters as a whole one does
   if (rc == ORDA_ERR_CUDA) cudaMemsetAsync(ctx->d_words + 4, 0, 2 * sizeof(int), st);
   return rc;

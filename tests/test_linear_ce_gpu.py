@@ -764,3 +764,24 @@ def test_the_capture_stream_may_end(ctx):
                 assert torch.equal(rows, w[labels].float())
             else:
                 assert not (table == 7.0).any()
+
+
+def test_phase_timing_and_capture(ctx):
+    """A captured call leaves no events behind whose times could not be read."""
+    from orda_b200.device import DeviceContext, linear_cross_entropy_device
+
+    x, w, labels = make(150, 64, 900, seed=24)
+    with DeviceContext(0) as own:
+        own.enable_timing()
+        call(own, x, w, labels)
+        once = own.phase_times()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            linear_cross_entropy_device(own, x, w, labels)
+        graph.replay()
+        torch.cuda.synchronize()
+        assert own.phase_times() == once
+        check(call(own, x, w, labels), formula(x, w, labels))
+        twice = own.phase_times()
+        assert all(twice[k][1] == 2 * n and twice[k][0] >= ms for k, (ms, n) in once.items())
+        del graph
