@@ -252,6 +252,7 @@ __global__ void __cluster_dims__(kSortCtas, 1, 1) __launch_bounds__(THREADS, 1) 
       }
       total[td] = s;
     }
+    __syncwarp();  // with fewer digits than lanes: the cluster's barriers take whole warps
     cluster_sync();
     uint32_t before = 0, all = 0;
     if (td < digits) {
@@ -265,6 +266,7 @@ __global__ void __cluster_dims__(kSortCtas, 1, 1) __launch_bounds__(THREADS, 1) 
     // no CTA ends before its totals have been read; the last pass needs no more of
     // the cluster, so that barrier runs while the pairs are placed
     const bool last = pass + 1 == a.passes;
+    __syncwarp();
     if (last) cluster_arrive();
     // inclusive scan over the digits: within warps, then the warps' sums
     auto warp_scan = [lane](uint32_t x) {

@@ -380,3 +380,19 @@ def test_two_contexts_at_once(ctx):
         torch.cuda.synchronize()
         for k in range(2):
             assert all(torch.equal(o, work[k][4]) for o in outs[k])
+
+@pytest.mark.parametrize("n", [1500, 20000])
+@pytest.mark.parametrize("v", [1, 2, 3, 7, 20])
+def test_sort_of_few_different_ids(ctx, n, v):
+    """Fewer digits than a warp has lanes in the sort."""
+    from orda_b200.device import embedding_grad_device
+
+    gen = rng(n + v)
+    for h in (24, 2056):
+        g, ids = rand((n, h), BF16, gen), torch.randint(0, v, (n,), generator=gen, device="cuda")
+        got = embedding_grad_device(ctx, g, ids, v, dtype=F32)
+        acc = got.clone()
+        embedding_grad_device(ctx, g, ids, v, out=acc, accumulate=True)
+        finish(ctx)
+        check_grad(got, *grad_formula(g, ids, v, 1.0))
+        check_grad(acc, *grad_formula(g, ids, v, 1.0, old=got))
