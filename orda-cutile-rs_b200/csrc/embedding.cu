@@ -617,8 +617,10 @@ void by_types(int in_bf16, int out_bf16, int vec, const F& f) {
   auto go = [&](auto ti, auto to) {
     using TI = decltype(ti);
     using TO = decltype(to);
-    if (vec == 8) f.template operator()<TI, TO, 8>();
-    else if (vec == 4) f.template operator()<TI, TO, 4>();
+    if constexpr (sizeof(TI) == 2) {  // 16 bytes of the first matrix at most (pick_vec)
+      if (vec == 8) return f.template operator()<TI, TO, 8>();
+    }
+    if (vec == 4) f.template operator()<TI, TO, 4>();
     else if (vec == 2) f.template operator()<TI, TO, 2>();
     else f.template operator()<TI, TO, 1>();
   };
