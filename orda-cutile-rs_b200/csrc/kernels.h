@@ -94,7 +94,7 @@ struct EpiArgs {
   float2* ce_rec = nullptr;          // CeStats: [rows][ce_rec_ld] records of the parts, from column 0 of this launch
   float* ce_sx = nullptr;            // CeStats, optional: [rows][ce_rec_ld] sums of the logits
   long long ce_rec_ld = 0;
-  const float4* ce_const = nullptr;  // CeGrad: per row constants (CeRowConst)
+  const float4* ce_const = nullptr;  // CeGrad: per row (-lse log2 e, label as int bits, a / V, the label's gradient)
 };
 
 struct GemmDesc {

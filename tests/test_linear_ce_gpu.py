@@ -785,3 +785,133 @@ def test_phase_timing_and_capture(ctx):
         twice = own.phase_times()
         assert all(twice[k][1] == 2 * n and twice[k][0] >= ms for k, (ms, n) in once.items())
         del graph
+
+
+def test_loss_of_certain_tokens(ctx):
+    """Rows that are all but certain: the loss is the sum of the other entries' e^(z - z_label), each off by its
+    logit's error (2 H 2^-24 sum |h w| = 8e-4 at H = 64 here) and an exponential's, none by a cancellation."""
+    h, v = 64, 1200
+    gen = torch.Generator(device="cuda").manual_seed(2)
+    w = (torch.randn(v, h, generator=gen, device="cuda") * 0.1).bfloat16()
+    w[:, 0] = -1.0
+    w[-1, 0] = 1.0
+    for bt in (4, 200):
+        x = torch.zeros(bt, h, device="cuda", dtype=torch.bfloat16)
+        x[:, 0] = torch.linspace(6, 40, bt, device="cuda").to(torch.bfloat16)
+        x[:, 1:] = (torch.randn(bt, h - 1, generator=gen, device="cuda") * 0.1).bfloat16()
+        labels = torch.full((bt,), v - 1, device="cuda")
+        z = x.double() @ w.double().T
+        want = torch.log1p(torch.exp(z[:, :-1] - z[:, -1:]).sum(1))
+        ez = 2 * h * 2.0**-24 * (x.double().abs() @ w.double().abs().T).amax(1)
+        # ... and 2^-24 of the exponent z log2 e, at the row's reference and in the sum
+        tol = (2 * ez + 4 * 2.0**-24 * z.abs().amax(1) * 2 + 2.0**-20) * want
+        for piece in (0, 1):
+            r = call(ctx, x, w, labels, piece_bytes=piece)
+            assert float(want.min()) > 1e-32 and float(want.max()) < 1e-1
+            assert torch.all((r.nll.double() - want).abs() <= tol), float(((r.nll.double() - want).abs() / want).max())
+
+
+@pytest.mark.parametrize("piece_bytes", [0, 1])
+@pytest.mark.parametrize("bt", [300, 1100])
+def test_far_labels_of_many_tokens(ctx, piece_bytes, bt):
+    """As test_far_labels, with the logits of more tokens than the few-row kernel takes."""
+    h, v = 64, 1200
+    gen = torch.Generator(device="cuda").manual_seed(2)
+    w = torch.zeros(v, h, device="cuda")
+    w[:, 0] = torch.linspace(-1, 1, v, device="cuda")
+    w[:, 1:] = torch.randn(v, h - 1, generator=gen, device="cuda") * 0.1
+    w = w.bfloat16()
+    x = torch.randn(bt, h, generator=gen, device="cuda")
+    x[:, 0] = torch.linspace(-150, 150, bt, device="cuda")
+    x = x.bfloat16()
+    labels = torch.randint(0, v, (bt,), generator=gen, device="cuda")
+    labels[::3] = 0
+    labels[1::3] = v - 1
+    f = formula(x, w, labels)
+    check(call(ctx, x, w, labels, grad_dtype=torch.bfloat16, piece_bytes=piece_bytes), f)
+    check(call(ctx, x, w, labels, need_grad_hidden=False, need_grad_weight=False), f)
+    f = formula(x, w, labels, 0.1)
+    check(call(ctx, x, w, labels, 0.1, grad_dtype=torch.bfloat16, piece_bytes=piece_bytes), f)
+
+
+@pytest.mark.parametrize("piece_bytes", [0, 1])
+def test_lowest_value_logits_of_many_tokens(ctx, piece_bytes):
+    x, w, labels = make(300, 64, 640, seed=6)
+    x[:, 0] = 1.0
+    w[:, 0] = 0.0
+    w[128:384, 0] = -3.0e38
+    labels[(labels >= 128) & (labels < 384)] = 5
+    r = call(ctx, x, w, labels, grad_dtype=torch.bfloat16, piece_bytes=piece_bytes)
+    keep = torch.cat([torch.arange(128), torch.arange(384, 640)]).cuda()
+    sub = torch.full((640,), 0, device="cuda")
+    sub[keep] = torch.arange(len(keep), device="cuda")
+    f = formula(x, w[keep].contiguous(), sub[labels])
+    assert torch.all((r.nll.double() - f["nll"]).abs() <= f["row_tol"])
+    assert not r.grad_weight[128:384].any()
+    assert ((r.grad_weight[keep].double() - f["dw"]).norm() / f["dw"].norm()) < 5e-3
+
+
+@pytest.mark.parametrize("piece_bytes", [0, 1])
+def test_nan_of_a_live_row_of_many_shows(ctx, piece_bytes):
+    x, w, labels = make(300, 64, 1300)
+    x[133, 5] = float("nan")
+    r = call(ctx, x, w, labels, piece_bytes=piece_bytes)
+    assert torch.isnan(r.loss) and torch.isnan(r.nll[133]) and torch.isnan(r.grad_hidden[133]).all()
+    rest = [i for i in range(300) if i != 133]
+    assert torch.isfinite(r.nll[rest]).all() and torch.isfinite(r.grad_hidden[rest]).all()
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_wide_weight_gradient_tiles(ctx, dtype):
+    """8200 tokens: a K loop long enough for the 256 x 512 tiles of grad_weight. Relative L2 as in
+    test_larger_products."""
+    x, w, labels = make(8200, 512, 38005, seed=23, ignored=0.1)
+    r = call(ctx, x, w, labels, grad_dtype=dtype)
+    live = labels != -100
+    n = int(live.sum())
+    wd, dw = w.double(), torch.zeros(38005, 512, dtype=torch.float64, device="cuda")
+    for rows in torch.arange(8200, device="cuda").split(2050):
+        xd = torch.where(live[rows, None], x[rows].double(), 0.0)
+        d = torch.softmax(xd @ wd.T, 1)
+        d[torch.arange(len(rows), device="cuda"), torch.where(live[rows], labels[rows], 0)] -= 1
+        d *= live[rows, None] / n
+        dw += d.T @ xd
+        dh = d @ wd
+        assert (r.grad_hidden[rows].double() - dh).norm() < 1.6e-3 * math.sqrt(3) * dh.norm()
+    assert (r.grad_weight.double() - dw).norm() < 1.6e-3 * math.sqrt(3) * dw.norm()
+
+
+@pytest.mark.parametrize("env", [{"ORDA_GEMM_CTA_PAIR": "0"}, {"ORDA_GEMM_WIDE": "2"}])
+@pytest.mark.parametrize("bt,h,v", [(300, 520, 4099), (260, 2200, 1500)])
+def test_other_tiles(ctx, monkeypatch, env, bt, h, v):
+    """Single-CTA tiles, and 256 x 512 ones wherever they can be; K in one part and in two."""
+    for k, val in env.items():
+        monkeypatch.setenv(k, val)
+    x, w, labels = make(bt, h, v, seed=25, ignored=0.1)
+    for a, piece in ((0.0, 0), (0.1, bt * 1024 * 2)):
+        f = formula(x, w, labels, a)
+        for dtype in (torch.float32, torch.bfloat16):
+            check(call(ctx, x, w, labels, a, grad_dtype=dtype, piece_bytes=piece), f)
+        check(call(ctx, x, w, labels, a, need_grad_hidden=False, need_grad_weight=False), f)
+
+
+@pytest.mark.parametrize("bt", [70, 300])
+@pytest.mark.parametrize("h", [2048, 2056, 4096, 4160])
+def test_long_rows(ctx, bt, h):
+    """K of the logits in one, two and three parts, with labels far above, far below and among the others."""
+    x, w, labels = make(bt, h, 1201, seed=h, ignored=0.1)
+    w[:, 0] = 0.0
+    w[:600, 0] = 1.0
+    x[:, 0] = torch.linspace(-100, 100, bt, device="cuda").to(torch.bfloat16)
+    # In the part where the two groups of entries meet the fixed point holds a probability as zero that is at most
+    # 2^-64 of its reference's, the label's or one of the part's: at most 2^-64. Elsewhere such probabilities count.
+    live = labels != -100
+    p = torch.where(live[:, None], torch.softmax(x.double() @ w.double().T, 1), 0.0)
+    p = torch.where(p <= 2.0**-64, p, 0.0)[:, 576:640] / int(live.sum())
+    for a in (0.0, 0.1):
+        f = formula(x, w, labels, a)
+        f["dh_tol"] += p @ w[576:640].double().abs()
+        f["dw_tol"][576:640] += p.T @ x.double().abs()
+        for piece in (0, 1):
+            check(call(ctx, x, w, labels, a, piece_bytes=piece), f)
+        check(call(ctx, x, w, labels, a, need_grad_hidden=False, need_grad_weight=False), f)
