@@ -352,8 +352,8 @@ constexpr int kEpiCeParts = 72;  // CeStats (+ 1, + 2 as there) of K loops longe
 // out over the vocabulary. The cross entropy's logits therefore sum K in even
 // parts of at most 2048, each from zero, and the epilogue adds the parts in fp32.
 // Losses at H = 4096 against 64 bits: 5e-7 (1e-6 in one part, 2.5e-7 in parts of
-// 1024; fp32 torch 6e-7). Each further part costs the products' time: 2048 x 4096
-// x 32000 without gradients 362 us in one part, 377 in two, 388 in four.
+// 1024; fp32 torch 6e-7). A further part costs the products' time: 2048 x 4096 x
+// 32000 without gradients 536k SM cycles in one part, 562k in two, 593k in four.
 constexpr int kCeKBlocks = 2048 / BK;
 __host__ __device__ constexpr int ce_k_parts(int kblocks) { return (kblocks + kCeKBlocks - 1) / kCeKBlocks; }
 // First K block of part i.
@@ -544,10 +544,11 @@ __device__ __forceinline__ void ce_parts_epilogue(const KParams& p, const CUtens
   if (colh >= p.N) return;
   const long long lab_rel = static_cast<long long>(__float_as_int(row_c.y)) - p.e.ce_v0 - colh;
   const int lab = lab_rel >= 0 && lab_rel < kCePartCols ? static_cast<int>(lab_rel) : -1;
-  float d = 0.f, sx = 0.f;
+  float d, sx;
   float ref2 = row_c.x;
-#pragma unroll 1
-  for (int again = 0; again < 2; ++again) {
+  auto pass = [&]() {
+    d = 0.f;
+    sx = 0.f;
 #pragma unroll
     for (int c = 0; c < 2; ++c) {
       const int nvalid = p.N - (colh + c * 32);
@@ -579,8 +580,10 @@ __device__ __forceinline__ void ce_parts_epilogue(const KParams& p, const CUtens
         stage16_send(buf, lane, map, col, row0, row0 < p.M && col < p.N, pol_c);
       }
     }
-    const bool out_of_range = !(d >= kCeSumLow && d < kCeSumHigh);
-    if (again == 1 || !__any_sync(0xffffffffu, out_of_range)) break;
+  };
+  pass();
+  const bool out_of_range = !(d >= kCeSumLow && d < kCeSumHigh);
+  if (__any_sync(0xffffffffu, out_of_range)) {
     // against the part's own maximum, as in ce_epilogue
     float m = -INFINITY;
 #pragma unroll
@@ -592,10 +595,9 @@ __device__ __forceinline__ void ce_parts_epilogue(const KParams& p, const CUtens
     }
     __syncwarp();
     if (out_of_range && m * LOG2E > -INFINITY) ref2 = m * LOG2E;
-    d = 0.f;
-    sx = 0.f;
     if (STORE && lane == 0) bulk_wait_all();
     __syncwarp();
+    pass();
   }
   if (row_ok) {
     const long long ri = grow * p.e.ce_rec_ld + part;
