@@ -474,8 +474,8 @@ ORDA_API int orda_vocab_backward_device(OrdaContext* ctx, const OrdaDeviceMat* s
  *
  * hidden [BT, H] and weight [V, H] as in orda_distillation_loss_device. The
  * products take bf16 operands: gradients carry the rounding of the logit
- * gradients to bf16 (relative L2 about 2e-3) whatever their type; losses come
- * from fp32 sums of the fp32 products. Enqueued on `stream` without host
+ * gradients to bf16 (relative L2 1.0e-3 to 1.5e-3) whatever their type; losses
+ * come from fp32 sums of the fp32 products. Enqueued on `stream` without host
  * synchronisation; labels out of range are reported by orda_context_check.
  * Under stream capture the context must hold the workspace already (make the
  * same call once before); the graph may be replayed until the context is

@@ -1372,8 +1372,10 @@ bool use_wide(const GemmDesc& d, long long k_blocks, long long m_blocks, int num
 // entries) and the tokens are its N, so the tensor cores' time follows the
 // tokens: with the tokens as a 256-row tile they keep it to 9 TB/s at best, and
 // half of the ring holds rows that are zero. Here a CTA has 96 to 160 KB of W in
-// flight: one token at H = 4096, V = 131072 takes 172 us (6.2 TB/s; 186 us as a
-// 256 x 256 tile), 77 tokens at H = 2048, V = 128256 98 us (102 us). W comes in
+// flight. Calls without gradients: one token at H = 4096, V = 131072 takes 176 us
+// (6.1 TB/s; 257 us as 256 x 256 tiles); 33, 64, 96 and 128 tokens 180, 182, 194 and
+// 198 us (209, 211, 217 and 217 us); at H = 2048, V = 128256 96, 97, 102 and 105 us (104,
+// 106, 108 and 110 us). 129 tokens, as tiles, take 218 and 111 us. W comes in
 // boxes of 128 rows: boxes of 32 rows, which would let the CTAs' shares differ by
 // less, took 233 us for the one token.
 //   * Tiles go round the CTAs, so at any time neighbouring tiles are read.
