@@ -1261,7 +1261,8 @@ int check_status(OrdaContext* ctx, char* err, size_t len) {
   if (e != cudaSuccess) return cuda_fail(e, "status read", err, len);
   // one report a call; a word is cleared with its own report, so that what else
   // happened is reported by the next calls. Word 0 stays until the next loss call
-  // clears it, marked as reported.
+  // clears it, marked as reported unless that has happened already: kernels give
+  // their waits up while it is set.
   auto put = [&](int word, int value) {
     return cudaMemcpy(ctx->d_words + word, &value, sizeof value, cudaMemcpyHostToDevice);
   };
@@ -1278,7 +1279,9 @@ int check_status(OrdaContext* ctx, char* err, size_t len) {
     if ((e = put(6, DEV_OK)) != cudaSuccess) return cuda_fail(e, "status write", err, len);
     status = words[6];
   } else if (status != DEV_OK) {
-    if ((e = put(0, status | kStatusReported)) != cudaSuccess) return cuda_fail(e, "status write", err, len);
+    if ((e = launch_mark_reported(ctx->d_words, status, ctx->last_stream)) != cudaSuccess ||
+        (e = cudaStreamSynchronize(ctx->last_stream)) != cudaSuccess)
+      return cuda_fail(e, "status write", err, len);
   }
   if (status == DEV_LABEL_RANGE) {
     set_error(err, len, "a label is out of range [0, V) and != ignore_index (device label check)");
@@ -1632,6 +1635,7 @@ void orda_context_destroy(OrdaContext* ctx) {
 
 int orda_context_check(OrdaContext* ctx, char* err, size_t err_len) {
   if (!ctx) return ORDA_ERR_INVALID;
+  std::lock_guard<std::mutex> lock(ctx->mu);
   cudaSetDevice(ctx->device);
   return check_status(ctx, err, err_len);
 }

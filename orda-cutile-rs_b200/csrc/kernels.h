@@ -174,6 +174,8 @@ struct CeArgs {
 };
 // Labels, reference logits and the copy of the hidden states with ignored rows cleared.
 cudaError_t launch_ce_prep(const CeArgs& a, cudaStream_t stream);
+// Marks the status word as reported if it still holds `status`.
+cudaError_t launch_mark_reported(int* word, int status, cudaStream_t stream);
 // Records -> nll, lse, the gradient's row constants and the loss; and with a
 // piece the kept 16-bit logits of its n first columns -> bf16 logit gradients.
 cudaError_t launch_ce_rows(const CeArgs& a, uint16_t* piece, long long ld, long long n, cudaStream_t stream);

@@ -125,6 +125,8 @@ __global__ void __launch_bounds__(kPrepThreads) ce_prep_kernel(const CeArgs a) {
   }
 }
 
+__global__ void mark_reported_kernel(int* word, int status) { atomicCAS(word, status, status | kStatusReported); }
+
 // Sum of 2^(r_i) * d_i with a running maximum of the references r_i.
 struct Acc {
   double d;
@@ -394,6 +396,11 @@ __global__ void __launch_bounds__(256)
 
 cudaError_t launch_ce_prep(const CeArgs& a, cudaStream_t stream) {
   ce_prep_kernel<<<static_cast<unsigned>(a.clean_rows), kPrepThreads, 0, stream>>>(a);
+  return cudaGetLastError();
+}
+
+cudaError_t launch_mark_reported(int* word, int status, cudaStream_t stream) {
+  mark_reported_kernel<<<1, 1, 0, stream>>>(word, status);
   return cudaGetLastError();
 }
 

@@ -915,3 +915,45 @@ def test_long_rows(ctx, bt, h):
         for piece in (0, 1):
             check(call(ctx, x, w, labels, a, piece_bytes=piece), f)
         check(call(ctx, x, w, labels, a, need_grad_hidden=False, need_grad_weight=False), f)
+
+
+def test_checks_from_another_thread(ctx):
+    """check() beside calls of the same context: every bad call is heard of, the good calls' results stand."""
+    import threading
+
+    import orda_b200 as ob
+    from orda_b200.device import DeviceContext, distillation_loss_device, linear_cross_entropy_device
+
+    x, w, labels = make(150, 64, 900, seed=26)
+    bad = labels.clone()
+    bad[3] = 900
+    opts = ob.LossOptions(kd_weight=0.0, teacher_ce_weight=0.0)
+    with DeviceContext(0) as own:
+        want = call(own, x, w, labels)
+        stop, heard, other = threading.Event(), [], []
+
+        def listen():
+            while not stop.is_set():
+                try:
+                    own.check()
+                except ob.OrdaError as e:
+                    (heard if "label is out of range" in str(e) else other).append(str(e))
+
+        thread = threading.Thread(target=listen)
+        thread.start()
+        results = []
+        for i in range(60):
+            if i % 10 == 0:
+                distillation_loss_device(own, x, w, bad, ob.TeacherMode.Tied, teacher_hidden=x, opts=opts)
+            results.append(linear_cross_entropy_device(own, x, w, labels))
+        torch.cuda.synchronize()
+        stop.set()
+        thread.join()
+        try:
+            own.check()
+        except ob.OrdaError as e:
+            heard.append(str(e))
+        own.check()
+        assert heard and not other
+        for r in results:
+            assert torch.equal(r.grad_weight, want.grad_weight) and float(r.loss) == float(want.loss)
